@@ -291,6 +291,65 @@ int32_t hq_tol_min_tiles(int32_t tiles);
  * tokens a launch) or the prompt tiles.  Every path gives the same numbers.  Host-only: no device is touched. */
 int32_t hq_job_path(int32_t kind, int32_t n, int32_t count, int64_t frame, int64_t sframe);
 
+/* ---- a layer's operators between its products (no counterpart among the reference's kernels) --------------------- */
+
+/* The norm between two products, with the activations it readies, in one launch: for `count` tokens (x, r x_stride bytes
+ * apart, d d_stride, y y_stride; all rows of n float32)
+ *   r = x + d  (float32; d NULL: r = x)       y = r w / sqrt(mean(r^2) + eps)  (in 64 bits, rounded once)
+ * and y quantized into xq + t frame and xs + t frame as `ready` says: quantize_x at bias 64 (int8, int6) or 0, with
+ * interleave's planes and sums (ternary, binary) or sums_x's sums (llama.cpp's blocks), to the bit what those give for y.
+ * d, r, y and xq (with xs) may be NULL: r then is not stored (it has to be where d is given), y not stored, or nothing
+ * readied.  r may be x; nothing else may overlap.  n a multiple of 32, 128 (planes) or 256 (sums); x, d, w, r, y and their
+ * strides 16-byte aligned, frame a multiple of 16, xq and xs 4-byte aligned; eps >= 0. */
+enum { HQ_READY_BIASED = 0, HQ_READY_PLAIN = 1, HQ_READY_PLANES = 2, HQ_READY_SUMS = 3 };
+int32_t hq_norm_ready_ex(void *xq, void *xs, void *y, void *r, const void *x, const void *d, const void *w, int32_t n,
+                         float eps, int32_t ready, int32_t count, int32_t frame, int32_t x_stride, int32_t d_stride,
+                         int32_t y_stride, void *stream);
+
+/* A layer's paged key/value cache: `pages` pages of `page` positions (16, 32, 64, 128 or 256) of `heads` heads of `dim`
+ * values (a multiple of 16 up to 256).
+ *   k  [pages][heads][page][dim]   v  [pages][heads][dim][page]   the elements, int8 or float16
+ *   ks [pages][heads][page]        vs [pages][heads][page]        float32: a vector's values are its elements times this
+ * All 16-byte aligned device memory of the caller's, which needs no initial value. */
+enum { HQ_CACHE_INT8 = 0, HQ_CACHE_F16 = 1 };
+typedef struct hq_cache {
+  void *k, *v, *ks, *vs;
+  int32_t form, pages, page, heads, dim;
+} hq_cache;
+/* A batch of new tokens: `sequences` sequences, sequence s's new tokens the rows starts[s] .. starts[s + 1] - 1 of the
+ * call's `tokens` rows (starts: sequences + 1 numbers, rising; a sequence may have none), and its last `starts[s + 1] -
+ * starts[s]` of lengths[s] positions; position p is on page table[s width + p / page].  starts, lengths and table are
+ * device memory and are read when the call's kernels run (a captured call can be replayed with other contents).  An entry
+ * of the table outside 0 .. pages - 1 is no page: what would be written there is left out, what is there reads as zeros
+ * and is not attended to, as is a position past the table's end or before position 0.  Rows that no sequence has are left
+ * alone.  longest: no sequence has more new tokens (0: not known), a hint: the results do not depend on it. */
+typedef struct hq_batch {
+  const void *starts, *lengths, *table;
+  int32_t sequences, tokens, longest, width;
+} hq_batch;
+/* The new tokens' keys and values (token t's head h at k + t k_stride + 4 h dim, float32; 16-byte aligned, strides in bytes)
+ * quantized into their pages.  int8: scale = largest |x| / 127, element = x (1 / scale) rounded to even, as quantize_x does
+ * over a group; float16: scale = 2^(e - 14) where 2^e <= largest |x| < 2^(e + 1), element = x / scale.  A scale below
+ * 2^-100 is stored as 0 with zeros; a vector with an infinity or NaN as scale NaN with zeros: all of it reads as NaN. */
+int32_t hq_cache_write_ex(const hq_cache *cache, const hq_batch *batch, const void *k, const void *v, int32_t k_stride,
+                          int32_t v_stride, void *stream);
+/* The keys and values at the batch's tokens' positions as float32 (element times scale, one rounding), laid out as
+ * hq_cache_write_ex's */
+int32_t hq_cache_read_ex(const hq_cache *cache, const hq_batch *batch, void *k, void *v, int32_t k_stride, int32_t v_stride,
+                         void *stream);
+/* Attention of the batch's tokens, whose keys and values are in the cache: token t's query head g (q + t q_stride + 4 g dim,
+ * float32) over the head g / (heads / cache heads) of the cache, at the positions up to its own (the last `window` of them,
+ * its own among them, where window > 0):
+ *   out = sum_j e^(s_j) v_j / sum_j e^(s_j)     s_j = scale q.k_j    (cap > 0: cap tanh(scale q.k_j / cap))
+ * and zeros where no position is seen; laid out as q.  To float32's accuracy: sums in float32, products of float32 values
+ * held to 22 bits.  Results do not depend on what pages hold at positions that nobody sees, but for a page's positions
+ * below lengths[s], which the cache's writes have filled.  work: hq_attention_work_bytes bytes (-1: bad arguments), 256-byte
+ * aligned, of any content; calls that share it on one stream follow each other, on two they race.  scale > 0. */
+int64_t hq_attention_work_bytes(const hq_cache *cache, const hq_batch *batch, int32_t heads);
+int32_t hq_attention_ex(void *out, const void *q, int32_t heads, int32_t out_stride, int32_t q_stride,
+                        const hq_cache *cache, const hq_batch *batch, float scale, int32_t window, float cap, void *work,
+                        int64_t work_bytes, void *stream);
+
 /* The ceilings the kernels are measured against (no counterpart on this path: the reference's CPU ceiling loops,
  * kernels/ceilings.ts:12-25 and ceilings_relaxed.ts:34-52, are its model).  hq_ceiling_read reads every byte of
  * [p, p + bytes) once (bytes a multiple of 16): time it for the achievable HBM read bandwidth of a buffer past the

@@ -9,6 +9,8 @@ side above that ABI, mirroring the reference's own interface for the path:
     device address.  A call that the library refuses raises HQError (the library keeps the reason).
   * `jobs` mirrors src/runtime/jobs.ts: the kinds of jobs (WORK), the packings (PACKED), their activations'
     preparation (ready), and a phase of jobs run in one call (hq_phase).
+  * `cache` holds what the operators between the products take: the descriptions of a paged key/value cache and of a
+    batch of new tokens (hq_cache, hq_batch), and how the norm readies activations (READY).
 
 There is no CPU fallback: without libhq.so (or without a gfx950 GPU, for the calls that compute) every call
 raises.
@@ -16,6 +18,7 @@ raises.
 import ctypes
 import os
 
+from . import cache  # (the paged cache's and a batch's descriptions)
 from . import jobs  # noqa: F401  (the jobs.ts mirror)
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -33,6 +36,7 @@ class HQError(RuntimeError):
 
 
 p, i32, f32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_float
+pcache, pbatch = ctypes.POINTER(cache.Cache), ctypes.POINTER(cache.Batch)
 
 # the reference's kernels, by name: src/runtime/jobs.ts:101-140 (Arguments), src/python/engine/kernels.py:42-51
 REFERENCE_SIGNATURES = {
@@ -110,6 +114,11 @@ OWN_SIGNATURES = {
     "hq_tol_work_bytes": ([i32, i32], ctypes.c_int64),
     "hq_tol_min_tiles": ([i32], i32),
     "hq_matmul_q8r_tile_tol_ex": ([p, p, p, p, p, i32, i32, i32, i32, i32, i32, p, ctypes.c_int64, p], i32),
+    "hq_norm_ready_ex": ([p, p, p, p, p, p, p, i32, f32, i32, i32, i32, i32, i32, i32, p], i32),
+    "hq_cache_write_ex": ([pcache, pbatch, p, p, i32, i32, p], i32),
+    "hq_cache_read_ex": ([pcache, pbatch, p, p, i32, i32, p], i32),
+    "hq_attention_work_bytes": ([pcache, pbatch, i32], ctypes.c_int64),
+    "hq_attention_ex": ([p, p, i32, i32, i32, pcache, pbatch, f32, i32, f32, p, ctypes.c_int64, p], i32),
     "hq_ceiling_read": ([p, ctypes.c_int64, p, p], i32),
     "hq_ceiling_mfma": ([i32, i32, p, p], i32),
     "hq_ceiling_epilogue": ([i32, i32, i32, p, p], i32),

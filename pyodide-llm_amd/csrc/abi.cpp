@@ -415,6 +415,59 @@ int32_t group_of(int32_t packing, int32_t dim) {
   while (size > 1 && dim % size) size >>= 1;
   return size;
 }
+// the cache and the batch of a call, checked (memory: whether their device pointers are)
+int32_t paged_of(const char *who, const hq_cache *cache, const hq_batch *batch, hq::Cache &c, hq::Batch &b,
+                 bool memory = true) {
+  if (!cache || !batch) return fail(HQ_ERR_NULL, "%s: cache or batch NULL", who);
+  if (cache->form != HQ_CACHE_INT8 && cache->form != HQ_CACHE_F16)
+    return fail(HQ_ERR_ARGUMENT, "%s: form %d is neither int8 nor float16", who, cache->form);
+  int32_t shift = 4;
+  while (shift < 8 && (1 << shift) != cache->page) shift++;
+  if ((1 << shift) != cache->page)
+    return fail(HQ_ERR_ARGUMENT, "%s: page = %d is none of 16, 32, 64, 128, 256", who, cache->page);
+  if (cache->dim <= 0 || cache->dim % 16 || cache->dim > 256)
+    return fail(HQ_ERR_ARGUMENT, "%s: dim = %d is not a multiple of 16 up to 256", who, cache->dim);
+  if (cache->heads <= 0 || cache->heads > 1024) return fail(HQ_ERR_ARGUMENT, "%s: heads = %d", who, cache->heads);
+  if (cache->pages < 0) return fail(HQ_ERR_ARGUMENT, "%s: pages = %d", who, cache->pages);
+  if (batch->sequences < 0 || batch->tokens < 0 || batch->longest < 0 || batch->width < 0)
+    return fail(HQ_ERR_ARGUMENT, "%s: sequences = %d, tokens = %d, longest = %d, width = %d", who, batch->sequences,
+                batch->tokens, batch->longest, batch->width);
+  if (((int64_t)batch->width << shift) > INT32_MAX)
+    return fail(HQ_ERR_ARGUMENT, "%s: a table of %d pages of %d positions", who, batch->width, cache->page);
+  if (batch->tokens > (1 << 24)) return fail(HQ_ERR_ARGUMENT, "%s: tokens = %d", who, batch->tokens);
+  c = hq::Cache{(char *)cache->k, (char *)cache->v, (float *)cache->ks, (float *)cache->vs, cache->form == HQ_CACHE_F16,
+                cache->pages, shift, cache->heads, cache->dim};
+  const int32_t longest = batch->longest && batch->longest < batch->tokens ? batch->longest : batch->tokens;
+  b = hq::Batch{(const int32_t *)batch->starts, (const int32_t *)batch->lengths, (const int32_t *)batch->table,
+                batch->sequences, batch->tokens, longest, batch->width};
+  if (!memory || b.tokens == 0 || b.sequences == 0) return HQ_OK;
+  if (!b.starts || !b.lengths || (!b.table && b.width)) return fail(HQ_ERR_NULL, "%s: starts, lengths or table NULL", who);
+  if (!aligned(b.starts, 4) || !aligned(b.lengths, 4) || !aligned(b.table, 4))
+    return fail(HQ_ERR_ALIGNMENT, "%s: starts, lengths or table not 4-byte aligned", who);
+  if (c.pages && (!c.k || !c.v || !c.ks || !c.vs)) return fail(HQ_ERR_NULL, "%s: the cache's k, v, ks or vs NULL", who);
+  if (!aligned(c.k, 16) || !aligned(c.v, 16) || !aligned(c.ks, 16) || !aligned(c.vs, 16))
+    return fail(HQ_ERR_ALIGNMENT, "%s: the cache's k, v, ks or vs not 16-byte aligned", who);
+  return HQ_OK;
+}
+
+// the float32 rows of a batch's tokens
+int32_t rows_of(const char *who, const hq::Batch &b, const void *p, int32_t stride, int64_t values) {
+  if (b.tokens == 0 || b.sequences == 0) return HQ_OK;
+  if (!p) return fail(HQ_ERR_NULL, "%s: a token row's pointer is NULL", who);
+  if (!aligned(p, 16)) return fail(HQ_ERR_ALIGNMENT, "%s: a token row's pointer is not 16-byte aligned", who);
+  if (b.tokens > 1 && (stride % 16 || stride < 0))
+    return fail(HQ_ERR_ALIGNMENT, "%s: a token stride of %d is not a multiple of 16", who, stride);
+  if (b.tokens > 1 && stride < 4 * values)
+    return fail(HQ_ERR_ARGUMENT, "%s: a token stride of %d, a token's row takes %lld", who, stride, (long long)(4 * values));
+  return HQ_OK;
+}
+
+int32_t heads_of(const char *who, const hq::Cache &c, const hq::Batch &b, int32_t heads) {
+  if (heads <= 0 || heads % c.heads || heads > 1024)
+    return fail(HQ_ERR_ARGUMENT, "%s: %d query heads over %d of keys and values", who, heads, c.heads);
+  return HQ_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -716,6 +769,96 @@ int32_t hq_binary_x_ex(void *out, void *xs, const void *x, int32_t n, void *bad,
   return hip_status(hq::launch_binary_x((uint8_t *)out, (float *)xs, (const float *)x, n / 128, (int32_t *)bad,
                                         stream_of(stream)),
                     "binary_x");
+}
+
+// ---- a layer's operators between its products ---------------------------------------------------------------------
+int32_t hq_norm_ready_ex(void *xq, void *xs, void *y, void *r, const void *x, const void *d, const void *w, int32_t n,
+                         float eps, int32_t ready, int32_t count, int32_t frame, int32_t x_stride, int32_t d_stride,
+                         int32_t y_stride, void *stream) {
+  g_error = HQ_OK;
+  if (ready < HQ_READY_BIASED || ready > HQ_READY_SUMS) return fail(HQ_ERR_ARGUMENT, "norm_ready: ready = %d", ready);
+  const int32_t unit = ready == HQ_READY_PLANES ? 128 : ready == HQ_READY_SUMS ? 256 : 32;
+  if (n <= 0 || n % unit) return fail(HQ_ERR_ARGUMENT, "norm_ready: n = %d is not a positive multiple of %d", n, unit);
+  if (!(eps >= 0.0f) || std::isinf(eps)) return fail(HQ_ERR_ARGUMENT, "norm_ready: eps = %g", (double)eps);
+  if (count < 0) return fail(HQ_ERR_ARGUMENT, "norm_ready: count = %d", count);
+  if (count == 0) return HQ_OK;
+  if (!x || !w) return fail(HQ_ERR_NULL, "norm_ready: x or w NULL");
+  if (!y && !xq) return fail(HQ_ERR_NULL, "norm_ready: y and xq both NULL");
+  if (d && !r) return fail(HQ_ERR_NULL, "norm_ready: d without r");
+  if (xq && !xs) return fail(HQ_ERR_NULL, "norm_ready: xq without xs");
+  if (!aligned(x, 16) || !aligned(w, 16) || !aligned(d, 16) || !aligned(r, 16) || !aligned(y, 16))
+    return fail(HQ_ERR_ALIGNMENT, "norm_ready: x, d, w, r or y not 16-byte aligned");
+  if (xq && (!aligned(xq, 4) || !aligned(xs, 4))) return fail(HQ_ERR_ALIGNMENT, "norm_ready: xq or xs not 4-byte aligned");
+  if (count > 1) {
+    if (x_stride < 0 || x_stride % 16 || (d && (d_stride < 0 || d_stride % 16)) || (y && (y_stride < 0 || y_stride % 16)))
+      return fail(HQ_ERR_ALIGNMENT, "norm_ready: a token stride is not a multiple of 16");
+    if (xq && (frame < 0 || frame % 16)) return fail(HQ_ERR_ALIGNMENT, "norm_ready: frame = %d is not a multiple of 16", frame);
+  }
+  if (int32_t st = ensure_device()) return st;
+  const hq::NormRows a{(char *)xq, (char *)xs, (char *)y, (char *)r, (const char *)x, (const char *)d, (const char *)w,
+                       frame, x_stride, d_stride, y_stride, count};
+  const hq::Ready mode = ready == HQ_READY_PLANES ? hq::kReadyPlanes : ready == HQ_READY_SUMS ? hq::kReadySums : hq::kReadyBytes;
+  return hip_status(hq::launch_norm(mode, a, n, eps, ready == HQ_READY_BIASED ? 64 : 0, stream_of(stream)), "norm_ready");
+}
+
+int32_t hq_cache_write_ex(const hq_cache *cache, const hq_batch *batch, const void *k, const void *v, int32_t k_stride,
+                          int32_t v_stride, void *stream) {
+  g_error = HQ_OK;
+  hq::Cache c;
+  hq::Batch b;
+  if (int32_t st = paged_of("cache_write", cache, batch, c, b)) return st;
+  if (int32_t st = rows_of("cache_write", b, k, k_stride, (int64_t)c.heads * c.dim)) return st;
+  if (int32_t st = rows_of("cache_write", b, v, v_stride, (int64_t)c.heads * c.dim)) return st;
+  if (b.tokens == 0 || b.sequences == 0) return HQ_OK;
+  if (int32_t st = ensure_device()) return st;
+  return hip_status(hq::launch_cache_write(c, b, (const char *)k, (const char *)v, k_stride, v_stride, stream_of(stream)),
+                    "cache_write");
+}
+
+int32_t hq_cache_read_ex(const hq_cache *cache, const hq_batch *batch, void *k, void *v, int32_t k_stride, int32_t v_stride,
+                         void *stream) {
+  g_error = HQ_OK;
+  hq::Cache c;
+  hq::Batch b;
+  if (int32_t st = paged_of("cache_read", cache, batch, c, b)) return st;
+  if (int32_t st = rows_of("cache_read", b, k, k_stride, (int64_t)c.heads * c.dim)) return st;
+  if (int32_t st = rows_of("cache_read", b, v, v_stride, (int64_t)c.heads * c.dim)) return st;
+  if (b.tokens == 0 || b.sequences == 0) return HQ_OK;
+  if (int32_t st = ensure_device()) return st;
+  return hip_status(hq::launch_cache_read(c, b, (char *)k, (char *)v, k_stride, v_stride, stream_of(stream)), "cache_read");
+}
+
+int64_t hq_attention_work_bytes(const hq_cache *cache, const hq_batch *batch, int32_t heads) {
+  g_error = HQ_OK;
+  hq::Cache c;
+  hq::Batch b;
+  if (paged_of("attention_work_bytes", cache, batch, c, b, false)) return -1;
+  if (heads_of("attention_work_bytes", c, b, heads)) return -1;
+  return hq::attention_work_bytes(c, b, heads);
+}
+
+int32_t hq_attention_ex(void *out, const void *q, int32_t heads, int32_t out_stride, int32_t q_stride,
+                        const hq_cache *cache, const hq_batch *batch, float scale, int32_t window, float cap, void *work,
+                        int64_t work_bytes, void *stream) {
+  g_error = HQ_OK;
+  hq::Cache c;
+  hq::Batch b;
+  if (int32_t st = paged_of("attention", cache, batch, c, b)) return st;
+  if (int32_t st = heads_of("attention", c, b, heads)) return st;
+  if (!(scale > 0.0f) || std::isinf(scale)) return fail(HQ_ERR_ARGUMENT, "attention: scale = %g", (double)scale);
+  if (window < 0) return fail(HQ_ERR_ARGUMENT, "attention: window = %d", window);
+  if (!(cap >= 0.0f) || std::isinf(cap)) return fail(HQ_ERR_ARGUMENT, "attention: cap = %g", (double)cap);
+  if (int32_t st = rows_of("attention", b, out, out_stride, (int64_t)heads * c.dim)) return st;
+  if (int32_t st = rows_of("attention", b, q, q_stride, (int64_t)heads * c.dim)) return st;
+  if (b.tokens == 0 || b.sequences == 0) return HQ_OK;
+  const int64_t need = hq::attention_work_bytes(c, b, heads);
+  if (work_bytes < need)
+    return fail(HQ_ERR_ARGUMENT, "attention: a workspace of %lld bytes, %lld are needed", (long long)work_bytes, (long long)need);
+  if (need && !work) return fail(HQ_ERR_NULL, "attention: work NULL");
+  if (!aligned(work, 256)) return fail(HQ_ERR_ALIGNMENT, "attention: work not 256-byte aligned");
+  if (int32_t st = ensure_device()) return st;
+  const hq::Attention a{(char *)out, (const char *)q, (char *)work, out_stride, q_stride, heads, window, scale, cap};
+  return hip_status(hq::launch_attention(a, c, b, stream_of(stream)), "attention");
 }
 
 // ---- a phase of jobs in the reference's table form ------------------------------------------------------------

@@ -1,4 +1,4 @@
-// launch.hpp — the host-side launchers of libhq.so's kernels (defined in quantize.hip, gemv.hip, gemm.hip) and
+// launch.hpp — the host-side launchers of libhq.so's kernels (defined in quantize.hip, gemv.hip, gemm.hip and the other .hip files) and
 // the job descriptors they take.  abi.cpp validates the C-ABI's arguments and calls these; they only launch.
 #pragma once
 #include <hip/hip_runtime.h>
@@ -133,6 +133,44 @@ int64_t tol_work_bytes(int32_t n, int32_t count);
 hipError_t launch_gemm_tol(const Job &job, char *work, hipStream_t s);
 // the tiles launch_gemm_tol gives `rows` rows of `count` tokens
 int64_t tol_tiles(int32_t rows, int32_t count);
+
+// a layer's norm between two products (norm.hip): count tokens, x and r x_stride bytes apart, d d_stride, y y_stride; d, r, y
+// and xq may be NULL (r not where d is given); n values a token, quantized with `bias` as `mode` says into xq + t frame,
+// xs + t frame
+struct NormRows {
+  char *xq, *xs, *y, *r;
+  const char *x, *d, *w;
+  int64_t frame, x_stride, d_stride, y_stride;
+  int32_t count;
+};
+hipError_t launch_norm(Ready mode, const NormRows &a, int32_t n, float eps, int32_t bias, hipStream_t s);
+
+// the paged key/value cache and a batch of new tokens (hq_cache and hq_batch of hq.h, checked): a page is 1 << shift positions
+struct Cache {
+  char *k, *v;
+  float *ks, *vs;
+  int32_t f16, pages, shift, heads, dim;
+};
+struct Batch {
+  const int32_t *starts, *lengths, *table;
+  int32_t sequences, tokens, longest, width;
+};
+hipError_t launch_cache_write(const Cache &c, const Batch &b, const char *k, const char *v, int64_t k_stride,
+                              int64_t v_stride, hipStream_t s);
+hipError_t launch_cache_read(const Cache &c, const Batch &b, char *k, char *v, int64_t k_stride, int64_t v_stride,
+                             hipStream_t s);
+// attention (attention.hip): `heads` query heads, token t's at q + t q_stride and out + t out_stride (bytes), with
+// attention_work_bytes bytes of scratch at work
+struct Attention {
+  char *out;
+  const char *q;
+  char *work;
+  int64_t out_stride, q_stride;
+  int32_t heads, window;
+  float scale, cap;
+};
+int64_t attention_work_bytes(const Cache &c, const Batch &b, int32_t heads);
+hipError_t launch_attention(const Attention &a, const Cache &c, const Batch &b, hipStream_t s);
 
 // the ceilings (ceilings.hip): every byte of [p, p + bytes) read once; `iterations` x 8 MFMAs a wave of `blocks`
 // blocks of 4 waves.  sink: 256 words that are almost never written

@@ -5,6 +5,7 @@
 // Byte-for-byte the reference's outputs; a token's activations are a few KB (latency-bound), a prompt's tens of MB.
 #include "common.hpp"
 #include "launch.hpp"
+#include "ready.hpp"
 
 namespace hq {
 
@@ -61,33 +62,9 @@ __global__ __launch_bounds__(256) void ready_kernel(char *xq, char *xs, const ch
   const int32_t at = blockIdx.x * kReadyValues + threadIdx.x * 4;  // the lane's first value of the token
   const bool live = at < n;
   const int64_t t = blockIdx.y;
-  const int g = at >> 5, lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63;
   const float4 f = *(const float4 *)(x + t * x_stride + 4 * (int64_t)(live ? at : 0));
-  const Quantized4 o = quantize4(f, bias);
-  char *to = xq + t * frame, *st = xs + t * frame;
-  if (live && (lane & 7) == 0) ((float *)st)[g] = o.scale;
-  if (MODE == 0) {
-    if (live) *(uint32_t *)(to + at) = o.d;
-    return;
-  }
-  if (MODE == 1) {
-    const int32_t s32 = o.s16 + dpp<0x141>(o.s16);
-    if (live && (lane & 7) == 0) ((int32_t *)st)[(n >> 5) + g] = -s32;
-    // byte 16 p + c of a block of 64 is value 4 c + p: the quad m of the block's 16 lanes holds c = 4 m .. + 3, and
-    // its lane p gathers byte p of the four lanes into the dword at 16 p + 4 m
-    const uint32_t q0 = (uint32_t)dpp<0x00>((int32_t)o.d), q1 = (uint32_t)dpp<0x55>((int32_t)o.d);
-    const uint32_t q2 = (uint32_t)dpp<0xAA>((int32_t)o.d), q3 = (uint32_t)dpp<0xFF>((int32_t)o.d);
-    const uint32_t p = lane & 3, sel = p | ((4 + p) << 8);
-    const uint32_t plane = perm(perm(q3, q2, sel), perm(q1, q0, sel), 0x05040100u);
-    if (live) *(uint32_t *)(to + (at & ~63) + 16 * p + (lane & 12)) = plane;
-  } else {
-    int16_t *a16 = (int16_t *)(st + 4 * (n >> 5)), *a8 = a16 + (n >> 4);
-    if (live) {
-      *(uint32_t *)(to + at) = o.d;
-      if ((lane & 1) == 0) a8[at >> 3] = (int16_t)o.s8;
-      if ((lane & 3) == 0) a16[at >> 4] = (int16_t)o.s16;
-    }
-  }
+  store_ready<MODE>(quantize4(f, bias), xq + t * frame, xs + t * frame, at, n, lane, live);
 }
 
 template <int MODE>
