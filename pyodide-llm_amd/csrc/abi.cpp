@@ -439,7 +439,7 @@ int32_t paged_of(const char *who, const hq_cache *cache, const hq_batch *batch, 
                 cache->pages, shift, cache->heads, cache->dim};
   const int32_t longest = batch->longest && batch->longest < batch->tokens ? batch->longest : batch->tokens;
   b = hq::Batch{(const int32_t *)batch->starts, (const int32_t *)batch->lengths, (const int32_t *)batch->table,
-                batch->sequences, batch->tokens, longest, batch->width};
+                batch->sequences, batch->tokens, longest, c.pages ? batch->width : 0};
   if (!memory || b.tokens == 0 || b.sequences == 0) return HQ_OK;
   if (!b.starts || !b.lengths || (!b.table && b.width)) return fail(HQ_ERR_NULL, "%s: starts, lengths or table NULL", who);
   if (!aligned(b.starts, 4) || !aligned(b.lengths, 4) || !aligned(b.table, 4))

@@ -53,9 +53,9 @@ HQ_DEV Place place_of(int32_t sequences, int32_t at, Count count_of) {
     const uint64_t past = __ballot(upto > at);
     if (past) {
       const int l = __ffsll((unsigned long long)past) - 1;
-      return {s0 + l, at - (__shfl(upto, l, 64) - __shfl(mine, l, 64))};
+      return {s0 + l, __builtin_amdgcn_readlane(mine, l) - __builtin_amdgcn_readlane(upto, l) + at};
     }
-    at -= __shfl(upto, 63, 64);
+    at -= __builtin_amdgcn_readlane(upto, 63);
   }
   return {-1, 0};
 }
