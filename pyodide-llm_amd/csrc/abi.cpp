@@ -834,7 +834,9 @@ int64_t hq_attention_work_bytes(const hq_cache *cache, const hq_batch *batch, in
   hq::Batch b;
   if (paged_of("attention_work_bytes", cache, batch, c, b, false)) return -1;
   if (heads_of("attention_work_bytes", c, b, heads)) return -1;
-  return hq::attention_work_bytes(c, b, heads);
+  const int64_t need = hq::attention_work_bytes(c, b, heads);
+  if (need < 0) return fail(HQ_ERR_ARGUMENT, "attention_work_bytes: more work than a call can count"), -1;
+  return need;
 }
 
 int32_t hq_attention_ex(void *out, const void *q, int32_t heads, int32_t out_stride, int32_t q_stride,
@@ -852,6 +854,7 @@ int32_t hq_attention_ex(void *out, const void *q, int32_t heads, int32_t out_str
   if (int32_t st = rows_of("attention", b, q, q_stride, (int64_t)heads * c.dim)) return st;
   if (b.tokens == 0 || b.sequences == 0) return HQ_OK;
   const int64_t need = hq::attention_work_bytes(c, b, heads);
+  if (need < 0) return fail(HQ_ERR_ARGUMENT, "attention: more work than a call can count");
   if (work_bytes < need)
     return fail(HQ_ERR_ARGUMENT, "attention: a workspace of %lld bytes, %lld are needed", (long long)work_bytes, (long long)need);
   if (need && !work) return fail(HQ_ERR_NULL, "attention: work NULL");

@@ -63,7 +63,7 @@ __global__ __launch_bounds__(256) void write_kernel(Cache c, Batch b, const char
   if (place.s < 0) return;
   const int32_t h = blockIdx.y;
   const bool values = blockIdx.z;
-  const Sequence q = sequence_of(b, place.s);
+  const Sequence q = wave_sequence_of(b, place.s);
   const int32_t first = q.length - q.count, base = ((first >> 6) + place.rest) * kChunk;
   const int32_t from = max(max(first, base), 0), to = min(q.length, base + kChunk);  // the positions to write
   const int row = threadIdx.x >> 4, l = threadIdx.x & 15;
@@ -148,7 +148,7 @@ __global__ __launch_bounds__(256) void read_kernel(Cache c, Batch b, char *k, ch
   if (place.s < 0) return;
   const int32_t h = blockIdx.y;
   const bool values = blockIdx.z;
-  const Sequence q = sequence_of(b, place.s);
+  const Sequence q = wave_sequence_of(b, place.s);
   const int32_t first = q.length - q.count, base = ((first >> 6) + place.rest) * kChunk;
   const int32_t from = max(first, base), to = min(q.length, base + kChunk);
   constexpr int PARTS = kChunk * ES / 16, EACH = 16 / ES;

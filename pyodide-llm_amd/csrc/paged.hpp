@@ -20,6 +20,15 @@ HQ_DEV Sequence sequence_of(const Batch &b, int32_t s) {
   return q;
 }
 
+// the same of a sequence that the whole wave asks for
+HQ_DEV Sequence wave_sequence_of(const Batch &b, int32_t s) {
+  Sequence q = sequence_of(b, s);
+  q.begin = __builtin_amdgcn_readfirstlane(q.begin);
+  q.count = __builtin_amdgcn_readfirstlane(q.count);
+  q.length = __builtin_amdgcn_readfirstlane(q.length);
+  return q;
+}
+
 // the page that holds position `at` of sequence s, or -1: none (a position before the first or past the table, an entry that
 // is no page)
 HQ_DEV int32_t page_of(const Batch &b, const Cache &c, int32_t s, int32_t at) {

@@ -173,6 +173,38 @@ def test_longest_is_a_hint(pkg, arena, form):
         check(p, queries(rng, p, 8))
 
 
+@pytest.mark.parametrize("starts", [[0, 5, 3, 9], [-4, 2, 100, 9], [3, 3, 8, 9], [0, 9, 0, 9]])
+@pytest.mark.parametrize("longest", [0, 1])
+def test_contradicting_starts(pkg, arena, starts, longest):
+    """starts that fall, start below 0 or pass the tokens' end write nothing outside the rows and the workspace (numbers undefined)"""
+    rng = np.random.default_rng(1)
+    arena.reset()
+    p = Paged(pkg, arena, rng, "int8", 1, 32, 16, [300, 20, 300], [3, 3, 3], longest=longest)
+    p.fill(rng)
+    arena.write(p.batch.starts, np.asarray(starts, np.int32))
+    lib, heads = pkg.library(), 30
+    q = arena.put(queries(rng, p, heads))
+    guards = [arena.put(np.full(4096, 77, np.uint8))]
+    out = arena.alloc(9 * heads * 128)
+    guards.append(arena.put(np.full(4096, 77, np.uint8)))
+    need = lib.hq_attention_work_bytes(p.cache, p.batch, heads)
+    work = arena.alloc(need)
+    guards.append(arena.put(np.full(4096, 77, np.uint8)))
+    assert lib.hq_attention_ex(out, q, heads, heads * 128, heads * 128, p.cache, p.batch, 0.1, 0, 0.0, work, need, None) == 0
+    for at in guards:
+        assert (arena.get(at, np.uint8, 4096) == 77).all()
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_no_pages(pkg, arena, new):
+    """a cache without pages (its pointers NULL): zeros, and nothing is read"""
+    rng = np.random.default_rng(1)
+    arena.reset()
+    p = Paged(pkg, arena, rng, "f16", 2, 64, 16, [50, 60], [new, new])
+    p.cache.pages, p.cache.k, p.cache.v, p.cache.ks, p.cache.vs = 0, None, None, None, None
+    assert (p.run_attention(queries(rng, p, 8), 0.1) == 0).all()
+
+
 def test_stream_and_graph(pkg, arena):
     """another stream than torch's, and a captured step (write, attention) replayed with other lengths and inputs, each replay
     against the eager call"""
