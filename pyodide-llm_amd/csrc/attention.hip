@@ -29,6 +29,7 @@ namespace {
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -40,73 +41,115 @@ constexpr int kLeast = -100;  // the exponent of the smallest scale a cache stor
 struct Share {
   int32_t blocks;     // blocks that share the work
   int32_t rows;       // of a tile
-  int32_t positions;  // of a block's step
+  int32_t log;        // of a block's step's positions, to base 2
+  int32_t group;      // query heads that share a key/value head
+  uint32_t per;       // ceil(2^32 / group) (0: group is 1): the token of a row without a division
   int32_t tiles;      // there can be
+  bool shared;        // whether an item can have more than one step
   int64_t parts;      // where in the workspace the shared items' parts are
   int64_t bytes;      // the workspace
-  int64_t most;       // steps there can be
+  bool countable;     // whether its numbers fit their types
 };
+
+// what a kernel is called with
+struct Call {
+  Attention a;
+  Cache c;
+  Batch b;
+  Share sh;
+};
+
+// row / group: exact while row group < 2^32, which the host makes sure of
+HQ_DEV int32_t token_of(const Share &sh, int32_t row) { return sh.per ? (int32_t)__umulhi((uint32_t)row, sh.per) : row; }
 
 // a tile's rows r0 .. r1 - 1 of a sequence, the positions from .. to - 1 that some of them see, and the steps that hold
 // these: first .. first + steps - 1 (one at least: rows that see nothing are written too)
 struct Tile {
   int32_t r0, r1, from, to, first, steps;
 };
-HQ_DEV Tile tile_of(const Attention &a, const Cache &c, const Batch &b, const Share &sh, const Sequence &q, int32_t group,
-                    int32_t rt) {
+HQ_DEV Tile tile_of(const Call &k, const Sequence &q, int32_t rt) {
   Tile t;
-  t.r0 = rt * sh.rows;
-  t.r1 = min(t.r0 + sh.rows, q.count * group);
-  const int32_t before = q.length - q.count, reach = b.width << c.shift;
-  t.to = min(max(before + (t.r1 - 1) / group + 1, 0), reach);
-  t.from = a.window ? max(before + t.r0 / group + 1 - a.window, 0) : 0;
-  t.first = t.from / sh.positions;
-  t.steps = max((t.to + sh.positions - 1) / sh.positions - t.first, 1);
+  t.r0 = rt * k.sh.rows;
+  t.r1 = min(t.r0 + k.sh.rows, q.count * k.sh.group);
+  const int32_t before = q.length - q.count, reach = k.b.width << k.c.shift;
+  t.to = min(max(before + token_of(k.sh, t.r1 - 1) + 1, 0), reach);
+  t.from = k.a.window ? max(before + token_of(k.sh, t.r0) + 1 - k.a.window, 0) : 0;
+  t.first = t.from >> k.sh.log;
+  t.steps = max((int32_t)(((int64_t)t.to + (1 << k.sh.log) - 1) >> k.sh.log) - t.first, 1);
   return t;
 }
 
-HQ_DEV int32_t steps_of(const Attention &a, const Cache &c, const Batch &b, const Share &sh, int32_t s) {
-  const Sequence q = sequence_of(b, s);
-  const int32_t group = a.heads / c.heads, rows = q.count * group;
+// the steps of a sequence's tiles over all heads
+HQ_DEV int32_t steps_of(const Call &k, int32_t s) {
+  const Sequence q = sequence_of(k.b, s);
+  const int32_t rows = q.count * k.sh.group;
   int32_t n = 0;
-  for (int32_t rt = 0; rt * kFewRows < rows; rt++) n += tile_of(a, c, b, sh, q, group, rt).steps;
-  return n * c.heads;
+  for (int32_t rt = 0; rt * kFewRows < rows; rt++) n += tile_of(k, q, rt).steps;
+  return n * k.c.heads;
 }
 
-// All steps in a row: sequences, their row tiles, the heads, the steps.  Where step `at` is.
+// All steps in a row: sequences, their row tiles, the heads, the steps.  Where a step is.
 struct Spot {
   int32_t s, rt, h, step;
   Sequence q;
   Tile t;
 };
-HQ_DEV Spot spot_of(const Attention &a, const Cache &c, const Batch &b, const Share &sh, int32_t at) {
-  const Place p = place_of(b.sequences, at, [&](int32_t s) { return steps_of(a, c, b, sh, s); });
-  Spot o;
-  o.s = p.s, o.rt = 0;
-  o.q = wave_sequence_of(b, max(p.s, 0));
-  const int32_t group = a.heads / c.heads;
-  int32_t rest = p.rest;
-  for (;; o.rt++) {
-    o.t = tile_of(a, c, b, sh, o.q, group, o.rt);
-    if (rest < o.t.steps * c.heads || (o.rt + 1) * kFewRows >= o.q.count * group) break;
-    rest -= o.t.steps * c.heads;
+
+// the sums up to each lane's value; INT32_MAX where they pass it (which sequences that overlap could make them)
+HQ_DEV int32_t wave_sums_of(int32_t v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t w = (uint32_t)__shfl_up(v, o, 64);
+    if (lane >= o) v = (int32_t)min((uint32_t)v + w, (uint32_t)INT32_MAX);
   }
-  o.h = rest / o.t.steps;
-  o.step = rest - o.h * o.t.steps;
-  return o;
+  return v;
 }
 
-// (sequences that overlap could have more steps than 32 bits count, which the host has made sure of for others: none then)
-HQ_DEV int32_t all_steps(const Attention &a, const Cache &c, const Batch &b, const Share &sh) {
-  int64_t n = 0;
-  for (int32_t s = threadIdx.x & 63; s < b.sequences; s += 64) n += steps_of(a, c, b, sh, s);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
-  return __builtin_amdgcn_readfirstlane(n <= INT32_MAX ? (int32_t)n : 0);
-}
 HQ_DEV int32_t share_start(int32_t steps, int32_t block, int32_t blocks) {
   return (int32_t)((int64_t)steps * block / blocks);
 }
+
+
+// The block's share [u, end) of all steps, and where its first is (u < end): one look at every 64 sequences, two where there are
+// more of them.
+HQ_DEV void find_share(const Call &k, int32_t block, int32_t &all, int32_t &u, int32_t &end, Spot &o) {
+  const int lane = threadIdx.x & 63;
+  const int32_t n = k.b.sequences;
+  int32_t mine = lane < n ? steps_of(k, lane) : 0, upto = wave_sums_of(mine);
+  uint32_t total = (uint32_t)__builtin_amdgcn_readlane(upto, 63);
+  for (int32_t s0 = 64; s0 < n; s0 += 64) {
+    const int32_t more = wave_sums_of(s0 + lane < n ? steps_of(k, s0 + lane) : 0);
+    total = min(total + (uint32_t)__builtin_amdgcn_readlane(more, 63), (uint32_t)INT32_MAX);
+  }
+  all = total < (uint32_t)INT32_MAX ? (int32_t)total : 0;
+  u = share_start(all, block, k.sh.blocks), end = share_start(all, block + 1, k.sh.blocks);
+  if (u >= end) return;
+  int32_t rest = u, s0 = 0;
+  uint64_t past;
+  while (!(past = __ballot(upto > rest))) {  // (all steps are more than u: one chunk has it)
+    rest -= __builtin_amdgcn_readlane(upto, 63);
+    s0 += 64;
+    mine = s0 + lane < n ? steps_of(k, s0 + lane) : 0, upto = wave_sums_of(mine);
+  }
+  const int l = __ffsll((unsigned long long)past) - 1;
+  rest -= __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(mine, l);
+  o.s = s0 + l, o.rt = 0;
+  o.q = wave_sequence_of(k.b, o.s);
+  for (;; o.rt++) {
+    o.t = tile_of(k, o.q, o.rt);
+    if (rest < o.t.steps * k.c.heads || (o.rt + 1) * kFewRows >= o.q.count * k.sh.group) break;
+    rest -= o.t.steps * k.c.heads;
+  }
+  o.h = rest / o.t.steps;
+  o.step = rest - o.h * o.t.steps;
+}
+
+// What join_kernel needs of the item whose start a block has and whose end it has not: its rows' first token and row there, how many
+// rows, the head, the item's last step (-1: the block has no such item), and all steps
+struct Tail {
+  int32_t begin, r0, rows, h, last, all, pad[2];
+};
 
 // ---- arithmetic ---------------------------------------------------------------------------------------------------
 HQ_DEV float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -159,12 +202,6 @@ HQ_DEV uint32_t opaque_lane(uint32_t x) {
 
 // A kernel's arguments, read anew: what only the start and the end of an item need is not held in scalar registers through the
 // steps between (the kernel's one argument is a Call)
-struct Call {
-  Attention a;
-  Cache c;
-  Batch b;
-  Share sh;
-};
 HQ_DEV const Call *call_again() {
   auto p = (const __attribute__((address_space(4))) Call *)__builtin_amdgcn_kernarg_segment_ptr();
   asm volatile("" : "+s"(p));
@@ -211,9 +248,18 @@ HQ_DEV v8h widen8(uint32_t w0, uint32_t w1) {
 // the two float16 of 8 float32
 HQ_DEV void halves_of(const float *x, v8h &hi, v8h &lo) {
 #pragma unroll
-  for (int j = 0; j < 8; j++) {
-    hi[j] = (_Float16)x[j];
-    lo[j] = (_Float16)(x[j] - (float)hi[j]);
+  for (int j = 0; j < 8; j += 2) {
+    const v2f two = {x[j], x[j + 1]};
+    const v2h h = __builtin_convertvector(two, v2h);
+    // what is left of each: the mixed-precision multiply-add reads the float16 as it is
+    v2f rest;
+    float r0, r1;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(h), "v"(two[0]));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(h), "v"(two[1]));
+    rest = v2f{r0, r1};
+    const v2h l = __builtin_convertvector(rest, v2h);
+    hi[j] = h[0], hi[j + 1] = h[1];
+    lo[j] = l[0], lo[j + 1] = l[1];
   }
 }
 
@@ -240,37 +286,38 @@ struct Elements {
 // memory to registers: the waves share nothing, and the next step's keys are on their way while this one's weights are formed.
 // Steps of all (sequence, rows, head) are shared evenly among as many blocks as the GPU holds, whatever the lengths; what a
 // block finds of an item that it does not have whole goes to `work` and join_kernel.
-constexpr int few_np(int, int f16) { return f16 ? 8 : 16; }
+constexpr int few_np(int d, int f16) { return f16 || d <= 64 ? 8 : 16; }
 constexpr int few_blocks_a_cu(int d, int) { return d <= 64 ? 3 : d <= 128 ? 2 : 1; }
 template <int D, int F16>
 __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call) {
   constexpr int ES = F16 ? 2 : 1, DB = D / 64, DT = D / 16, PITCH = D + 4, NP = few_np(D, F16), WK = 4 * NP, STEP = 4 * WK;
   __shared__ float sums[4][kFewRows][PITCH];
   __shared__ float stats[2][4][kFewRows];
+  __shared__ int32_t parked[4][14];  // a wave's numbers that its steps do not need
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m16 = lane & 15, q4 = lane >> 4;
   int32_t u, end;
   Spot o;
   {
     const Call *k = call_again();
-    const int32_t all = all_steps(k->a, k->c, k->b, k->sh);
-    u = share_start(all, blockIdx.x, k->sh.blocks);
-    end = share_start(all, blockIdx.x + 1, k->sh.blocks);
+    int32_t all;
+    find_share(*k, blockIdx.x, all, u, end, o);
+    // (no tail yet: the share's last item says whether it has one)
+    if (threadIdx.x == 0) ((Tail *)k->a.work)[blockIdx.x].all = all, ((Tail *)k->a.work)[blockIdx.x].last = -1;
     if (u >= end) return;
-    o = spot_of(k->a, k->c, k->b, k->sh, u);
   }
   while (true) {
     const Call *call = call_again();
     const Attention &a = call->a;
     const Cache c = call->c;
     const Batch b = call->b;
-    const int32_t group = a.heads / c.heads, reach = b.width << c.shift, mask = (1 << c.shift) - 1;
+    const Share sh = call->sh;
+    const int32_t group = sh.group, reach = b.width << c.shift, mask = (1 << c.shift) - 1;
     const int32_t steps = min(o.t.steps - o.step, end - u);
-    const bool whole = steps == o.t.steps;
     // ---- the rows' queries
     const int32_t row = o.t.r0 + m16, before = o.q.length - o.q.count;
     const bool live = row < o.t.r1;
-    const int32_t token = (live ? row : o.t.r0) / group, g = (live ? row : o.t.r0) - token * group;
+    const int32_t token = token_of(sh, live ? row : o.t.r0), g = (live ? row : o.t.r0) - token * group;
     const float *x = (const float *)(a.q + (o.q.begin + token) * a.q_stride) + (int64_t)(o.h * group + g) * c.dim;
     v8h qh[DB][2], ql[DB][2];
     float rowf;
@@ -298,13 +345,19 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
           halves_of(e, qh[d][i], ql[d][i]);
         }
     }
-    if (a.cap == 0.0f) rowf *= kLog2e;
-    const float cap = a.cap, per_cap = 1.0f / cap;
+    // a score is its product times rowf, in base 2; with a cap row_cap comes before the tanh instead
+    const float cap = a.cap, row_cap = rowf / cap;
+    rowf = cap > 0.0f ? 1.0f : rowf * kLog2e;
     const int32_t sees = before + token + 1;
     const int32_t to = min(sees, reach), from = a.window ? sees - a.window : 0;  // the lane's row's own positions
     // the positions that every row sees lie in [every_from, every_to)
-    const int32_t every_to = min(before + o.t.r0 / group + 1, reach);
-    const int32_t every_from = a.window ? before + (o.t.r1 - 1) / group + 1 - a.window : 0;
+    const int32_t every_to = min(before + token_of(sh, o.t.r0) + 1, reach);
+    const int32_t every_from = a.window ? before + token_of(sh, o.t.r1 - 1) + 1 - a.window : 0;
+    {
+      const int32_t now[14] = {u, end, o.rt, o.step, o.h, steps, o.t.steps, o.t.r0, o.t.r1, o.q.begin, o.q.count, o.q.length, o.t.first, 0};
+#pragma unroll
+      for (int i = 0; i < 13; i++) parked[wave][i] = now[i];
+    }
     // ---- the wave's positions: WK from base on, every STEP
     float m = -INFINITY, l = 0.0f;
     int exponent = kLeast;
@@ -313,8 +366,11 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
     const int32_t stop = min((o.t.first + o.step + steps) * STEP, o.t.to);
     while (base + WK <= o.t.from) base += STEP;
     if (base < stop) {
+      // Registers are loaded for the next step as soon as this one has used them: keys after the scores, scales after the weights,
+      // values after their products, so that a step's bytes are always on their way.
       Elements<F16, 16> kk[NP / 4][DB];
-      int32_t page1 = page_of(b, c, o.s, base + NP * (m16 >> 2)), page2 = page_of(b, c, o.s, base + NP * q4);
+      Elements<F16, NP> vv[DT];
+      float ks[NP], vs[NP];
       const auto load_keys = [&](int32_t at, int32_t page) {
         const int64_t vec = vectors_of(c, max(page, 0), o.h) + ((at + NP * (m16 >> 2)) & mask) + (m16 & 3);
         const int32_t dim = opaque(c.dim);
@@ -326,28 +382,31 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
             // (dimensions past dim: the row's first, times zeros)
             kk[t][d].load(p + (t * 4 * dim + (64 * d + 16 * q4 < dim ? 64 * d + 16 * q4 : 0)) * ES);
       };
-      load_keys(base, page1);
-      while (true) {
-        const int32_t next = base + STEP;
-        const bool more = next < stop;
-        const int32_t at1 = (more ? next : base) + NP * (m16 >> 2), at2 = (more ? next : base) + NP * q4;
-        const int32_t next1 = page_of(b, c, o.s, at1), next2 = page_of(b, c, o.s, at2);
-        // ---- values and scales of the lane's 16 positions
-        const int64_t vec = vectors_of(c, max(page2, 0), o.h);
-        const int32_t slot = (base + NP * q4) & mask;
-        Elements<F16, NP> vv[DT];
-        float ks[NP], vs[NP];
+      // the lane's NP positions from at + NP q4 on, on `page`
+      const auto load_scales = [&](int32_t at, int32_t page) {
+        const int64_t vec = vectors_of(c, max(page, 0), o.h) + ((at + NP * q4) & mask);
 #pragma unroll
         for (int i = 0; i < NP / 4; i++) {
-          *(float4 *)(ks + 4 * i) = *(const float4 *)(c.ks + vec + slot + 4 * i);
-          *(float4 *)(vs + 4 * i) = *(const float4 *)(c.vs + vec + slot + 4 * i);
+          *(float4 *)(ks + 4 * i) = *(const float4 *)(c.ks + vec + 4 * i);
+          *(float4 *)(vs + 4 * i) = *(const float4 *)(c.vs + vec + 4 * i);
         }
-        {
-          const int32_t dim = opaque(c.dim), shift = opaque(c.shift);
-          const char *p = c.v + (vec * dim + (m16 << shift) + slot) * ES;
+      };
+      const auto values_at = [&](int32_t at, int32_t page) {
+        return c.v + (vectors_of(c, max(page, 0), o.h) * c.dim + (m16 << c.shift) + ((at + NP * q4) & mask)) * ES;
+      };
+      const auto value_row = [&](int d, int32_t dim, int32_t shift) { return (min(d * 16, dim - 16) << shift) * ES; };  // (past dim: the last again)
+      int32_t page2 = page_of(b, c, o.s, base + NP * q4);
+      load_keys(base, page_of(b, c, o.s, base + NP * (m16 >> 2)));
+      load_scales(base, page2);
+      {
+        const char *p = values_at(base, page2);
 #pragma unroll
-          for (int d = 0; d < DT; d++) vv[d].load(p + (min(d * 16, dim - 16) << shift) * ES);  // (past dim: the last again)
-        }
+        for (int d = 0; d < DT; d++) vv[d].load(p + value_row(d, c.dim, c.shift));
+      }
+      int32_t next = base + STEP < stop ? base + STEP : base;  // (the last step loads itself again)
+      int32_t next1 = page_of(b, c, o.s, next + NP * (m16 >> 2)), next2 = page_of(b, c, o.s, next + NP * q4);
+      while (true) {
+        const bool more = base + STEP < stop;
         // ---- scores
         v4f s[NP / 4] = {};
 #pragma unroll
@@ -360,14 +419,14 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
               s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, ql[d][i], s[t], 0, 0, 0);
               s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, qh[d][i], s[t], 0, 0, 0);
             }
-        load_keys(more ? next : base, next1);
+        load_keys(next, next1);
         float p[NP];
 #pragma unroll
-        for (int e = 0; e < NP; e++) p[e] = s[e >> 2][e & 3] * ks[e] * rowf;
+        for (int e = 0; e < NP; e++) p[e] = s[e >> 2][e & 3] * ks[e];
         if (cap > 0.0f) {
           const float bend = opaque(0.55f), twice = opaque(2.0f * kLog2e);
 #pragma unroll
-          for (int e = 0; e < NP; e++) p[e] = cap * kLog2e * tanh_of(p[e] * per_cap, bend, twice);
+          for (int e = 0; e < NP; e++) p[e] = cap * kLog2e * tanh_of(p[e] * row_cap, bend, twice);
         }
         const bool edge = base + WK > every_to || base < every_from || __any(page2 < 0);
         uint32_t seen = ~0u;
@@ -394,7 +453,7 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
         float most = p[0], wide = vs[0];
 #pragma unroll
         for (int e = 1; e < NP; e++) most = fmaxf(most, p[e]), wide = fmaxf(wide, vs[e]);
-        most = max_row(most), wide = max_row(wide);
+        most = max_row(most) * rowf, wide = max_row(wide);
         if (__any(most > m + kRoom)) {  // (the first that is seen too: m is -infinity before it)
           const float m1 = fmaxf(m, most);
           const float alpha = m1 == -INFINITY ? 0.0f : exp2_of(m - m1);
@@ -413,7 +472,7 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
         const float less = (m == -INFINITY ? 0.0f : m) - kShift, by = power_of_2(-exponent);
 #pragma unroll
         for (int e = 0; e < NP; e++) {
-          p[e] = exp2_of(p[e] - less);
+          p[e] = exp2_of(__builtin_fmaf(p[e], rowf, -less));
           l += p[e];
           p[e] = p[e] * (vs[e] * by);
         }
@@ -422,26 +481,42 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
           for (int e = 0; e < NP; e++)
             p[e] = kept(p[e], seen, e, 0u);  // (a NaN scale that others see)
         }
+        load_scales(next, next2);
         // ---- out += weights times values
         v8h ph[NP / 8], pl[NP / 8];
 #pragma unroll
         for (int i = 0; i < NP / 8; i++) halves_of(p + 8 * i, ph[i], pl[i]);
+        const char *v_next = values_at(next, next2);
+        const int32_t dim = opaque(c.dim), shift = opaque(c.shift);
 #pragma unroll
-        for (int d = 0; d < DT; d++)
+        for (int d = 0; d < DT; d++) {
+          v8h v8[NP / 8];
+#pragma unroll
+          for (int i = 0; i < NP / 8; i++) v8[i] = vv[d].half(i);
 #pragma unroll
           for (int i = 0; i < NP / 8; i++) {
-            const v8h v8 = vv[d].half(i);
-            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, pl[i], acc[d], 0, 0, 0);
-            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, ph[i], acc[d], 0, 0, 0);
+            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8[i], pl[i], acc[d], 0, 0, 0);
+            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8[i], ph[i], acc[d], 0, 0, 0);
           }
+          vv[d].load(v_next + value_row(d, dim, shift));
+        }
         if (!more) break;
-        base = next, page1 = next1, page2 = next2;
+        base = next, page2 = next2;
+        next = base + STEP < stop ? base + STEP : base;
+        next1 = page_of(b, c, o.s, next + NP * (m16 >> 2)), next2 = page_of(b, c, o.s, next + NP * q4);
       }
     }
     l = sum_row(l);
     // ---- the four waves together
     const Call *after = call_again();
-    const int32_t heads = after->c.heads, shared = after->a.heads / heads;
+    const int32_t heads = after->c.heads, shared = after->sh.group;
+    int32_t back[13];
+#pragma unroll
+    for (int i = 0; i < 13; i++) back[i] = __builtin_amdgcn_readfirstlane(parked[wave][i]);
+    u = back[0], end = back[1], o.rt = back[2], o.step = back[3], o.h = back[4], o.t.steps = back[6], o.t.r0 = back[7];
+    o.t.r1 = back[8], o.q.begin = back[9], o.q.count = back[10], o.q.length = back[11], o.t.first = back[12];
+    const int32_t done = back[5];
+    const bool whole = done == o.t.steps;
     if (q4 == 0) stats[0][wave][m16] = m, stats[1][wave][m16] = l;
     __syncthreads();
     const float m0 = stats[0][0][m16], m1 = stats[0][1][m16], m2 = stats[0][2][m16], m3 = stats[0][3][m16];
@@ -456,7 +531,7 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
     }
     __syncthreads();
     const int32_t slot = o.step > 0 ? 0 : 1;
-    float *part = (float *)after->a.work + (int64_t)(blockIdx.x * 2 + slot) * kFewRows * (D + 2);
+    float *part = (float *)(after->a.work + after->sh.parts) + (int64_t)(blockIdx.x * 2 + slot) * kFewRows * (D + 2);
     if (!whole && threadIdx.x < kFewRows) part[m16 * 2] = mm, part[m16 * 2 + 1] = ll;
     for (int i = threadIdx.x; i < kFewRows * (D / 4); i += 256) {
       const int r = i / (D / 4), d = i % (D / 4) * 4;
@@ -470,13 +545,20 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
         const float am = fmaxf(fmaxf(a0, a1), fmaxf(a2, a3)), ar = am == -INFINITY ? 0.0f : am;
         const float sum = stats[1][0][r] * exp2_of(a0 - ar) + stats[1][1][r] * exp2_of(a1 - ar) +
                           stats[1][2][r] * exp2_of(a2 - ar) + stats[1][3][r] * exp2_of(a3 - ar);
-        const int32_t i0 = (o.t.r0 + r) / shared, gg = o.t.r0 + r - i0 * shared;
+        const int32_t i0 = token_of(after->sh, o.t.r0 + r), gg = o.t.r0 + r - i0 * shared;
         v = sum != 0.0f ? v / sum : v4f{0.f, 0.f, 0.f, 0.f};
         *(v4f *)(after->a.out + (o.q.begin + i0) * after->a.out_stride + ((int64_t)(o.h * shared + gg) * after->c.dim + d) * 4) = v;
       }
     }
-    u += steps;
-    if (u >= end) break;
+    u += done;
+    if (u >= end) {
+      if (threadIdx.x == 0) {
+        Tail &tail = ((Tail *)after->a.work)[blockIdx.x];
+        tail.begin = o.q.begin, tail.r0 = o.t.r0, tail.rows = o.t.r1 - o.t.r0, tail.h = o.h;
+        tail.last = o.step == 0 && !whole ? end - done + o.t.steps - 1 : -1;
+      }
+      break;
+    }
     __syncthreads();
     // ---- the next item: the next head, row tile or sequence (one more step is left, so there is one)
     o.step = 0;
@@ -489,49 +571,84 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
           o.q = wave_sequence_of(after->b, o.s);
         } while (!o.q.count);
       }
-      o.t = tile_of(after->a, after->c, after->b, after->sh, o.q, shared, o.rt);
+      o.t = tile_of(*after, o.q, o.rt);
     }
   }
 }
 
-// The items that blocks share: the block whose share an item starts in (and does not end in) has its rows' parts joined here, a
-// wave a row.
-template <int D>
-__global__ __launch_bounds__(256) void join_kernel(Attention a, Cache c, Batch b, Share sh) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int32_t group = a.heads / c.heads;
-  const int32_t all = all_steps(a, c, b, sh);
-  const int32_t start = share_start(all, blockIdx.x, sh.blocks), end = share_start(all, blockIdx.x + 1, sh.blocks);
-  if (start >= end || end >= all) return;
-  const Spot o = spot_of(a, c, b, sh, end - 1);
-  const int32_t first = end - 1 - o.step, last = first + o.t.steps - 1;  // the item's steps
-  if (first < start || last < end) return;
-  const int r = blockIdx.y * 4 + wave;
-  if (o.t.r0 + r >= o.t.r1) return;
-  const int64_t size = kFewRows * (D + 2);
-  const float *work = (const float *)a.work;
-  float m = -INFINITY, l = 0.0f;
-  float acc[D / 64] = {};
-  int32_t at = blockIdx.x, slot = 1;
-  while (true) {
-    if (share_start(all, at + 1, sh.blocks) > share_start(all, at, sh.blocks)) {  // (a block may have no step)
-      const float *part = work + (int64_t)(at * 2 + slot) * size;
-      const float pm = part[r * 2], pl = part[r * 2 + 1];
-      const float m1 = fmaxf(m, pm), ref = m1 == -INFINITY ? 0.0f : m1;
-      const float f0 = exp2_of(m - ref), f1 = exp2_of(pm - ref);
-      m = m1;
-      l = l * f0 + pl * f1;
+// The parts of a row of an item that blocks share, joined by a wave: those of `parts` (two of `size` floats a block: rows' (m, l)
+// pairs, then rows of D) of block `at` (its second) and the blocks after it (their first) whose share starts in the item, which
+// start_of(block) says; `last` is the item's last step.  Lane i looks at the i-th block; then every lane sums D / 64 values.
+template <int D, typename StartOf>
+HQ_DEV void join_row(const float *parts, int64_t size, int rows, int r, int32_t at, int32_t blocks, int32_t last, StartOf start_of,
+                     float &l, float *acc) {
+  const int lane = threadIdx.x & 63;
+  float m = -INFINITY;
+  l = 0.0f;
 #pragma unroll
-      for (int i = 0; i < D / 64; i++) acc[i] = acc[i] * f0 + part[kFewRows * 2 + r * D + lane + 64 * i] * f1;
+  for (int i = 0; i < D / 64; i++) acc[i] = 0.0f;
+  for (int32_t b0 = at; b0 < blocks; b0 += 64) {
+    const int32_t mine = b0 + lane;
+    const int32_t start = mine < blocks ? start_of(mine) : INT32_MAX;
+    const bool in = start <= last;
+    const uint64_t all = __ballot(in);
+    if (!all) break;
+    const bool some = in && start_of(mine + 1) > start;  // (a share may have no step)
+    const float *part = parts + ((int64_t)mine * 2 + (mine == at ? 1 : 0)) * size;
+    const float pm = some ? part[2 * r] : -INFINITY, pl = some ? part[2 * r + 1] : 0.0f;
+    float m1 = fmaxf(m, pm);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m1 = fmaxf(m1, __shfl_xor(m1, o, 64));
+    const float ref = m1 == -INFINITY ? 0.0f : m1, f0 = exp2_of(m - ref), f = some ? exp2_of(pm - ref) : 0.0f;
+    float sum = pl * f;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    m = m1;
+    l = l * f0 + sum;
+#pragma unroll
+    for (int i = 0; i < D / 64; i++) acc[i] *= f0;
+    const uint64_t with = __ballot(some);
+    const int n = 64 - __builtin_clzll(all);
+    constexpr int AHEAD = 8;  // parts' loads on their way
+    for (int i0 = 0; i0 < n; i0 += AHEAD) {
+      float v[AHEAD][D / 64], fi[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; j++) {
+        const int i = min(i0 + j, 63);
+        const bool there = i0 + j < n && (with >> i & 1);
+        fi[j] = there ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), i)) : 0.0f;
+        const int32_t of = there ? b0 + i : at;  // (the first part is there always)
+        const float *row = parts + ((int64_t)of * 2 + (of == at ? 1 : 0)) * size + 2 * rows + r * D + (D / 64) * lane;
+#pragma unroll
+        for (int k = 0; k < D / 64; k++) v[j][k] = row[k];
+      }
+#pragma unroll
+      for (int j = 0; j < AHEAD; j++)
+#pragma unroll
+        for (int k = 0; k < D / 64; k++) acc[k] += v[j][k] * fi[j];
     }
-    slot = 0;
-    if (share_start(all, at + 1, sh.blocks) > last || ++at >= sh.blocks) break;
+    if (all != ~0ull) break;
   }
-  const int32_t i0 = (o.t.r0 + r) / group, g = o.t.r0 + r - i0 * group;
-  float *out = (float *)(a.out + (o.q.begin + i0) * a.out_stride) + (int64_t)(o.h * group + g) * c.dim;
+}
+
+// The items that blocks share: the block whose share an item starts in (and does not end in) has its rows' parts joined here, a
+// wave a row.  edge: the shares' edges (NULL: even shares of all steps).
+template <int D>
+__global__ __launch_bounds__(256) void join_kernel(Call k, const int32_t *edge) {
+  const Tail t = ((const Tail *)k.a.work)[blockIdx.x];
+  const int32_t rows = __builtin_amdgcn_readfirstlane(t.rows), last = __builtin_amdgcn_readfirstlane(t.last);
+  if (last < 0) return;
+  const int lane = threadIdx.x & 63, step = 4 * gridDim.y;
+  for (int r = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); r < rows; r += step) {
+    float l, acc[D / 64];
+    join_row<D>((const float *)(k.a.work + k.sh.parts), (int64_t)k.sh.rows * (D + 2), k.sh.rows, r, blockIdx.x, k.sh.blocks, last,
+                [&](int32_t i) { return edge ? edge[i] : share_start(t.all, i, k.sh.blocks); }, l, acc);
+    const int32_t i0 = token_of(k.sh, t.r0 + r), g = t.r0 + r - i0 * k.sh.group;
+    float *out = (float *)(k.a.out + (t.begin + i0) * k.a.out_stride) + (int64_t)(t.h * k.sh.group + g) * k.c.dim;
 #pragma unroll
-  for (int i = 0; i < D / 64; i++)
-    if (lane + 64 * i < c.dim) out[lane + 64 * i] = l != 0.0f ? acc[i] / l : 0.0f;
+    for (int i = 0; i < D / 64; i++)
+      if ((D / 64) * lane + i < k.c.dim) out[(D / 64) * lane + i] = l != 0.0f ? acc[i] / l : 0.0f;
+  }
 }
 
 // ---- prompts: 128 rows a block, 32 a wave, over 64 positions a step -----------------------------------------------------
@@ -547,27 +664,31 @@ constexpr int kRows = 128, kPositions = 64;
 
 // where in the row of all steps: sequence, row tile, head and step of the item
 struct Start {
-  int32_t s, rt, h, step;
+  int32_t s, k, h, step;  // (k: the place of the row tile in its sequence's order)
 };
-// the plan, in a call's workspace: the shares' edges (blocks + 1 numbers), the place of each share's first and last step, and the
+// A sequence's row tiles in order: the first, the last, the second, the last but one ...  Later rows see more positions, so that two
+// neighbours together take about the same time and a share of one tile's size ends near every second tile's end.
+HQ_DEV int32_t tile_at(int32_t k, int32_t tiles) { return k & 1 ? tiles - 1 - (k >> 1) : k >> 1; }
+// the plan, in a call's workspace: the shares' tails, their edges (blocks + 1 numbers), the place of each share's first step, and the
 // steps of one head: of all sequences up to s, of the tiles up to a tile of its sequence (tiles from base[s] on)
 struct Plan {
+  Tail *tail;
   int32_t *edge;
-  Start *first, *last;
+  Start *first;
   int32_t *upto, *base, *tile;
 };
-HQ_DEV Plan plan_of(char *work, int32_t blocks, int32_t sequences) {
+__host__ __device__ inline Plan plan_of(char *work, int32_t blocks, int32_t sequences) {
   Plan p;
-  p.first = (Start *)work;
-  p.last = p.first + blocks;
-  p.edge = (int32_t *)(p.last + blocks);
+  p.tail = (Tail *)work;
+  p.first = (Start *)(p.tail + blocks);
+  p.edge = (int32_t *)(p.first + blocks);
   p.upto = p.edge + blocks + 1;
   p.base = p.upto + sequences;
   p.tile = p.base + sequences;
   return p;
 }
 int64_t plan_bytes(int64_t blocks, int64_t sequences, int64_t tiles) {
-  return ((2 * blocks * (int64_t)sizeof(Start) + (blocks + 1 + 2 * sequences + tiles) * 4) + 255) / 256 * 256;
+  return blocks * (int64_t)(sizeof(Tail) + sizeof(Start)) + (blocks + 1 + 2 * sequences + tiles) * 4;
 }
 
 // inclusive sums over a block of 1024 threads
@@ -585,10 +706,17 @@ HQ_DEV int64_t sum_upto(int64_t v, int64_t *wave_sums) {
   return v;
 }
 
-__global__ __launch_bounds__(1024) void plan_kernel(Attention a, Cache c, Batch b, Share sh) {
+constexpr int kPlanSequences = 1024, kPlanTiles = 4096;
+__global__ __launch_bounds__(1024) void plan_kernel(Call k) {
+  const Share &sh = k.sh;
+  const Cache &c = k.c;
+  const Batch &b = k.b;
   __shared__ int64_t wave_sums[16], carry;
-  const Plan p = plan_of(a.work, sh.blocks, b.sequences);
-  const int32_t group = a.heads / c.heads, n = b.sequences;
+  __shared__ int32_t near_upto[kPlanSequences], near_base[kPlanSequences], near_tile[kPlanTiles];
+  Plan p = plan_of(k.a.work, sh.blocks, b.sequences);
+  const int32_t group = sh.group, n = b.sequences;
+  // the sums, which only this kernel reads, in LDS where they fit: the searches below are chains of loads
+  if (n <= kPlanSequences && sh.tiles <= kPlanTiles) p.upto = near_upto, p.base = near_base, p.tile = near_tile;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   // a sequence's first tile
   if (threadIdx.x == 0) carry = 0;
@@ -609,7 +737,7 @@ __global__ __launch_bounds__(1024) void plan_kernel(Attention a, Cache c, Batch 
     const int32_t tiles = p.base[s] < 0 ? 0 : (q.count * group + sh.rows - 1) / sh.rows;
     int32_t before = 0;
     for (int32_t t0 = 0; t0 < tiles; t0 += 64) {
-      int32_t v = t0 + lane < tiles ? tile_of(a, c, b, sh, q, group, t0 + lane).steps : 0;
+      int32_t v = t0 + lane < tiles ? tile_of(k, q, tile_at(t0 + lane, tiles)).steps : 0;
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
         const int32_t w = __shfl_up(v, o, 64);
@@ -632,7 +760,7 @@ __global__ __launch_bounds__(1024) void plan_kernel(Attention a, Cache c, Batch 
     if (threadIdx.x == 1023) carry = upto;
     __syncthreads();
   }
-  const int32_t all = (int32_t)carry * c.heads, near = all / sh.blocks / 8;
+  const int32_t all = (int32_t)carry * c.heads, near = all / sh.blocks / 32;
   // where step `at` is; first and size: its item's
   const auto find = [&](int32_t at, int32_t &first, int32_t &size) {
     int32_t lo = 0, hi = n - 1;
@@ -655,7 +783,7 @@ __global__ __launch_bounds__(1024) void plan_kernel(Attention a, Cache c, Batch 
       else t0 = mid + 1;
     }
     const int32_t begin = t0 ? tile[t0 - 1] : 0;
-    o.rt = t0;
+    o.k = t0;
     o.step = rest - begin;
     first = at - o.step;
     size = tile[t0] - begin;
@@ -673,10 +801,20 @@ __global__ __launch_bounds__(1024) void plan_kernel(Attention a, Cache c, Batch 
   __syncthreads();
   for (int32_t i = threadIdx.x; i < sh.blocks; i += 1024) {
     int32_t first, size;
+    p.tail[i].last = -1;
     if (p.edge[i] >= p.edge[i + 1]) continue;
     p.first[i] = find(p.edge[i], first, size);
-    p.last[i] = find(p.edge[i + 1] - 1, first, size);
   }
+}
+
+// the largest of a wave's numbers
+HQ_DEV uint32_t wave_max(uint32_t m) {
+  m = max8(m);
+  m = max(m, (uint32_t)dpp<0x140>((int32_t)m));  // row_mirror
+  auto r = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+  m = max(r[0], r[1]);
+  r = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+  return __builtin_amdgcn_readfirstlane(max(r[0], r[1]));
 }
 
 HQ_DEV uint32_t key_row(uint32_t r) { return (r & ~12u) | ((r & 4u) << 1) | ((r & 8u) >> 1); }  // bits 2 and 3 swapped
@@ -688,6 +826,7 @@ template <int D, int F16>
 __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
   constexpr int ES = F16 ? 2 : 1, KS = D / 16, DT = D / 32;
   constexpr int PIECES = D * ES / 64;  // 16-byte pieces of keys, and of values, a thread stages
+  constexpr bool BOTH = D <= 128;      // whether the registers hold a step's keys and values at once
   __shared__ __align__(16) char keys[2][kPositions * D * 2];
   __shared__ __align__(16) char values[2][kPositions * D * 2];
   __shared__ __align__(16) float scales[2][2][kPositions];  // of keys, of values (times 2^-exponent)
@@ -704,7 +843,7 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
     u = __builtin_amdgcn_readfirstlane(p.edge[block]);
     end = __builtin_amdgcn_readfirstlane(p.edge[block + 1]);
     if (u >= end) return;
-    o.s = __builtin_amdgcn_readfirstlane(p.first[block].s), o.rt = __builtin_amdgcn_readfirstlane(p.first[block].rt);
+    o.s = __builtin_amdgcn_readfirstlane(p.first[block].s), o.k = __builtin_amdgcn_readfirstlane(p.first[block].k);
     o.h = __builtin_amdgcn_readfirstlane(p.first[block].h), o.step = __builtin_amdgcn_readfirstlane(p.first[block].step);
   }
   while (true) {
@@ -712,9 +851,11 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
     const Attention &a = call->a;
     const Cache c = call->c;
     const Batch b = call->b;
-    const int32_t group = a.heads / c.heads, reach = b.width << c.shift, mask = (1 << c.shift) - 1;
+    const Share sh = call->sh;
+    const int32_t group = sh.group, reach = b.width << c.shift, mask = (1 << c.shift) - 1;
     const Sequence q = wave_sequence_of(b, o.s);
-    const Tile tile = tile_of(a, c, b, call->sh, q, group, o.rt);
+    const int32_t tiles = (q.count * group + kRows - 1) / kRows;
+    const Tile tile = tile_of(*call, q, tile_at(o.k, tiles));
     const int32_t steps = min(tile.steps - o.step, end - u);
     // ---- the rows' queries
     const int thread = opaque_lane(threadIdx.x), m32 = thread & 31, h2 = (thread >> 5) & 1;
@@ -722,13 +863,13 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
     const int32_t r0 = tile.r0 + 32 * wave, r1 = min(r0 + 32, tile.r1), before = q.length - q.count;
     const bool some = r0 < tile.r1, live = r0 + m32 < r1;
     const int32_t row = live ? r0 + m32 : tile.r0;
-    const int32_t token = row / group, g = row - token * group;
+    const int32_t token = token_of(sh, row), g = row - token * group;
     const int32_t sees = before + token + 1;
     const int32_t to = min(sees, reach), from = a.window ? sees - a.window : 0;  // the lane's row's own positions
     // what some of the wave's rows see lies before any_to, what all of them see in [every_from, every_to)
-    const int32_t any_to = some ? min(before + (r1 - 1) / group + 1, reach) : 0;
-    const int32_t every_to = some ? min(before + r0 / group + 1, reach) : 0;
-    const int32_t every_from = some && a.window ? before + (r1 - 1) / group + 1 - a.window : 0;
+    const int32_t any_to = some ? min(before + token_of(sh, r1 - 1) + 1, reach) : 0;
+    const int32_t every_to = some ? min(before + token_of(sh, r0) + 1, reach) : 0;
+    const int32_t every_from = some && a.window ? before + token_of(sh, r1 - 1) + 1 - a.window : 0;
     v8h qh[KS], ql[KS];
     float rowf;
     {
@@ -742,7 +883,7 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
       most = max_pair(most);
       const int up = most > 0.0f ? min(140 - (int)(__float_as_uint(most) >> 23), 126) : 0;
       const float by = live ? power_of_2(up) : 0.0f;
-      rowf = a.scale * power_of_2(-up) * (a.cap == 0.0f ? kLog2e : 1.0f);
+      rowf = a.scale * power_of_2(-up);
 #pragma unroll
       for (int k = 0; k < KS; k++) {
         const int at = 16 * k + 8 * h2;
@@ -752,11 +893,14 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
         halves_of(e, qh[k], ql[k]);
       }
     }
-    const float cap = a.cap, per_cap = 1.0f / cap;
+    // (as in few_kernel)
+    const float cap = a.cap, row_cap = rowf / cap;
+    rowf = cap > 0.0f ? 1.0f : rowf * kLog2e;
     // ---- staging: the wave's 16 keys (consecutive in memory), the thread's 16 (8) positions of some dimensions, a scale a lane
     // (what the thread's number gives is formed anew in every step: registers are what the rows leave few of)
     constexpr int ROW = D * ES / 16, PARTS = F16 ? 8 : 4, EACH = kPositions / PARTS;
-    uint4 reg[PIECES];  // the next step's keys, then its values
+    uint4 reg[BOTH ? 2 * PIECES : PIECES];  // the next step's keys and its values, or one after the other
+    constexpr int V0 = BOTH ? PIECES : 0;
     float sreg;
     const float *scale_at = wave ? c.vs : c.ks;  // (waves 0 and 1)
     int32_t kpage, vpage, spage;  // of the step to load next
@@ -788,7 +932,7 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
 #pragma unroll
       for (int i = 0; i < PIECES; i++) {
         const int d = (int)(tid / PARTS) + i * (256 / PARTS);
-        reg[i] = *(const uint4 *)(vp + (min(d, c.dim - 1) << c.shift) * ES);  // (past dim: the last again)
+        reg[V0 + i] = *(const uint4 *)(vp + (min(d, c.dim - 1) << c.shift) * ES);  // (past dim: the last again)
       }
       const int32_t at = base + (int32_t)ln;
       const bool there = spage >= 0 && at >= tile.from && at < tile.to;
@@ -823,7 +967,7 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
         const int d = (int)(tid / PARTS) + i * (256 / PARTS);
         char *to_row = values[buf] + d * (kPositions * 2);
         if (F16) {
-          uint4 w = reg[i];
+          uint4 w = reg[V0 + i];
           if (keep_bits != 0xffu) {
             uint32_t *e = (uint32_t *)&w;
 #pragma unroll
@@ -834,23 +978,20 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
           }
           *(uint4 *)(to_row + 16 * (part ^ (d & 7))) = w;
         } else {
-          *(v8h *)(to_row + 16 * ((2 * part) ^ (d & 7))) = widen8(reg[i].x, reg[i].y);
-          *(v8h *)(to_row + 16 * ((2 * part + 1) ^ (d & 7))) = widen8(reg[i].z, reg[i].w);
+          *(v8h *)(to_row + 16 * ((2 * part) ^ (d & 7))) = widen8(reg[V0 + i].x, reg[V0 + i].y);
+          *(v8h *)(to_row + 16 * ((2 * part + 1) ^ (d & 7))) = widen8(reg[V0 + i].z, reg[V0 + i].w);
         }
       }
       if (wave == 0) scales[buf][0][ln] = sreg;
       if (wave == 1) {
-        float wide = sreg;
-#pragma unroll
-        for (int i = 32; i > 0; i >>= 1) wide = fmaxf(wide, __shfl_xor(wide, i, 64));
-        const int e1 = __builtin_amdgcn_readfirstlane((int)(__float_as_uint(wide) >> 23) - 127);
-        if (e1 > exponent_run && e1 < 128) exponent_run = e1;  // (128: nothing but NaN)
+        const int e1 = (int)(wave_max(sreg == sreg ? __float_as_uint(sreg) : 0u) >> 23) - 127;
+        if (e1 > exponent_run) exponent_run = e1;
         scales[buf][1][ln] = sreg * power_of_2(-exponent_run);
         if (ln == 0) info[buf][0] = exponent_run, info[buf][1] = on_page;
       }
     };
     {
-      const int32_t now[10] = {u, end, block, o.rt, o.step, steps, tile.steps, q.begin, q.count, o.h};
+      const int32_t now[10] = {u, end, block, o.k, o.step, steps, tile.steps, q.begin, q.count, o.h};
 #pragma unroll
       for (int i = 0; i < 10; i++) parked[wave][i] = now[i];
     }
@@ -871,7 +1012,13 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
     __syncthreads();
     for (int buf = 0; base < stop; base += kPositions, buf ^= 1) {
       const bool more = base + kPositions < stop;
-      if (more) load_keys(base + kPositions);
+      if (more) {
+        load_keys(base + kPositions);
+        if (BOTH) {
+          load_values(base + kPositions);
+          pages_at(base + 2 * kPositions);
+        }
+      }
       // 32 positions at a time, as the registers allow
 #pragma unroll 1
       for (int t = 0; t < 2; t++) {
@@ -894,12 +1041,12 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
           for (int i = 0; i < 2; i++) {
             const v4f k0 = *(const v4f *)(sc + 16 * i), k1 = *(const v4f *)(sc + 16 * i + 4);
 #pragma unroll
-            for (int e = 0; e < 8; e++) p[8 * i + e] = s[8 * i + e] * (e < 4 ? k0[e & 3] : k1[e & 3]) * rowf;
+            for (int e = 0; e < 8; e++) p[8 * i + e] = s[8 * i + e] * (e < 4 ? k0[e & 3] : k1[e & 3]);
           }
           if (cap > 0.0f) {
             const float bend = opaque(0.55f), twice = opaque(2.0f * kLog2e);
 #pragma unroll
-            for (int e = 0; e < 16; e++) p[e] = cap * kLog2e * tanh_of(p[e] * per_cap, bend, twice);
+            for (int e = 0; e < 16; e++) p[e] = cap * kLog2e * tanh_of(p[e] * row_cap, bend, twice);
           }
           const bool edge = at32 + 32 > every_to || at32 < every_from || pages_here != 3;
           uint32_t seen = ~0u;
@@ -913,7 +1060,7 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
           float most = p[0];
 #pragma unroll
           for (int e = 1; e < 16; e++) most = fmaxf(most, p[e]);
-          most = max_pair(most);
+          most = max_pair(most) * rowf;
           if (__any(most > m + kRoom)) {
             const float m1 = fmaxf(m, most);
             const float alpha = m1 == -INFINITY ? 0.0f : exp2_of(m - m1);
@@ -936,7 +1083,7 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
             const v4f v0 = *(const v4f *)(sc + kPositions + 16 * i), v1 = *(const v4f *)(sc + kPositions + 16 * i + 4);
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-              const float w = exp2_of(p[8 * i + e] - less);
+              const float w = exp2_of(__builtin_fmaf(p[8 * i + e], rowf, -less));
               l += w;
               p[8 * i + e] = w * (e < 4 ? v0[e & 3] : v1[e & 3]);
             }
@@ -958,13 +1105,16 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
             }
           }
         }
-        if (more && t == 0) {
+        if (!BOTH && more && t == 0) {
           store_keys(buf ^ 1);
           load_values(base + kPositions);
           pages_at(base + 2 * kPositions);
         }
       }
-      if (more) store_values(buf ^ 1);
+      if (more) {
+        if (BOTH) store_keys(buf ^ 1);
+        store_values(buf ^ 1);
+      }
       __syncthreads();
     }
     l = sum_pair(l);
@@ -973,14 +1123,14 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
     int32_t kept_back[10];
 #pragma unroll
     for (int i = 0; i < 10; i++) kept_back[i] = __builtin_amdgcn_readfirstlane(parked[wave][i]);
-    u = kept_back[0], end = kept_back[1], block = kept_back[2], o.rt = kept_back[3], o.step = kept_back[4], o.h = kept_back[9];
+    u = kept_back[0], end = kept_back[1], block = kept_back[2], o.k = kept_back[3], o.step = kept_back[4], o.h = kept_back[9];
     const int32_t done = kept_back[5], begin = kept_back[7], count = kept_back[8];
     const bool whole = done == kept_back[6];
     if (live) {
       const int thread = opaque_lane(threadIdx.x), m32 = thread & 31, h2 = (thread >> 5) & 1, wave = thread >> 6;
       const float by = power_of_2(exponent);
       if (whole) {
-        const int32_t heads = after->a.heads, shared = heads / after->c.heads, dim = after->c.dim;
+        const int32_t shared = after->sh.group, dim = after->c.dim;
         const float per = l != 0.0f ? by / l : 0.0f;
         float *out = (float *)(after->a.out + (begin + token) * after->a.out_stride) + (int64_t)(o.h * shared + g) * dim;
 #pragma unroll
@@ -1005,11 +1155,19 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
       }
     }
     u += done;
-    if (u >= end) break;
+    if (u >= end) {
+      if (threadIdx.x == 0 && o.step == 0 && !whole) {
+        Tail &tail = ((Tail *)after->a.work)[block];
+        const int32_t rows = count * after->sh.group, r0 = kRows * tile_at(o.k, (rows + kRows - 1) / kRows);
+        tail.begin = begin, tail.r0 = r0, tail.rows = min(kRows, rows - r0), tail.h = o.h;
+        tail.last = end - done + kept_back[6] - 1;
+      }
+      break;
+    }
     // ---- the next item: the next row tile, head or sequence (one more step is left, so there is one)
     o.step = 0;
-    if (++o.rt * kRows >= count * (after->a.heads / after->c.heads)) {
-      o.rt = 0;
+    if (++o.k * kRows >= count * after->sh.group) {
+      o.k = 0;
       if (++o.h == after->c.heads) {
         o.h = 0;
         do {
@@ -1020,64 +1178,31 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
   }
 }
 
-// what blocks found of an item that they shared, a wave a row: the block whose share it starts in joins the parts
-template <int D>
-__global__ __launch_bounds__(256) void rows_join_kernel(Attention a, Cache c, Batch b, Share sh) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int32_t group = a.heads / c.heads;
-  const Plan p = plan_of(a.work, sh.blocks, b.sequences);
-  const int32_t start = p.edge[blockIdx.x], end = p.edge[blockIdx.x + 1];
-  if (start >= end || end >= p.edge[sh.blocks]) return;
-  const Start o = p.last[blockIdx.x];
-  const Sequence q = sequence_of(b, o.s);
-  const Tile t = tile_of(a, c, b, sh, q, group, o.rt);
-  const int32_t first = end - 1 - o.step, last = first + t.steps - 1;  // the item's steps
-  if (first < start || last < end) return;
-  const int r = blockIdx.y * 4 + wave;
-  if (t.r0 + r >= t.r1) return;
-  const int64_t size = kRows * (D + 2);
-  const float *parts = (const float *)(a.work + sh.parts);
-  float m = -INFINITY, l = 0.0f;
-  float acc[D / 64] = {};
-  for (int32_t at = blockIdx.x, slot = 1; at < sh.blocks && p.edge[at] <= last; at++, slot = 0) {
-    if (p.edge[at + 1] <= p.edge[at]) {  // (a share without steps)
-      continue;
-    }
-    const float *part = parts + (int64_t)(at * 2 + slot) * size;
-    const float pm = part[r * 2], pl = part[r * 2 + 1];
-    const float m1 = fmaxf(m, pm), ref = m1 == -INFINITY ? 0.0f : m1;
-    const float f0 = exp2_of(m - ref), f1 = exp2_of(pm - ref);
-    m = m1;
-    l = l * f0 + pl * f1;
-#pragma unroll
-    for (int i = 0; i < D / 64; i++) acc[i] = acc[i] * f0 + part[kRows * 2 + r * D + lane + 64 * i] * f1;
-  }
-  const int32_t i0 = (t.r0 + r) / group, g = t.r0 + r - i0 * group;
-  float *out = (float *)(a.out + (q.begin + i0) * a.out_stride) + (int64_t)(o.h * group + g) * c.dim;
-#pragma unroll
-  for (int i = 0; i < D / 64; i++)
-    if (lane + 64 * i < c.dim) out[lane + 64 * i] = l != 0.0f ? acc[i] / l : 0.0f;
-}
-
 int padded(int32_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
 // How a call's steps are shared: by as many blocks as the GPU holds, or as there can be steps.
+Share share_of(const Cache &c, const Batch &b, int32_t heads, int32_t a_cu, int32_t rows_of_a_tile, int32_t log, bool plan) {
+  Share sh{};
+  sh.rows = rows_of_a_tile, sh.log = log, sh.group = heads / c.heads;
+  sh.per = sh.group > 1 ? (uint32_t)((((uint64_t)1 << 32) + sh.group - 1) / sh.group) : 0;
+  const int64_t rows = (int64_t)b.tokens * sh.group;
+  const int64_t tiles = std::min(rows, rows / rows_of_a_tile + b.sequences);
+  const int64_t steps = std::max<int64_t>((((int64_t)b.width << c.shift) + (1 << log) - 1) >> log, 1);
+  sh.blocks = (int32_t)std::min<int64_t>(a_cu * cu_count(), tiles * c.heads * steps);
+  sh.tiles = (int32_t)tiles;
+  sh.shared = steps > 1 && sh.blocks > 1;
+  sh.parts = ((plan ? plan_bytes(sh.blocks, b.sequences, tiles) : sh.blocks * (int64_t)sizeof(Tail)) + 255) / 256 * 256;
+  sh.bytes = sh.parts + (int64_t)sh.blocks * 2 * rows_of_a_tile * (padded(c.dim) + 2) * 4;
+  // (steps are counted in 32 bits, and a row's token is row ceil(2^32 / group) / 2^32)
+  sh.countable = tiles * c.heads * steps < INT32_MAX && rows * sh.group < (int64_t)1 << 32;
+  return sh;
+}
 Share few_share(const Cache &c, const Batch &b, int32_t heads) {
-  const int32_t d = padded(c.dim), positions = 16 * few_np(d, c.f16);
-  const int64_t rows = (int64_t)b.tokens * (heads / c.heads);
-  const int64_t tiles = std::min(rows, rows / kFewRows + b.sequences);
-  const int64_t steps = (((int64_t)b.width << c.shift) + positions - 1) / positions + 1;
-  const int32_t blocks = (int32_t)std::min<int64_t>(few_blocks_a_cu(d, c.f16) * 256, tiles * c.heads * steps);
-  return {blocks, kFewRows, positions, (int32_t)tiles, 0, (int64_t)blocks * 2 * kFewRows * (d + 2) * 4, tiles * c.heads * steps};
+  const int32_t d = padded(c.dim);
+  return share_of(c, b, heads, few_blocks_a_cu(d, c.f16), kFewRows, few_np(d, c.f16) == 16 ? 8 : 7, false);
 }
 Share rows_share(const Cache &c, const Batch &b, int32_t heads) {
-  const int32_t d = padded(c.dim);
-  const int64_t rows = (int64_t)b.tokens * (heads / c.heads);
-  const int64_t tiles = std::min(rows, rows / kRows + b.sequences);
-  const int64_t steps = (((int64_t)b.width << c.shift) + kPositions - 1) / kPositions + 1;
-  const int32_t blocks = (int32_t)std::min<int64_t>(rows_blocks_a_cu(d) * 256, tiles * c.heads * steps);
-  const int64_t plan = plan_bytes(blocks, b.sequences, tiles);
-  return {blocks, kRows, kPositions, (int32_t)tiles, plan, plan + (int64_t)blocks * 2 * kRows * (d + 2) * 4, tiles * c.heads * steps};
+  return share_of(c, b, heads, rows_blocks_a_cu(padded(c.dim)), kRows, 6, true);
 }
 
 // whether few_kernel takes the call: no sequence has more rows of a head than two of its tiles (8 sequences of 5 tokens, 20 rows,
@@ -1086,15 +1211,17 @@ bool few_rows(const Cache &c, const Batch &b, int32_t heads) { return (int64_t)b
 
 template <int D>
 hipError_t launch(const Attention &a, const Cache &c, const Batch &b, hipStream_t s) {
-  if (few_rows(c, b, a.heads)) {
-    const Share sh = few_share(c, b, a.heads);
-    hipLaunchKernelGGL((c.f16 ? few_kernel<D, 1> : few_kernel<D, 0>), dim3(sh.blocks), dim3(256), 0, s, Call{a, c, b, sh});
-    if (sh.blocks > 1) hipLaunchKernelGGL(join_kernel<D>, dim3(sh.blocks, kFewRows / 4), dim3(256), 0, s, a, c, b, sh);
+  const bool few = few_rows(c, b, a.heads);
+  const Call call{a, c, b, few ? few_share(c, b, a.heads) : rows_share(c, b, a.heads)};
+  const dim3 blocks(call.sh.blocks);
+  if (few) {
+    hipLaunchKernelGGL((c.f16 ? few_kernel<D, 1> : few_kernel<D, 0>), blocks, dim3(256), 0, s, call);
+    if (call.sh.shared) hipLaunchKernelGGL(join_kernel<D>, blocks, dim3(256), 0, s, call, nullptr);
   } else {
-    const Share sh = rows_share(c, b, a.heads);
-    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, s, a, c, b, sh);
-    hipLaunchKernelGGL((c.f16 ? rows_kernel<D, 1> : rows_kernel<D, 0>), dim3(sh.blocks), dim3(256), 0, s, Call{a, c, b, sh});
-    if (sh.blocks > 1) hipLaunchKernelGGL(rows_join_kernel<D>, dim3(sh.blocks, kRows / 4), dim3(256), 0, s, a, c, b, sh);
+    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, s, call);
+    hipLaunchKernelGGL((c.f16 ? rows_kernel<D, 1> : rows_kernel<D, 0>), blocks, dim3(256), 0, s, call);
+    const Plan p = plan_of(a.work, call.sh.blocks, b.sequences);
+    if (call.sh.shared) hipLaunchKernelGGL(join_kernel<D>, dim3(call.sh.blocks, 4), dim3(256), 0, s, call, (const int32_t *)p.edge);
   }
   return hipGetLastError();
 }
@@ -1104,7 +1231,7 @@ hipError_t launch(const Attention &a, const Cache &c, const Batch &b, hipStream_
 int64_t attention_work_bytes(const Cache &c, const Batch &b, int32_t heads) {
   if (b.tokens <= 0 || b.sequences <= 0) return 0;
   const Share few = few_share(c, b, heads), rows = rows_share(c, b, heads);
-  if (few.most > INT32_MAX || rows.most > INT32_MAX) return -1;  // (steps are counted in 32 bits)
+  if (!few.countable || !rows.countable) return -1;
   return few_rows(c, b, heads) ? few.bytes : rows.bytes;
 }
 
