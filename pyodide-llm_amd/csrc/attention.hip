@@ -576,78 +576,53 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
   }
 }
 
-// The parts of a row of an item that blocks share, joined by a wave: those of `parts` (two of `size` floats a block: rows' (m, l)
-// pairs, then rows of D) of block `at` (its second) and the blocks after it (their first) whose share starts in the item, which
-// start_of(block) says; `last` is the item's last step.  Lane i looks at the i-th block; then every lane sums D / 64 values.
-template <int D, typename StartOf>
-HQ_DEV void join_row(const float *parts, int64_t size, int rows, int r, int32_t at, int32_t blocks, int32_t last, StartOf start_of,
-                     float &l, float *acc) {
-  const int lane = threadIdx.x & 63;
-  float m = -INFINITY;
-  l = 0.0f;
-#pragma unroll
-  for (int i = 0; i < D / 64; i++) acc[i] = 0.0f;
-  for (int32_t b0 = at; b0 < blocks; b0 += 64) {
-    const int32_t mine = b0 + lane;
-    const int32_t start = mine < blocks ? start_of(mine) : INT32_MAX;
-    const bool in = start <= last;
-    const uint64_t all = __ballot(in);
-    if (!all) break;
-    const bool some = in && start_of(mine + 1) > start;  // (a share may have no step)
-    const float *part = parts + ((int64_t)mine * 2 + (mine == at ? 1 : 0)) * size;
-    const float pm = some ? part[2 * r] : -INFINITY, pl = some ? part[2 * r + 1] : 0.0f;
-    float m1 = fmaxf(m, pm);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m1 = fmaxf(m1, __shfl_xor(m1, o, 64));
-    const float ref = m1 == -INFINITY ? 0.0f : m1, f0 = exp2_of(m - ref), f = some ? exp2_of(pm - ref) : 0.0f;
-    float sum = pl * f;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    m = m1;
-    l = l * f0 + sum;
-#pragma unroll
-    for (int i = 0; i < D / 64; i++) acc[i] *= f0;
-    const uint64_t with = __ballot(some);
-    const int n = 64 - __builtin_clzll(all);
-    constexpr int AHEAD = 8;  // parts' loads on their way
-    for (int i0 = 0; i0 < n; i0 += AHEAD) {
-      float v[AHEAD][D / 64], fi[AHEAD];
-#pragma unroll
-      for (int j = 0; j < AHEAD; j++) {
-        const int i = min(i0 + j, 63);
-        const bool there = i0 + j < n && (with >> i & 1);
-        fi[j] = there ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), i)) : 0.0f;
-        const int32_t of = there ? b0 + i : at;  // (the first part is there always)
-        const float *row = parts + ((int64_t)of * 2 + (of == at ? 1 : 0)) * size + 2 * rows + r * D + (D / 64) * lane;
-#pragma unroll
-        for (int k = 0; k < D / 64; k++) v[j][k] = row[k];
-      }
-#pragma unroll
-      for (int j = 0; j < AHEAD; j++)
-#pragma unroll
-        for (int k = 0; k < D / 64; k++) acc[k] += v[j][k] * fi[j];
-    }
-    if (all != ~0ull) break;
-  }
-}
-
 // The items that blocks share: the block whose share an item starts in (and does not end in) has its rows' parts joined here, a
-// wave a row.  edge: the shares' edges (NULL: even shares of all steps).
+// thread 4 values of a row: the largest of the parts' maxima, then their sum.  A block's parts are two of (rows' (m, l) pairs, rows
+// of D): what its first item's end and its last item's start gave.  edge: the shares' edges (NULL: even shares of all steps).
+constexpr int kMostBlocks = 4096;  // of a launch that shares its items
 template <int D>
 __global__ __launch_bounds__(256) void join_kernel(Call k, const int32_t *edge) {
+  constexpr int ROWS = 256 / (D / 4);  // rows at a time
+  __shared__ int32_t of[kMostBlocks];  // the blocks that have a part
+  __shared__ int32_t found;
   const Tail t = ((const Tail *)k.a.work)[blockIdx.x];
-  const int32_t rows = __builtin_amdgcn_readfirstlane(t.rows), last = __builtin_amdgcn_readfirstlane(t.last);
-  if (last < 0) return;
-  const int lane = threadIdx.x & 63, step = 4 * gridDim.y;
-  for (int r = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); r < rows; r += step) {
-    float l, acc[D / 64];
-    join_row<D>((const float *)(k.a.work + k.sh.parts), (int64_t)k.sh.rows * (D + 2), k.sh.rows, r, blockIdx.x, k.sh.blocks, last,
-                [&](int32_t i) { return edge ? edge[i] : share_start(t.all, i, k.sh.blocks); }, l, acc);
+  if (t.last < 0 || (int32_t)blockIdx.y * ROWS >= t.rows) return;
+  if (threadIdx.x < 64) {
+    const int lane = threadIdx.x;
+    const auto start_of = [&](int32_t i) { return edge ? edge[i] : share_start(t.all, i, k.sh.blocks); };
+    int32_t n = 0;
+    for (int32_t b0 = blockIdx.x; b0 < k.sh.blocks; b0 += 64) {
+      const int32_t mine = b0 + lane, start = mine < k.sh.blocks ? start_of(mine) : INT32_MAX;
+      const bool in = start <= t.last, some = in && start_of(mine + 1) > start;  // (a share may have no step)
+      const uint64_t with = __ballot(some);
+      if (some) of[n + __popcll(with & (((uint64_t)1 << lane) - 1))] = 2 * mine + (mine == (int32_t)blockIdx.x ? 1 : 0);
+      n += __popcll(with);
+      if (!__all(in)) break;
+    }
+    if (lane == 0) found = n;
+  }
+  __syncthreads();
+  const int n = found, col = threadIdx.x % (D / 4) * 4;
+  const int64_t size = (int64_t)k.sh.rows * (D + 2);
+  const float *parts = (const float *)(k.a.work + k.sh.parts);
+  for (int r = blockIdx.y * ROWS + threadIdx.x / (D / 4); r < t.rows; r += ROWS * gridDim.y) {
+    float m = -INFINITY;  // (the row's threads look at a part each)
+    for (int i = threadIdx.x % (D / 4); i < n; i += D / 4) m = fmaxf(m, parts[of[i] * size + 2 * r]);
+#pragma unroll
+    for (int o = D / 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f;
+    v4f acc = {};
+#pragma unroll 16
+    for (int i = 0; i < n; i++) {
+      const float *part = parts + of[i] * size;
+      const float f = exp2_of(part[2 * r] - ref);
+      l += part[2 * r + 1] * f;
+      acc += *(const v4f *)(part + 2 * k.sh.rows + r * D + col) * f;
+    }
     const int32_t i0 = token_of(k.sh, t.r0 + r), g = t.r0 + r - i0 * k.sh.group;
     float *out = (float *)(k.a.out + (t.begin + i0) * k.a.out_stride) + (int64_t)(t.h * k.sh.group + g) * k.c.dim;
-#pragma unroll
-    for (int i = 0; i < D / 64; i++)
-      if ((D / 64) * lane + i < k.c.dim) out[(D / 64) * lane + i] = l != 0.0f ? acc[i] / l : 0.0f;
+    if (col < k.c.dim) *(v4f *)(out + col) = l != 0.0f ? acc / l : v4f{0.f, 0.f, 0.f, 0.f};
   }
 }
 
@@ -1188,7 +1163,7 @@ Share share_of(const Cache &c, const Batch &b, int32_t heads, int32_t a_cu, int3
   const int64_t rows = (int64_t)b.tokens * sh.group;
   const int64_t tiles = std::min(rows, rows / rows_of_a_tile + b.sequences);
   const int64_t steps = std::max<int64_t>((((int64_t)b.width << c.shift) + (1 << log) - 1) >> log, 1);
-  sh.blocks = (int32_t)std::min<int64_t>(a_cu * cu_count(), tiles * c.heads * steps);
+  sh.blocks = (int32_t)std::min<int64_t>(std::min(a_cu * cu_count(), kMostBlocks), tiles * c.heads * steps);
   sh.tiles = (int32_t)tiles;
   sh.shared = steps > 1 && sh.blocks > 1;
   sh.parts = ((plan ? plan_bytes(sh.blocks, b.sequences, tiles) : sh.blocks * (int64_t)sizeof(Tail)) + 255) / 256 * 256;
@@ -1214,15 +1189,17 @@ hipError_t launch(const Attention &a, const Cache &c, const Batch &b, hipStream_
   const bool few = few_rows(c, b, a.heads);
   const Call call{a, c, b, few ? few_share(c, b, a.heads) : rows_share(c, b, a.heads)};
   const dim3 blocks(call.sh.blocks);
+  const int32_t *edge = nullptr;
   if (few) {
     hipLaunchKernelGGL((c.f16 ? few_kernel<D, 1> : few_kernel<D, 0>), blocks, dim3(256), 0, s, call);
-    if (call.sh.shared) hipLaunchKernelGGL(join_kernel<D>, blocks, dim3(256), 0, s, call, nullptr);
   } else {
+    edge = plan_of(a.work, call.sh.blocks, b.sequences).edge;
     hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, s, call);
     hipLaunchKernelGGL((c.f16 ? rows_kernel<D, 1> : rows_kernel<D, 0>), blocks, dim3(256), 0, s, call);
-    const Plan p = plan_of(a.work, call.sh.blocks, b.sequences);
-    if (call.sh.shared) hipLaunchKernelGGL(join_kernel<D>, dim3(call.sh.blocks, 4), dim3(256), 0, s, call, (const int32_t *)p.edge);
   }
+  // (a block of join_kernel takes 1024 / D rows at a time)
+  const dim3 join(call.sh.blocks, std::min(call.sh.rows * D / 1024, 8));
+  if (call.sh.shared) hipLaunchKernelGGL(join_kernel<D>, join, dim3(256), 0, s, call, edge);
   return hipGetLastError();
 }
 
