@@ -46,6 +46,8 @@ struct Share {
   uint32_t per;       // ceil(2^32 / group) (0: group is 1): the token of a row without a division
   int32_t tiles;      // there can be
   bool shared;        // whether an item can have more than one step
+  // few_kernel: 0, or how many row tiles a sequence has a block a head for, which takes its tile's positions whole
+  int32_t whole;
   int64_t parts;      // where in the workspace the shared items' parts are
   int64_t bytes;      // the workspace
   bool countable;     // whether its numbers fit their types
@@ -80,8 +82,7 @@ HQ_DEV Tile tile_of(const Call &k, const Sequence &q, int32_t rt) {
 }
 
 // the steps of a sequence's tiles over all heads
-HQ_DEV int32_t steps_of(const Call &k, int32_t s) {
-  const Sequence q = sequence_of(k.b, s);
+HQ_DEV int32_t steps_of(const Call &k, const Sequence &q) {
   const int32_t rows = q.count * k.sh.group;
   int32_t n = 0;
   for (int32_t rt = 0; rt * kFewRows < rows; rt++) n += tile_of(k, q, rt).steps;
@@ -96,14 +97,18 @@ struct Spot {
 };
 
 // the sums up to each lane's value; INT32_MAX where they pass it (which sequences that overlap could make them)
+template <int CTRL, int ROWS>
+HQ_DEV int32_t plus_dpp(int32_t v) {
+  const uint32_t w = (uint32_t)__builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+  return (int32_t)min((uint32_t)v + w, (uint32_t)INT32_MAX);
+}
 HQ_DEV int32_t wave_sums_of(int32_t v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t w = (uint32_t)__shfl_up(v, o, 64);
-    if (lane >= o) v = (int32_t)min((uint32_t)v + w, (uint32_t)INT32_MAX);
-  }
-  return v;
+  v = plus_dpp<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8: within a row of 16
+  v = plus_dpp<0x112, 0xf>(v);
+  v = plus_dpp<0x114, 0xf>(v);
+  v = plus_dpp<0x118, 0xf>(v);
+  v = plus_dpp<0x142, 0xa>(v);  // row_bcast 15: the row before, into rows 1 and 3
+  return plus_dpp<0x143, 0xc>(v);  // row_bcast 31: the first half, into the second
 }
 
 HQ_DEV int32_t share_start(int32_t steps, int32_t block, int32_t blocks) {
@@ -116,12 +121,20 @@ HQ_DEV int32_t share_start(int32_t steps, int32_t block, int32_t blocks) {
 HQ_DEV void find_share(const Call &k, int32_t block, int32_t &all, int32_t &u, int32_t &end, Spot &o) {
   const int lane = threadIdx.x & 63;
   const int32_t n = k.b.sequences;
-  int32_t mine = lane < n ? steps_of(k, lane) : 0, upto = wave_sums_of(mine);
-  uint32_t total = (uint32_t)__builtin_amdgcn_readlane(upto, 63);
+  Sequence q;
+  int32_t mine, upto;
+  const auto look = [&](int32_t s0) {  // at 64 sequences
+    q = sequence_of(k.b, min(s0 + lane, n - 1));
+    mine = s0 + lane < n ? steps_of(k, q) : 0;
+    upto = wave_sums_of(mine);
+  };
+  uint32_t total = 0;
   for (int32_t s0 = 64; s0 < n; s0 += 64) {
-    const int32_t more = wave_sums_of(s0 + lane < n ? steps_of(k, s0 + lane) : 0);
-    total = min(total + (uint32_t)__builtin_amdgcn_readlane(more, 63), (uint32_t)INT32_MAX);
+    look(s0);
+    total = min(total + (uint32_t)__builtin_amdgcn_readlane(upto, 63), (uint32_t)INT32_MAX);
   }
+  look(0);
+  total = min(total + (uint32_t)__builtin_amdgcn_readlane(upto, 63), (uint32_t)INT32_MAX);
   all = total < (uint32_t)INT32_MAX ? (int32_t)total : 0;
   u = share_start(all, block, k.sh.blocks), end = share_start(all, block + 1, k.sh.blocks);
   if (u >= end) return;
@@ -130,12 +143,13 @@ HQ_DEV void find_share(const Call &k, int32_t block, int32_t &all, int32_t &u, i
   while (!(past = __ballot(upto > rest))) {  // (all steps are more than u: one chunk has it)
     rest -= __builtin_amdgcn_readlane(upto, 63);
     s0 += 64;
-    mine = s0 + lane < n ? steps_of(k, s0 + lane) : 0, upto = wave_sums_of(mine);
+    look(s0);
   }
   const int l = __ffsll((unsigned long long)past) - 1;
   rest -= __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(mine, l);
   o.s = s0 + l, o.rt = 0;
-  o.q = wave_sequence_of(k.b, o.s);
+  o.q.begin = __builtin_amdgcn_readlane(q.begin, l), o.q.count = __builtin_amdgcn_readlane(q.count, l);
+  o.q.length = __builtin_amdgcn_readlane(q.length, l);
   for (;; o.rt++) {
     o.t = tile_of(k, o.q, o.rt);
     if (rest < o.t.steps * k.c.heads || (o.rt + 1) * kFewRows >= o.q.count * k.sh.group) break;
@@ -298,8 +312,14 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
   const int m16 = lane & 15, q4 = lane >> 4;
   int32_t u, end;
   Spot o;
-  {
-    const Call *k = call_again();
+  const Call *k = call_again();
+  if (k->sh.whole) {
+    o.s = blockIdx.x, o.rt = blockIdx.y, o.h = blockIdx.z, o.step = 0;
+    o.q = wave_sequence_of(k->b, o.s);
+    if (o.rt * kFewRows >= o.q.count * k->sh.group) return;
+    o.t = tile_of(*k, o.q, o.rt);
+    u = 0, end = o.t.steps;
+  } else {
     int32_t all;
     find_share(*k, blockIdx.x, all, u, end, o);
     // (no tail yet: the share's last item says whether it has one)
@@ -319,19 +339,67 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
     const bool live = row < o.t.r1;
     const int32_t token = token_of(sh, live ? row : o.t.r0), g = (live ? row : o.t.r0) - token * group;
     const float *x = (const float *)(a.q + (o.q.begin + token) * a.q_stride) + (int64_t)(o.h * group + g) * c.dim;
+    float4 raw[DB][4];
+#pragma unroll
+    for (int d = 0; d < DB; d++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int at = 64 * d + 16 * q4 + 4 * i;
+        raw[d][i] = live && at < c.dim ? *(const float4 *)(x + at) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    // ---- the wave's positions: WK from base on, every STEP; their first loads are on their way before the queries are used
+    int32_t base = (o.t.first + o.step) * STEP + WK * wave;
+    const int32_t stop = min((o.t.first + o.step + steps) * STEP, o.t.to);
+    while (base + WK <= o.t.from) base += STEP;
+    const int32_t next0 = base + STEP < stop ? base + STEP : base;  // (the last step loads itself again)
+    const int32_t page1 = page_of(b, c, o.s, base + NP * (m16 >> 2));
+    int32_t page2 = page_of(b, c, o.s, base + NP * q4);
+    int32_t next = next0, next1 = page_of(b, c, o.s, next + NP * (m16 >> 2)), next2 = page_of(b, c, o.s, next + NP * q4);
+    // Registers are loaded for the next step as soon as this one has used them: keys after the scores, scales after the weights,
+    // values after their products, so that a step's bytes are always on their way.
+    Elements<F16, 16> kk[NP / 4][DB];
+    Elements<F16, NP> vv[DT];
+    float ks[NP], vs[NP];
+    const auto load_keys = [&](int32_t at, int32_t page) {
+      const int64_t vec = vectors_of(c, max(page, 0), o.h) + ((at + NP * (m16 >> 2)) & mask) + (m16 & 3);
+      const int32_t dim = opaque(c.dim);
+      const char *p = c.k + vec * dim * ES;
+#pragma unroll
+      for (int t = 0; t < NP / 4; t++)
+#pragma unroll
+        for (int d = 0; d < DB; d++)
+          // (dimensions past dim: the row's first, times zeros)
+          kk[t][d].load(p + (t * 4 * dim + (64 * d + 16 * q4 < dim ? 64 * d + 16 * q4 : 0)) * ES);
+    };
+    // the lane's NP positions from at + NP q4 on, on `page`
+    const auto load_scales = [&](int32_t at, int32_t page) {
+      const int64_t vec = vectors_of(c, max(page, 0), o.h) + ((at + NP * q4) & mask);
+#pragma unroll
+      for (int i = 0; i < NP / 4; i++) {
+        *(float4 *)(ks + 4 * i) = *(const float4 *)(c.ks + vec + 4 * i);
+        *(float4 *)(vs + 4 * i) = *(const float4 *)(c.vs + vec + 4 * i);
+      }
+    };
+    const auto values_at = [&](int32_t at, int32_t page) {
+      return c.v + (vectors_of(c, max(page, 0), o.h) * c.dim + (m16 << c.shift) + ((at + NP * q4) & mask)) * ES;
+    };
+    const auto value_row = [&](int d, int32_t dim, int32_t shift) { return (min(d * 16, dim - 16) << shift) * ES; };  // (past dim: the last again)
+    if (base < stop) {
+      load_keys(base, page1);
+      load_scales(base, page2);
+      const char *p = values_at(base, page2);
+#pragma unroll
+      for (int d = 0; d < DT; d++) vv[d].load(p + value_row(d, c.dim, c.shift));
+    }
     v8h qh[DB][2], ql[DB][2];
     float rowf;
     {
-      float4 f[DB][4];
       float most = 0.0f;
 #pragma unroll
       for (int d = 0; d < DB; d++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int at = 64 * d + 16 * q4 + 4 * i;
-          f[d][i] = live && at < c.dim ? *(const float4 *)(x + at) : make_float4(0.f, 0.f, 0.f, 0.f);
-          most = fmaxf(fmaxf(most, fmaxf(fabsf(f[d][i].x), fabsf(f[d][i].y))), fmaxf(fabsf(f[d][i].z), fabsf(f[d][i].w)));
-        }
+        for (int i = 0; i < 4; i++)
+          most = fmaxf(fmaxf(most, fmaxf(fabsf(raw[d][i].x), fabsf(raw[d][i].y))), fmaxf(fabsf(raw[d][i].z), fabsf(raw[d][i].w)));
       most = max_row(most);
       const int up = most > 0.0f ? min(140 - (int)(__float_as_uint(most) >> 23), 126) : 0;
       const float by = power_of_2(up);
@@ -340,7 +408,7 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
       for (int d = 0; d < DB; d++)
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-          const float4 e0 = f[d][2 * i], e1 = f[d][2 * i + 1];
+          const float4 e0 = raw[d][2 * i], e1 = raw[d][2 * i + 1];
           const float e[8] = {e0.x * by, e0.y * by, e0.z * by, e0.w * by, e1.x * by, e1.y * by, e1.z * by, e1.w * by};
           halves_of(e, qh[d][i], ql[d][i]);
         }
@@ -358,53 +426,10 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
 #pragma unroll
       for (int i = 0; i < 13; i++) parked[wave][i] = now[i];
     }
-    // ---- the wave's positions: WK from base on, every STEP
     float m = -INFINITY, l = 0.0f;
     int exponent = kLeast;
     v4f acc[DT] = {};
-    int32_t base = (o.t.first + o.step) * STEP + WK * wave;
-    const int32_t stop = min((o.t.first + o.step + steps) * STEP, o.t.to);
-    while (base + WK <= o.t.from) base += STEP;
     if (base < stop) {
-      // Registers are loaded for the next step as soon as this one has used them: keys after the scores, scales after the weights,
-      // values after their products, so that a step's bytes are always on their way.
-      Elements<F16, 16> kk[NP / 4][DB];
-      Elements<F16, NP> vv[DT];
-      float ks[NP], vs[NP];
-      const auto load_keys = [&](int32_t at, int32_t page) {
-        const int64_t vec = vectors_of(c, max(page, 0), o.h) + ((at + NP * (m16 >> 2)) & mask) + (m16 & 3);
-        const int32_t dim = opaque(c.dim);
-        const char *p = c.k + vec * dim * ES;
-#pragma unroll
-        for (int t = 0; t < NP / 4; t++)
-#pragma unroll
-          for (int d = 0; d < DB; d++)
-            // (dimensions past dim: the row's first, times zeros)
-            kk[t][d].load(p + (t * 4 * dim + (64 * d + 16 * q4 < dim ? 64 * d + 16 * q4 : 0)) * ES);
-      };
-      // the lane's NP positions from at + NP q4 on, on `page`
-      const auto load_scales = [&](int32_t at, int32_t page) {
-        const int64_t vec = vectors_of(c, max(page, 0), o.h) + ((at + NP * q4) & mask);
-#pragma unroll
-        for (int i = 0; i < NP / 4; i++) {
-          *(float4 *)(ks + 4 * i) = *(const float4 *)(c.ks + vec + 4 * i);
-          *(float4 *)(vs + 4 * i) = *(const float4 *)(c.vs + vec + 4 * i);
-        }
-      };
-      const auto values_at = [&](int32_t at, int32_t page) {
-        return c.v + (vectors_of(c, max(page, 0), o.h) * c.dim + (m16 << c.shift) + ((at + NP * q4) & mask)) * ES;
-      };
-      const auto value_row = [&](int d, int32_t dim, int32_t shift) { return (min(d * 16, dim - 16) << shift) * ES; };  // (past dim: the last again)
-      int32_t page2 = page_of(b, c, o.s, base + NP * q4);
-      load_keys(base, page_of(b, c, o.s, base + NP * (m16 >> 2)));
-      load_scales(base, page2);
-      {
-        const char *p = values_at(base, page2);
-#pragma unroll
-        for (int d = 0; d < DT; d++) vv[d].load(p + value_row(d, c.dim, c.shift));
-      }
-      int32_t next = base + STEP < stop ? base + STEP : base;  // (the last step loads itself again)
-      int32_t next1 = page_of(b, c, o.s, next + NP * (m16 >> 2)), next2 = page_of(b, c, o.s, next + NP * q4);
       while (true) {
         const bool more = base + STEP < stop;
         // ---- scores
@@ -551,6 +576,15 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
       }
     }
     u += done;
+    if (after->sh.whole) {
+      // (a sequence may have more tiles than it has blocks)
+      o.rt += after->sh.whole;
+      if (o.rt * kFewRows >= o.q.count * shared) break;
+      __syncthreads();
+      o.t = tile_of(*after, o.q, o.rt);
+      u = 0, end = o.t.steps;
+      continue;
+    }
     if (u >= end) {
       if (threadIdx.x == 0) {
         Tail &tail = ((Tail *)after->a.work)[blockIdx.x];
@@ -1172,9 +1206,17 @@ Share share_of(const Cache &c, const Batch &b, int32_t heads, int32_t a_cu, int3
   sh.countable = tiles * c.heads * steps < INT32_MAX && rows * sh.group < (int64_t)1 << 32;
   return sh;
 }
+// Where a sequence has room for four steps at most, a block takes a tile whole: two launches, the shares and their join cost more
+// than three more steps (a head of 128 int8: 1.2 us a step alone; measured over 16 to 4096 positions).
+constexpr int kWholeSteps = 4;
 Share few_share(const Cache &c, const Batch &b, int32_t heads) {
   const int32_t d = padded(c.dim);
-  return share_of(c, b, heads, few_blocks_a_cu(d, c.f16), kFewRows, few_np(d, c.f16) == 16 ? 8 : 7, false);
+  Share sh = share_of(c, b, heads, few_blocks_a_cu(d, c.f16), kFewRows, few_np(d, c.f16) == 16 ? 8 : 7, false);
+  if (((int64_t)b.width << c.shift) <= (int64_t)kWholeSteps << sh.log && b.sequences < 1 << 20) {
+    sh.whole = (b.longest * sh.group + kFewRows - 1) / kFewRows;
+    sh.shared = false;
+  }
+  return sh;
 }
 Share rows_share(const Cache &c, const Batch &b, int32_t heads) {
   return share_of(c, b, heads, rows_blocks_a_cu(padded(c.dim)), kRows, 6, true);
@@ -1188,7 +1230,7 @@ template <int D>
 hipError_t launch(const Attention &a, const Cache &c, const Batch &b, hipStream_t s) {
   const bool few = few_rows(c, b, a.heads);
   const Call call{a, c, b, few ? few_share(c, b, a.heads) : rows_share(c, b, a.heads)};
-  const dim3 blocks(call.sh.blocks);
+  const dim3 blocks = call.sh.whole ? dim3(b.sequences, call.sh.whole, c.heads) : dim3(call.sh.blocks);
   const int32_t *edge = nullptr;
   if (few) {
     hipLaunchKernelGGL((c.f16 ? few_kernel<D, 1> : few_kernel<D, 0>), blocks, dim3(256), 0, s, call);

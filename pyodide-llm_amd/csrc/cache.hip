@@ -19,12 +19,6 @@ namespace {
 constexpr int kChunk = 64;  // positions of a block
 constexpr float kSmallest = 7.888609052210118e-31f;  // 2^-100: a smaller scale is stored as 0 and its vector as zeros
 
-HQ_DEV int32_t chunks_of(const Batch &b, int32_t s) {
-  const Sequence q = sequence_of(b, s);
-  if (!q.count) return 0;
-  return ((q.length - 1) >> 6) - ((q.length - q.count) >> 6) + 1;
-}
-
 // the largest bits over a row of 16 lanes
 HQ_DEV uint32_t max16(uint32_t m) {
   m = max8(m);
@@ -54,56 +48,81 @@ HQ_DEV void scale_of(uint32_t m, float &scale, float &inv) {
   inv = scale > 0.0f ? fdiv(1.0f, scale) : 0.0f;
 }
 
-template <int F16>
+// the positions of the block's chunk: [from, to), from base on, the first new one `first`; none: to <= from
+struct Chunk {
+  Place place;
+  int32_t first, base, from, to;
+};
+HQ_DEV Chunk chunk_of(const Batch &b, int32_t at) {
+  Chunk o;
+  o.place = place_of(b, at);
+  o.first = o.place.q.length - o.place.q.count;
+  o.base = ((o.first >> 6) + o.place.rest) * kChunk;
+  o.from = max(o.first, o.base), o.to = o.place.s < 0 ? o.from : min(o.place.q.length, o.base + kChunk);
+  return o;
+}
+
+// DIM: the head's values in 64s.  All of the block's loads are on their way before the first is used.
+template <int F16, int DIM>
 __global__ __launch_bounds__(256) void write_kernel(Cache c, Batch b, const char *k, const char *v, int64_t k_stride,
                                                     int64_t v_stride) {
   constexpr int ES = F16 ? 2 : 1, PITCH = kChunk * ES + 4;  // 17 (33) dwords: 16 lanes' dimensions fall into 16 banks
-  __shared__ char turned[256 * PITCH];
-  const Place place = place_of(b.sequences, blockIdx.x, [&](int32_t s) { return chunks_of(b, s); });
-  if (place.s < 0) return;
-  const int32_t h = blockIdx.y;
+  constexpr int PARTS = kChunk * ES / 16, EACH = 16 / ES;   // 16 bytes of a dimension's positions
+  __shared__ char turned[64 * DIM * PITCH];
+  const Chunk o = chunk_of(b, blockIdx.x);
+  if (o.to <= o.from || o.to <= 0) return;  // (no such chunk, or before position 0)
+  const int32_t h = blockIdx.y, from = max(o.from, 0), to = o.to;
   const bool values = blockIdx.z;
-  const Sequence q = wave_sequence_of(b, place.s);
-  const int32_t first = q.length - q.count, base = ((first >> 6) + place.rest) * kChunk;
-  const int32_t from = max(max(first, base), 0), to = min(q.length, base + kChunk);  // the positions to write
   const int row = threadIdx.x >> 4, l = threadIdx.x & 15;
-  for (int p0 = base + ((from - base) & ~15); p0 < to; p0 += 16) {
-    const int32_t at = p0 + row;
+  float4 f[4][DIM];
+  int32_t page[4];
+#pragma unroll
+  for (int r = 0; r < 4; r++) {
+    const int32_t at = o.base + 16 * r + row;
     const bool live = at >= from && at < to;
-    const int32_t page = live ? page_of(b, c, place.s, at) : -1;
-    // (a lane without a token reads the sequence's first)
-    const int64_t t = q.begin + (live ? at - first : 0);
+    page[r] = live ? page_of(b, c, o.place.s, at) : -1;
+    const int64_t t = o.place.q.begin + (at - o.first);
     const float *x = (const float *)((values ? v + t * v_stride : k + t * k_stride) + 4 * (int64_t)h * c.dim);
-    float4 f[4];
+#pragma unroll
+    for (int i = 0; i < DIM; i++) {
+      const int at4 = 64 * i + 4 * l;
+      f[r][i] = live && at4 < c.dim ? *(const float4 *)(x + at4) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  }
+  // (the pages of the values' 16 bytes: the thread's part is the same for all its dimensions)
+  const int part = threadIdx.x % PARTS, p0 = o.base + part * EACH;
+  const int32_t part_page = values && p0 + EACH > from && p0 < to ? page_of(b, c, o.place.s, p0) : -1;
+#pragma unroll
+  for (int r = 0; r < 4; r++) {
+    const int32_t at = o.base + 16 * r + row;
+    if (!__any(page[r] >= 0)) continue;
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int at4 = 64 * i + 4 * l;
-      f[i] = at4 < c.dim ? *(const float4 *)(x + at4) : make_float4(0.f, 0.f, 0.f, 0.f);
-      m = max(max(m, __float_as_uint(f[i].x) & 0x7fffffffu), __float_as_uint(f[i].y) & 0x7fffffffu);
-      m = max(max(m, __float_as_uint(f[i].z) & 0x7fffffffu), __float_as_uint(f[i].w) & 0x7fffffffu);
+    for (int i = 0; i < DIM; i++) {
+      m = max(max(m, __float_as_uint(f[r][i].x) & 0x7fffffffu), __float_as_uint(f[r][i].y) & 0x7fffffffu);
+      m = max(max(m, __float_as_uint(f[r][i].z) & 0x7fffffffu), __float_as_uint(f[r][i].w) & 0x7fffffffu);
     }
     float scale, inv;
     scale_of<F16>(max16(m), scale, inv);
     const bool zero = inv == 0.0f;  // (an infinity times 0 is no element)
-    const int64_t vec = page >= 0 ? vectors_of(c, page, h) + (at & ((1 << c.shift) - 1)) : 0;
-    if (page >= 0 && l == 0) (values ? c.vs : c.ks)[vec] = scale;
+    const int64_t vec = page[r] >= 0 ? vectors_of(c, page[r], h) + (at & ((1 << c.shift) - 1)) : 0;
+    if (page[r] >= 0 && l == 0) (values ? c.vs : c.ks)[vec] = scale;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < DIM; i++) {
       const int at4 = 64 * i + 4 * l;
       if (at4 >= c.dim) continue;
-      const float e[4] = {f[i].x, f[i].y, f[i].z, f[i].w};
+      const float e[4] = {f[r][i].x, f[r][i].y, f[r][i].z, f[r][i].w};
       uint32_t u[4];
 #pragma unroll
       for (int j = 0; j < 4; j++) u[j] = zero ? 0u : element<F16>(e[j], inv);
       if (values) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          char *to_lds = turned + (at4 + j) * PITCH + (at - base) * ES;
+          char *to_lds = turned + (at4 + j) * PITCH + (16 * r + row) * ES;
           if (F16) *(uint16_t *)to_lds = (uint16_t)u[j];
           else *(uint8_t *)to_lds = (uint8_t)u[j];
         }
-      } else if (page >= 0) {
+      } else if (page[r] >= 0) {
         char *to_mem = c.k + (vec * c.dim + at4) * ES;
         if (F16) *(uint2 *)to_mem = make_uint2(u[0] | (u[1] << 16), u[2] | (u[3] << 16));
         else *(uint32_t *)to_mem = u[0] | (u[1] << 8) | (u[2] << 16) | (u[3] << 24);
@@ -112,21 +131,16 @@ __global__ __launch_bounds__(256) void write_kernel(Cache c, Batch b, const char
   }
   if (!values) return;
   __syncthreads();
-  // 16 bytes of a dimension's positions a thread (16 or 8 of them: all in one page)
-  constexpr int PARTS = kChunk * ES / 16, EACH = 16 / ES;
-  for (int i = threadIdx.x; i < c.dim * PARTS; i += 256) {
-    const int d = i / PARTS, part = i % PARTS, p0 = base + part * EACH;
-    if (p0 + EACH <= from || p0 >= to) continue;
-    const int32_t page = page_of(b, c, place.s, p0);
-    if (page < 0) continue;
-    char *to_mem = c.v + (((vectors_of(c, page, h) * c.dim) + ((int64_t)d << c.shift)) + (p0 & ((1 << c.shift) - 1))) * ES;
+  if (part_page < 0) return;
+  char *to_part = c.v + (vectors_of(c, part_page, h) * c.dim + (p0 & ((1 << c.shift) - 1))) * ES;
+  for (int d = threadIdx.x / PARTS; d < c.dim; d += 256 / PARTS) {
+    char *to_mem = to_part + ((int64_t)d << c.shift) * ES;
     const char *lds = turned + d * PITCH + part * 16;
     if (p0 >= from && p0 + EACH <= to) {
       const uint32_t *w = (const uint32_t *)lds;
       *(uint4 *)to_mem = make_uint4(w[0], w[1], w[2], w[3]);
     } else {
-      for (int j = 0; j < EACH; j++) {
-        if (p0 + j < from || p0 + j >= to) continue;
+      for (int j = max(from - p0, 0); j < min(to - p0, EACH); j++) {
         if (F16) *(uint16_t *)(to_mem + 2 * j) = *(const uint16_t *)(lds + 2 * j);
         else *(uint8_t *)(to_mem + j) = *(const uint8_t *)(lds + j);
       }
@@ -140,71 +154,89 @@ HQ_DEV float value_of(uint32_t u, float scale) {
   return fmul((float)(int32_t)(int8_t)(uint8_t)u, scale);
 }
 
-template <int F16>
+template <int F16, int DIM>
 __global__ __launch_bounds__(256) void read_kernel(Cache c, Batch b, char *k, char *v, int64_t k_stride, int64_t v_stride) {
-  constexpr int ES = F16 ? 2 : 1, PITCH = kChunk * ES + 4;
-  __shared__ char turned[256 * PITCH];
-  const Place place = place_of(b.sequences, blockIdx.x, [&](int32_t s) { return chunks_of(b, s); });
-  if (place.s < 0) return;
+  constexpr int ES = F16 ? 2 : 1, PITCH = kChunk * ES + 4, PARTS = kChunk * ES / 16, EACH = 16 / ES;
+  constexpr int ROWS = 64 * DIM * PARTS / 256;  // dimensions whose 16 bytes a thread turns
+  __shared__ char turned[64 * DIM * PITCH];
+  const Chunk o = chunk_of(b, blockIdx.x);
+  if (o.to <= o.from) return;
   const int32_t h = blockIdx.y;
   const bool values = blockIdx.z;
-  const Sequence q = wave_sequence_of(b, place.s);
-  const int32_t first = q.length - q.count, base = ((first >> 6) + place.rest) * kChunk;
-  const int32_t from = max(first, base), to = min(q.length, base + kChunk);
-  constexpr int PARTS = kChunk * ES / 16, EACH = 16 / ES;
-  if (values) {
-    for (int i = threadIdx.x; i < c.dim * PARTS; i += 256) {
-      const int d = i / PARTS, part = i % PARTS, p0 = base + part * EACH;
-      if (p0 + EACH <= from || p0 >= to) continue;
-      const int32_t page = page_of(b, c, place.s, p0);
-      if (page < 0) continue;
-      const uint4 w = *(const uint4 *)(c.v + (((vectors_of(c, page, h) * c.dim) + ((int64_t)d << c.shift)) +
-                                              (p0 & ((1 << c.shift) - 1))) * ES);
-      uint32_t *lds = (uint32_t *)(turned + d * PITCH + part * 16);
-      lds[0] = w.x, lds[1] = w.y, lds[2] = w.z, lds[3] = w.w;
-    }
-    __syncthreads();
-  }
   const int row = threadIdx.x >> 4, l = threadIdx.x & 15;
-  for (int p0 = base + ((from - base) & ~15); p0 < to; p0 += 16) {
-    const int32_t at = p0 + row;
-    if (at < from || at >= to) continue;
-    const int32_t page = page_of(b, c, place.s, at);
-    const int64_t t = q.begin + (at - first);
-    float *x = (float *)((values ? v + t * v_stride : k + t * k_stride) + 4 * (int64_t)h * c.dim);
-    const int64_t vec = page >= 0 ? vectors_of(c, page, h) + (at & ((1 << c.shift) - 1)) : 0;
-    const float scale = page >= 0 ? (values ? c.vs : c.ks)[vec] : 0.0f;
+  int32_t page[4];
+  float scale[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+  for (int r = 0; r < 4; r++) {
+    const int32_t at = o.base + 16 * r + row;
+    page[r] = at >= o.from && at < o.to ? page_of(b, c, o.place.s, at) : -1;
+  }
+  uint2 w[4][DIM];  // the lane's 4 elements
+  if (values) {
+    const int part = threadIdx.x % PARTS, p0 = o.base + part * EACH, d0 = threadIdx.x / PARTS;
+    const int32_t part_page = p0 + EACH > o.from && p0 < o.to ? page_of(b, c, o.place.s, p0) : -1;
+    const char *from_part = c.v + (vectors_of(c, max(part_page, 0), h) * c.dim + (p0 & ((1 << c.shift) - 1))) * ES;
+    uint4 q[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) {
+      const int d = d0 + i * (256 / PARTS);
+      q[i] = part_page >= 0 && d < c.dim ? *(const uint4 *)(from_part + ((int64_t)d << c.shift) * ES) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) {
+      uint32_t *lds = (uint32_t *)(turned + (d0 + i * (256 / PARTS)) * PITCH + part * 16);
+      lds[0] = q[i].x, lds[1] = q[i].y, lds[2] = q[i].z, lds[3] = q[i].w;
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < 4; r++) {
+    const int64_t vec = vectors_of(c, max(page[r], 0), h) + ((o.base + 16 * r + row) & ((1 << c.shift) - 1));
+    scale[r] = page[r] >= 0 ? (values ? c.vs : c.ks)[vec] : 0.0f;
+    if (values) continue;
+#pragma unroll
+    for (int i = 0; i < DIM; i++) {
+      const int at4 = 64 * i + 4 * l;
+      w[r][i] = make_uint2(0, 0);
+      if (page[r] >= 0 && at4 < c.dim) {
+        const char *mem = c.k + (vec * c.dim + at4) * ES;
+        if (F16) w[r][i] = *(const uint2 *)mem;
+        else w[r][i].x = *(const uint32_t *)mem;
+      }
+    }
+  }
+  if (values) __syncthreads();
+#pragma unroll
+  for (int r = 0; r < 4; r++) {
+    const int32_t at = o.base + 16 * r + row;
+    if (at < o.from || at >= o.to) continue;
+    const int64_t t = o.place.q.begin + (at - o.first);
+    float *x = (float *)((values ? v + t * v_stride : k + t * k_stride) + 4 * (int64_t)h * c.dim);
+#pragma unroll
+    for (int i = 0; i < DIM; i++) {
       const int at4 = 64 * i + 4 * l;
       if (at4 >= c.dim) continue;
-      uint32_t u[4] = {0, 0, 0, 0};
-      if (page >= 0 && values) {
+      uint32_t u[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const char *lds = turned + (at4 + j) * PITCH + (at - base) * ES;
-          u[j] = F16 ? *(const uint16_t *)lds : *(const uint8_t *)lds;
-        }
-      } else if (page >= 0) {
-        const char *mem = c.k + (vec * c.dim + at4) * ES;
-        if (F16) {
-          const uint2 w = *(const uint2 *)mem;
-          u[0] = w.x & 0xffffu, u[1] = w.x >> 16, u[2] = w.y & 0xffffu, u[3] = w.y >> 16;
-        } else {
-          const uint32_t w = *(const uint32_t *)mem;
-          u[0] = w & 0xffu, u[1] = (w >> 8) & 0xffu, u[2] = (w >> 16) & 0xffu, u[3] = w >> 24;
-        }
+      for (int j = 0; j < 4; j++) {
+        const char *lds = turned + (at4 + j) * PITCH + (16 * r + row) * ES;
+        if (values) u[j] = page[r] < 0 ? 0 : F16 ? *(const uint16_t *)lds : *(const uint8_t *)lds;
+        else u[j] = F16 ? (j < 2 ? w[r][i].x : w[r][i].y) >> (16 * (j & 1)) : w[r][i].x >> (8 * j);
       }
-      *(float4 *)(x + at4) = make_float4(value_of<F16>(u[0], scale), value_of<F16>(u[1], scale),
-                                         value_of<F16>(u[2], scale), value_of<F16>(u[3], scale));
+      *(float4 *)(x + at4) = make_float4(value_of<F16>(u[0], scale[r]), value_of<F16>(u[1], scale[r]),
+                                         value_of<F16>(u[2], scale[r]), value_of<F16>(u[3], scale[r]));
     }
   }
 }
 
-// every chunk holds a new token, and a sequence's tokens touch two chunks more than they fill at most
+// as many items as place_of gives the sequences
 dim3 grid_of(const Cache &c, const Batch &b) {
-  const int64_t chunks = (int64_t)b.tokens / kChunk + 2 * (int64_t)b.sequences;
-  return dim3((uint32_t)(chunks < b.tokens ? chunks : b.tokens), (uint32_t)c.heads, 2);
+  return dim3((uint32_t)(b.tokens / kChunk + 2 * b.sequences), (uint32_t)c.heads, 2);
+}
+
+template <typename Kernel, typename... Args>
+hipError_t run(const Cache &c, const Batch &b, hipStream_t s, Kernel kernel, Args... args) {
+  hipLaunchKernelGGL(kernel, grid_of(c, b), dim3(256), 0, s, c, b, args...);
+  return hipGetLastError();
 }
 
 }  // namespace
@@ -212,17 +244,17 @@ dim3 grid_of(const Cache &c, const Batch &b) {
 hipError_t launch_cache_write(const Cache &c, const Batch &b, const char *k, const char *v, int64_t k_stride,
                               int64_t v_stride, hipStream_t s) {
   if (b.tokens <= 0 || b.sequences <= 0) return hipSuccess;
-  const auto kernel = c.f16 ? write_kernel<1> : write_kernel<0>;
-  hipLaunchKernelGGL(kernel, grid_of(c, b), dim3(256), 0, s, c, b, k, v, k_stride, v_stride);
-  return hipGetLastError();
+  if (c.dim <= 64) return run(c, b, s, c.f16 ? write_kernel<1, 1> : write_kernel<0, 1>, k, v, k_stride, v_stride);
+  if (c.dim <= 128) return run(c, b, s, c.f16 ? write_kernel<1, 2> : write_kernel<0, 2>, k, v, k_stride, v_stride);
+  return run(c, b, s, c.f16 ? write_kernel<1, 4> : write_kernel<0, 4>, k, v, k_stride, v_stride);
 }
 
 hipError_t launch_cache_read(const Cache &c, const Batch &b, char *k, char *v, int64_t k_stride, int64_t v_stride,
                              hipStream_t s) {
   if (b.tokens <= 0 || b.sequences <= 0) return hipSuccess;
-  const auto kernel = c.f16 ? read_kernel<1> : read_kernel<0>;
-  hipLaunchKernelGGL(kernel, grid_of(c, b), dim3(256), 0, s, c, b, k, v, k_stride, v_stride);
-  return hipGetLastError();
+  if (c.dim <= 64) return run(c, b, s, c.f16 ? read_kernel<1, 1> : read_kernel<0, 1>, k, v, k_stride, v_stride);
+  if (c.dim <= 128) return run(c, b, s, c.f16 ? read_kernel<1, 2> : read_kernel<0, 2>, k, v, k_stride, v_stride);
+  return run(c, b, s, c.f16 ? read_kernel<1, 4> : read_kernel<0, 4>, k, v, k_stride, v_stride);
 }
 
 }  // namespace hq

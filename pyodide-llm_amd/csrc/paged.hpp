@@ -43,30 +43,26 @@ HQ_DEV int64_t vectors_of(const Cache &c, int32_t page, int32_t head) {
   return ((int64_t)page * c.heads + head) << c.shift;
 }
 
-// Which sequence the `at`-th of all their items is in, count_of(s) items a sequence, and its place there: 64 sequences at a
-// time, a lane each.  Every lane of the wave calls it; s is -1 where there are fewer items.
+// The sequence whose items a launch's `at`-th are, and which of them: sequence s has its tokens / 64 + 2 of the tokens / 64 +
+// 2 sequences items, from starts[s] / 64 + 2 s on (no sums over the sequences are needed), of which it may use fewer.  A lane a
+// sequence, 64 at a time; every lane of the wave calls it; s is -1 where no sequence has the item.
 struct Place {
   int32_t s, rest;
+  Sequence q;
 };
-template <typename Count>
-HQ_DEV Place place_of(int32_t sequences, int32_t at, Count count_of) {
+HQ_DEV Place place_of(const Batch &b, int32_t at) {
   const int lane = threadIdx.x & 63;
-  for (int32_t s0 = 0; s0 < sequences; s0 += 64) {
-    const int32_t mine = s0 + lane < sequences ? count_of(s0 + lane) : 0;
-    int32_t upto = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int32_t v = __shfl_up(upto, o, 64);
-      if (lane >= o) upto += v;
-    }
-    const uint64_t past = __ballot(upto > at);
-    if (past) {
-      const int l = __ffsll((unsigned long long)past) - 1;
-      return {s0 + l, __builtin_amdgcn_readlane(mine, l) - __builtin_amdgcn_readlane(upto, l) + at};
-    }
-    at -= __builtin_amdgcn_readlane(upto, 63);
+  for (int32_t s0 = 0; s0 < b.sequences; s0 += 64) {
+    const int32_t s = min(s0 + lane, b.sequences - 1);
+    const Sequence q = sequence_of(b, s);
+    const int32_t first = (q.begin >> 6) + 2 * s, end = ((q.begin + q.count) >> 6) + 2 * s + 2;
+    const uint64_t in = __ballot(s0 + lane < b.sequences && at >= first && at < end);
+    if (!in) continue;
+    const int l = __ffsll((unsigned long long)in) - 1;
+    return {s0 + l, at - __builtin_amdgcn_readlane(first, l),
+            {__builtin_amdgcn_readlane(q.begin, l), __builtin_amdgcn_readlane(q.count, l), __builtin_amdgcn_readlane(q.length, l)}};
   }
-  return {-1, 0};
+  return {-1, 0, {0, 0, 0}};
 }
 
 }  // namespace hq
