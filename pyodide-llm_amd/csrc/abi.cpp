@@ -440,8 +440,9 @@ int32_t paged_of(const char *who, const hq_cache *cache, const hq_batch *batch, 
   const int32_t longest = batch->longest && batch->longest < batch->tokens ? batch->longest : batch->tokens;
   b = hq::Batch{(const int32_t *)batch->starts, (const int32_t *)batch->lengths, (const int32_t *)batch->table,
                 batch->sequences, batch->tokens, longest, c.pages ? batch->width : 0};
+  if (!b.width) b.table = b.starts;
   if (!memory || b.tokens == 0 || b.sequences == 0) return HQ_OK;
-  if (!b.starts || !b.lengths || (!b.table && b.width)) return fail(HQ_ERR_NULL, "%s: starts, lengths or table NULL", who);
+  if (!b.starts || !b.lengths || !b.table) return fail(HQ_ERR_NULL, "%s: starts, lengths or table NULL", who);
   if (!aligned(b.starts, 4) || !aligned(b.lengths, 4) || !aligned(b.table, 4))
     return fail(HQ_ERR_ALIGNMENT, "%s: starts, lengths or table not 4-byte aligned", who);
   if (c.pages && (!c.k || !c.v || !c.ks || !c.vs)) return fail(HQ_ERR_NULL, "%s: the cache's k, v, ks or vs NULL", who);

@@ -352,9 +352,13 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
     const int32_t stop = min((o.t.first + o.step + steps) * STEP, o.t.to);
     while (base + WK <= o.t.from) base += STEP;
     const int32_t next0 = base + STEP < stop ? base + STEP : base;  // (the last step loads itself again)
-    const int32_t page1 = page_of(b, c, o.s, base + NP * (m16 >> 2));
-    int32_t page2 = page_of(b, c, o.s, base + NP * q4);
-    int32_t next = next0, next1 = page_of(b, c, o.s, next + NP * (m16 >> 2)), next2 = page_of(b, c, o.s, next + NP * q4);
+    // the table's entries of the step's positions, for the keys' lanes (1) and the others' (2)
+    const int32_t entry1 = entry_of(b, c, o.s, base + NP * (m16 >> 2));
+    const int32_t entry2 = entry_of(b, c, o.s, base + NP * q4);
+    // (Loads come back in order: an entry asked for after a step's values would be waited for with all of them, so that those of the
+    // step after the next are asked for before this one's scores.)
+    int32_t next = next0, next1 = entry_of(b, c, o.s, next + NP * (m16 >> 2)), next2 = entry_of(b, c, o.s, next + NP * q4);
+    int32_t page2 = page_in(b, c, entry2, base + NP * q4);
     // Registers are loaded for the next step as soon as this one has used them: keys after the scores, scales after the weights,
     // values after their products, so that a step's bytes are always on their way.
     Elements<F16, 16> kk[NP / 4][DB];
@@ -385,7 +389,7 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
     };
     const auto value_row = [&](int d, int32_t dim, int32_t shift) { return (min(d * 16, dim - 16) << shift) * ES; };  // (past dim: the last again)
     if (base < stop) {
-      load_keys(base, page1);
+      load_keys(base, page_in(b, c, entry1, base + NP * (m16 >> 2)));
       load_scales(base, page2);
       const char *p = values_at(base, page2);
 #pragma unroll
@@ -432,6 +436,8 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
     if (base < stop) {
       while (true) {
         const bool more = base + STEP < stop;
+        const int32_t after_next = next + STEP < stop ? next + STEP : next;
+        const int32_t after1 = entry_of(b, c, o.s, after_next + NP * (m16 >> 2)), after2 = entry_of(b, c, o.s, after_next + NP * q4);
         // ---- scores
         v4f s[NP / 4] = {};
 #pragma unroll
@@ -444,7 +450,8 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
               s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, ql[d][i], s[t], 0, 0, 0);
               s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, qh[d][i], s[t], 0, 0, 0);
             }
-        load_keys(next, next1);
+        load_keys(next, page_in(b, c, next1, next + NP * (m16 >> 2)));
+        const int32_t next_page2 = page_in(b, c, next2, next + NP * q4);
         float p[NP];
 #pragma unroll
         for (int e = 0; e < NP; e++) p[e] = s[e >> 2][e & 3] * ks[e];
@@ -506,12 +513,12 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
           for (int e = 0; e < NP; e++)
             p[e] = kept(p[e], seen, e, 0u);  // (a NaN scale that others see)
         }
-        load_scales(next, next2);
+        load_scales(next, next_page2);
         // ---- out += weights times values
         v8h ph[NP / 8], pl[NP / 8];
 #pragma unroll
         for (int i = 0; i < NP / 8; i++) halves_of(p + 8 * i, ph[i], pl[i]);
-        const char *v_next = values_at(next, next2);
+        const char *v_next = values_at(next, next_page2);
         const int32_t dim = opaque(c.dim), shift = opaque(c.shift);
 #pragma unroll
         for (int d = 0; d < DT; d++) {
@@ -526,9 +533,8 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
           vv[d].load(v_next + value_row(d, dim, shift));
         }
         if (!more) break;
-        base = next, page2 = next2;
-        next = base + STEP < stop ? base + STEP : base;
-        next1 = page_of(b, c, o.s, next + NP * (m16 >> 2)), next2 = page_of(b, c, o.s, next + NP * q4);
+        base = next, page2 = next_page2;
+        next = after_next, next1 = after1, next2 = after2;
       }
     }
     l = sum_row(l);
@@ -912,18 +918,19 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
     constexpr int V0 = BOTH ? PIECES : 0;
     float sreg;
     const float *scale_at = wave ? c.vs : c.ks;  // (waves 0 and 1)
-    int32_t kpage, vpage, spage;  // of the step to load next
-    const auto pages_at = [&](int32_t base) {
+    int32_t kentry, ventry, sentry;  // the table's entries for the step to load next
+    const auto entries_at = [&](int32_t base) {
       const uint32_t tid = opaque_lane(threadIdx.x);
       const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-      kpage = page_of(b, c, o.s, base + 16 * wave);
-      vpage = page_of(b, c, o.s, base + EACH * (int32_t)(tid % PARTS));
-      spage = page_of(b, c, o.s, base + (int32_t)(tid & 63));
+      kentry = entry_of(b, c, o.s, base + 16 * wave);
+      ventry = entry_of(b, c, o.s, base + EACH * (int32_t)(tid % PARTS));
+      sentry = entry_of(b, c, o.s, base + (int32_t)(tid & 63));
     };
     const auto load_keys = [&](int32_t base) {
       const uint32_t tid = opaque_lane(threadIdx.x), ln = tid & 63;
       const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
       const uint32_t row_pieces = (uint32_t)(opaque(c.dim) * ES) / 16;
+      const int32_t kpage = page_in(b, c, kentry, base + 16 * wave);
       const int64_t kvec = vectors_of(c, max(kpage, 0), o.h) + ((base + 16 * wave) & mask);
       const char *kp = c.k + kvec * c.dim * ES;
 #pragma unroll
@@ -933,10 +940,12 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
       }
     };
     uint32_t on_page = 0, keep_bits = 0;  // of the loaded step
+    uint32_t scale_bits = 0;  // (all where the lane's position has a scale)
     const auto load_values = [&](int32_t base) {
       const uint32_t tid = opaque_lane(threadIdx.x), ln = tid & 63;
       const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
       const int32_t part_at = EACH * (int32_t)(tid % PARTS), slot = (base + part_at) & mask;
+      const int32_t vpage = page_in(b, c, ventry, base + part_at), spage = page_in(b, c, sentry, base + (int32_t)ln);
       const char *vp = c.v + (vectors_of(c, max(vpage, 0), o.h) * c.dim + slot) * ES;
 #pragma unroll
       for (int i = 0; i < PIECES; i++) {
@@ -944,12 +953,12 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
         reg[V0 + i] = *(const uint4 *)(vp + (min(d, c.dim - 1) << c.shift) * ES);  // (past dim: the last again)
       }
       const int32_t at = base + (int32_t)ln;
-      const bool there = spage >= 0 && at >= tile.from && at < tile.to;
-      sreg = 0.0f;
-      if (wave < 2 && there) sreg = scale_at[vectors_of(c, spage, o.h) + (at & mask)];
+      const bool there = spage >= 0 && at < tile.to;
+      sreg = scale_at[vectors_of(c, max(spage, 0), o.h) + (at & mask)];
+      scale_bits = opaque_lane(there ? ~0u : 0u);
       const uint64_t mapped = __ballot(spage >= 0);
       on_page = (uint32_t)((mapped & 1) | (mapped >> 15 & 2) | (mapped >> 30 & 4) | (mapped >> 45 & 8));
-      if (F16) keep_bits = vpage >= 0 ? bits_between(tile.from - (base + part_at), tile.to - (base + part_at)) & 0xffu : 0u;
+      if (F16) keep_bits = vpage >= 0 ? bits_between(0, tile.to - (base + part_at)) & 0xffu : 0u;
     };
     const auto store_keys = [&](int buf) {
       const uint32_t tid = opaque_lane(threadIdx.x), ln = tid & 63;
@@ -991,6 +1000,7 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
           *(v8h *)(to_row + 16 * ((2 * part + 1) ^ (d & 7))) = widen8(reg[V0 + i].z, reg[V0 + i].w);
         }
       }
+      sreg = __uint_as_float(__float_as_uint(sreg) & scale_bits);
       if (wave == 0) scales[buf][0][ln] = sreg;
       if (wave == 1) {
         const int e1 = (int)(wave_max(sreg == sreg ? __float_as_uint(sreg) : 0u) >> 23) - 127;
@@ -1011,12 +1021,12 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
     int32_t base = (tile.first + o.step) * kPositions;
     const int32_t stop = base < tile.to ? base + steps * kPositions : base;  // (rows that see nothing: a step without positions)
     if (base < stop) {
-      pages_at(base);
+      entries_at(base);
       load_keys(base);
       store_keys(0);
       load_values(base);
       store_values(0);
-      pages_at(base + kPositions);
+      entries_at(base + kPositions);
     }
     __syncthreads();
     for (int buf = 0; base < stop; base += kPositions, buf ^= 1) {
@@ -1025,7 +1035,7 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
         load_keys(base + kPositions);
         if (BOTH) {
           load_values(base + kPositions);
-          pages_at(base + 2 * kPositions);
+          entries_at(base + 2 * kPositions);
         }
       }
       // 32 positions at a time, as the registers allow
@@ -1117,7 +1127,7 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
         if (!BOTH && more && t == 0) {
           store_keys(buf ^ 1);
           load_values(base + kPositions);
-          pages_at(base + 2 * kPositions);
+          entries_at(base + 2 * kPositions);
         }
       }
       if (more) {

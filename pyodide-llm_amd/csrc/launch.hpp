@@ -152,7 +152,7 @@ struct Cache {
   int32_t f16, pages, shift, heads, dim;
 };
 struct Batch {
-  const int32_t *starts, *lengths, *table;
+  const int32_t *starts, *lengths, *table;  // (table: some memory even where width is 0)
   int32_t sequences, tokens, longest, width;
 };
 hipError_t launch_cache_write(const Cache &c, const Batch &b, const char *k, const char *v, int64_t k_stride,

@@ -29,13 +29,17 @@ HQ_DEV Sequence wave_sequence_of(const Batch &b, int32_t s) {
   return q;
 }
 
-// the page that holds position `at` of sequence s, or -1: none (a position before the first or past the table, an entry that
-// is no page)
+// The table's entry for position `at` of sequence s (the nearest one where it has none), and the page that it means: -1 where
+// there is no such position (before the first or past the table) or the entry is no page.  The entry is loaded without a branch:
+// a load in one is waited for at its end, with every load before it.
+HQ_DEV int32_t entry_of(const Batch &b, const Cache &c, int32_t s, int32_t at) {
+  return b.table[(int64_t)s * b.width + max(min(at >> c.shift, b.width - 1), 0)];
+}
+HQ_DEV int32_t page_in(const Batch &b, const Cache &c, int32_t entry, int32_t at) {
+  return at >= 0 && (at >> c.shift) < b.width && (uint32_t)entry < (uint32_t)c.pages ? entry : -1;
+}
 HQ_DEV int32_t page_of(const Batch &b, const Cache &c, int32_t s, int32_t at) {
-  const int32_t i = at >> c.shift;
-  if (at < 0 || i >= b.width) return -1;
-  const int32_t p = b.table[(int64_t)s * b.width + i];
-  return (uint32_t)p < (uint32_t)c.pages ? p : -1;
+  return page_in(b, c, entry_of(b, c, s, at), at);
 }
 
 // the first of a (page, head)'s vectors
