@@ -432,7 +432,7 @@ int32_t paged_of(const char *who, const hq_cache *cache, const hq_batch *batch, 
   if (batch->sequences < 0 || batch->tokens < 0 || batch->longest < 0 || batch->width < 0)
     return fail(HQ_ERR_ARGUMENT, "%s: sequences = %d, tokens = %d, longest = %d, width = %d", who, batch->sequences,
                 batch->tokens, batch->longest, batch->width);
-  if (((int64_t)batch->width << shift) > INT32_MAX)
+  if (((int64_t)batch->width << shift) > 1 << 30)
     return fail(HQ_ERR_ARGUMENT, "%s: a table of %d pages of %d positions", who, batch->width, cache->page);
   if (batch->tokens > (1 << 24)) return fail(HQ_ERR_ARGUMENT, "%s: tokens = %d", who, batch->tokens);
   c = hq::Cache{(char *)cache->k, (char *)cache->v, (float *)cache->ks, (float *)cache->vs, cache->form == HQ_CACHE_F16,

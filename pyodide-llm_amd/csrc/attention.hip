@@ -837,7 +837,9 @@ HQ_DEV uint32_t key_row(uint32_t r) { return (r & ~12u) | ((r & 4u) << 1) | ((r 
 typedef float v16f __attribute__((ext_vector_type(16)));
 
 constexpr int rows_blocks_a_cu(int d) { return d <= 64 ? 3 : d <= 128 ? 2 : 1; }
-template <int D, int F16>
+// WHOLE: a step's 64 positions are on one page (pages of 64 and more), whose addresses the scalar unit then forms: a 2048-token chunk
+// 626 -> 611 us.  (For the other dims it does not fit the scalar registers.)
+template <int D, int F16, bool WHOLE>
 __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
   constexpr int ES = F16 ? 2 : 1, KS = D / 16, DT = D / 32;
   constexpr int PIECES = D * ES / 64;  // 16-byte pieces of keys, and of values, a thread stages
@@ -918,8 +920,13 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
     constexpr int V0 = BOTH ? PIECES : 0;
     float sreg;
     const float *scale_at = wave ? c.vs : c.ks;  // (waves 0 and 1)
-    int32_t kentry, ventry, sentry;  // the table's entries for the step to load next
+    int32_t kentry, ventry, sentry;  // the table's entries for the step to load next (WHOLE: all one)
     const auto entries_at = [&](int32_t base) {
+      if (WHOLE) {
+        const int64_t at = (int64_t)o.s * b.width + max(min(base >> c.shift, b.width - 1), 0);
+        kentry = *(const __attribute__((address_space(4))) int32_t *)(uintptr_t)(b.table + at);
+        return;
+      }
       const uint32_t tid = opaque_lane(threadIdx.x);
       const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
       kentry = entry_of(b, c, o.s, base + 16 * wave);
@@ -933,18 +940,43 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
       const int32_t kpage = page_in(b, c, kentry, base + 16 * wave);
       const int64_t kvec = vectors_of(c, max(kpage, 0), o.h) + ((base + 16 * wave) & mask);
       const char *kp = c.k + kvec * c.dim * ES;
+      if (D <= 128 && c.dim == D) {
+#pragma unroll
+        for (int i = 0; i < PIECES; i++) reg[i] = *(const uint4 *)(kp + (16 * ln + 1024 * i));
+        return;
+      }
 #pragma unroll
       for (int i = 0; i < PIECES; i++) {
         const uint32_t at = ln + 64 * i, col = min(at % ROW, row_pieces - 1);  // (past dim: the last again)
         reg[i] = *(const uint4 *)(kp + (at / ROW * row_pieces + col) * 16);
       }
     };
-    uint32_t on_page = 0, keep_bits = 0;  // of the loaded step
-    uint32_t scale_bits = 0;  // (all where the lane's position has a scale)
+    uint32_t on_page = 0;     // which 16 positions of the loaded step are on a page
+    uint32_t keep_bits = 0;   // which of the thread's (float16) positions may be looked at
+    int32_t left_over = 0;    // (WHOLE: 0 or more where all of the step's may be)
+    uint32_t scale_bits = 0;  // all where the lane's position has a scale
     const auto load_values = [&](int32_t base) {
       const uint32_t tid = opaque_lane(threadIdx.x), ln = tid & 63;
-      const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-      const int32_t part_at = EACH * (int32_t)(tid % PARTS), slot = (base + part_at) & mask;
+      const int32_t part_at = EACH * (int32_t)(tid % PARTS);
+      if (WHOLE) {
+        const int32_t page = page_in(b, c, kentry, base), left = page >= 0 ? tile.to - base : 0;
+        const int64_t vec = vectors_of(c, max(page, 0), o.h);
+        const char *vp = c.v + (vec * c.dim + (base & mask)) * ES;
+        const uint32_t lane_at = (((tid / PARTS) << c.shift) + part_at) * ES;
+#pragma unroll
+        for (int i = 0; i < PIECES; i++) {
+          // (past dim: the last again)
+          const uint32_t at = c.dim == D ? lane_at + (uint32_t)(((i * (256 / PARTS)) << c.shift) * ES)
+                                         : (uint32_t)(((min((int)(tid / PARTS) + i * (256 / PARTS), c.dim - 1) << c.shift) + part_at) * ES);
+          reg[V0 + i] = *(const uint4 *)(vp + at);
+        }
+        sreg = (scale_at + vec + (base & mask))[ln];
+        scale_bits = opaque_lane((int32_t)ln < left ? ~0u : 0u);
+        on_page = page >= 0 ? 15 : 0;
+        if (F16) left_over = left - kPositions, keep_bits = bits_between(0, left - part_at) & 0xffu;
+        return;
+      }
+      const int32_t slot = (base + part_at) & mask;
       const int32_t vpage = page_in(b, c, ventry, base + part_at), spage = page_in(b, c, sentry, base + (int32_t)ln);
       const char *vp = c.v + (vectors_of(c, max(vpage, 0), o.h) * c.dim + slot) * ES;
 #pragma unroll
@@ -986,7 +1018,7 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
         char *to_row = values[buf] + d * (kPositions * 2);
         if (F16) {
           uint4 w = reg[V0 + i];
-          if (keep_bits != 0xffu) {
+          if (WHOLE ? left_over < 0 : keep_bits != 0xffu) {
             uint32_t *e = (uint32_t *)&w;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
@@ -1003,8 +1035,8 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
       sreg = __uint_as_float(__float_as_uint(sreg) & scale_bits);
       if (wave == 0) scales[buf][0][ln] = sreg;
       if (wave == 1) {
-        const int e1 = (int)(wave_max(sreg == sreg ? __float_as_uint(sreg) : 0u) >> 23) - 127;
-        if (e1 > exponent_run) exponent_run = e1;
+        if (__any(sreg >= power_of_2(exponent_run + 1)))  // (a NaN is not)
+          exponent_run = (int)(wave_max(sreg == sreg ? __float_as_uint(sreg) : 0u) >> 23) - 127;
         scales[buf][1][ln] = sreg * power_of_2(-exponent_run);
         if (ln == 0) info[buf][0] = exponent_run, info[buf][1] = on_page;
       }
@@ -1247,7 +1279,10 @@ hipError_t launch(const Attention &a, const Cache &c, const Batch &b, hipStream_
   } else {
     edge = plan_of(a.work, call.sh.blocks, b.sequences).edge;
     hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, s, call);
-    hipLaunchKernelGGL((c.f16 ? rows_kernel<D, 1> : rows_kernel<D, 0>), blocks, dim3(256), 0, s, call);
+    if (D == 128 && c.shift >= 6)
+      hipLaunchKernelGGL((c.f16 ? rows_kernel<D, 1, D == 128> : rows_kernel<D, 0, D == 128>), blocks, dim3(256), 0, s, call);
+    else
+      hipLaunchKernelGGL((c.f16 ? rows_kernel<D, 1, false> : rows_kernel<D, 0, false>), blocks, dim3(256), 0, s, call);
   }
   // (a block of join_kernel takes 1024 / D rows at a time)
   const dim3 join(call.sh.blocks, std::min(call.sh.rows * D / 1024, 8));

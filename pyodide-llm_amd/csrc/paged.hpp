@@ -8,6 +8,9 @@
 
 namespace hq {
 
+// (a table holds 2^30 positions at most and a batch 2^24 tokens: from a longer sequence all of its new tokens are past its table)
+constexpr int32_t kMostPositions = (1 << 30) + (1 << 25);
+
 struct Sequence {
   int32_t begin, count, length;  // its first new token, how many there are, and its positions with them
 };
@@ -16,7 +19,7 @@ HQ_DEV Sequence sequence_of(const Batch &b, int32_t s) {
   Sequence q;
   q.begin = min(max(b.starts[s], 0), b.tokens);
   q.count = min(max(b.starts[s + 1], q.begin), b.tokens) - q.begin;
-  q.length = max(b.lengths[s], 0);
+  q.length = min(max(b.lengths[s], 0), kMostPositions);
   return q;
 }
 
