@@ -1264,9 +1264,14 @@ Share rows_share(const Cache &c, const Batch &b, int32_t heads) {
   return share_of(c, b, heads, rows_blocks_a_cu(padded(c.dim)), kRows, 6, true);
 }
 
-// whether few_kernel takes the call: no sequence has more rows of a head than two of its tiles (8 sequences of 5 tokens, 20 rows,
-// over 4100 positions: 43 us in its tiles, 74 in rows_kernel's)
-bool few_rows(const Cache &c, const Batch &b, int32_t heads) { return (int64_t)b.longest * (heads / c.heads) <= 2 * kFewRows; }
+// Whether few_kernel takes the call: no sequence has more rows of a head than six of its tiles (three where a head has 64 values
+// or fewer).  It reads a step's positions again for every tile, rows_kernel fills tiles of 128 rows with them.  Measured, few / rows
+// (us): heads of 128 int8, 8 sequences over 4100 positions, 20 rows 34 / 59, 48 rows 51 / 73, 64 rows 55 / 80, 96 rows 77 / 91, 192
+// rows 126 / 123; 32 over 1000, 64 rows 49 / 69, 256 rows 183 / 104; 256 int8, 96 rows 75 / 111; 64 float16, 48 rows 46 / 49, 64
+// rows 53 / 51.
+bool few_rows(const Cache &c, const Batch &b, int32_t heads) {
+  return (int64_t)b.longest * (heads / c.heads) <= (padded(c.dim) > 64 ? 6 : 3) * kFewRows;
+}
 
 template <int D>
 hipError_t launch(const Attention &a, const Cache &c, const Batch &b, hipStream_t s) {

@@ -173,6 +173,18 @@ def test_longest_is_a_hint(pkg, arena, form):
         check(p, queries(rng, p, 8))
 
 
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dim, new", [(64, [12, 3]), (64, [13, 3]), (128, [24, 1]), (128, [25, 1]), (256, [4, 24]), (256, [4, 25])])
+@pytest.mark.parametrize("lengths, width", [([140, 90], 0), ([140, 90], 60), ([1500, 700], 0)])
+def test_few_rows_or_many(pkg, arena, form, dim, new, lengths, width):
+    """on either side of what decides how rows are tiled, and whether a block has a tile's positions whole"""
+    rng = np.random.default_rng(dim + sum(new))
+    arena.reset()
+    p = Paged(pkg, arena, rng, form, 2, dim, 64, lengths, new, extra_width=width, longest=max(new))
+    p.fill(rng)
+    check(p, queries(rng, p, 8))
+
+
 @pytest.mark.parametrize("starts", [[0, 5, 3, 9], [-4, 2, 100, 9], [3, 3, 8, 9], [0, 9, 0, 9]])
 @pytest.mark.parametrize("longest", [0, 1])
 def test_contradicting_starts(pkg, arena, starts, longest):
