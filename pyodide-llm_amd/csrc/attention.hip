@@ -617,14 +617,19 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
 }
 
 // The items that blocks share: the block whose share an item starts in (and does not end in) has its rows' parts joined here, a
-// thread 4 values of a row: the largest of the parts' maxima, then their sum.  A block's parts are two of (rows' (m, l) pairs, rows
-// of D): what its first item's end and its last item's start gave.  edge: the shares' edges (NULL: even shares of all steps).
+// thread 4 values of a row over every SLICES-th part, the slices together in the end: the largest of the maxima so far, their sum.
+// A chain of loads, so that four parts are on their way at once, and where an item has few rows, it has many parts, which are
+// sliced: one token over 131072 positions (4 rows an item, 64 parts) 10.0 us in one slice, 8.6 in 4, 8.0 in 8, which cost short
+// items 1 us; 8 sequences of 5 tokens (20 rows) 5.1 us in one slice, 7.1 in 4.  A block's parts are two of (rows' (m, l) pairs,
+// rows of D): what its first item's end and its last item's start gave.  edge: the shares' edges (NULL: even shares of all steps).
 constexpr int kMostBlocks = 4096;  // of a launch that shares its items
-template <int D>
+template <int D, int SLICES>
 __global__ __launch_bounds__(256) void join_kernel(Call k, const int32_t *edge) {
-  constexpr int ROWS = 256 / (D / 4);  // rows at a time
+  constexpr int COLS = D / 4, ROWS = 256 / COLS / SLICES;  // rows at a time
   __shared__ int32_t of[kMostBlocks];  // the blocks that have a part
   __shared__ int32_t found;
+  __shared__ v4f sums[SLICES > 1 ? 256 : 1];
+  __shared__ float2 stats[SLICES > 1 ? 256 : 1];
   const Tail t = ((const Tail *)k.a.work)[blockIdx.x];
   if (t.last < 0 || (int32_t)blockIdx.y * ROWS >= t.rows) return;
   if (threadIdx.x < 64) {
@@ -642,24 +647,52 @@ __global__ __launch_bounds__(256) void join_kernel(Call k, const int32_t *edge) 
     if (lane == 0) found = n;
   }
   __syncthreads();
-  const int n = found, col = threadIdx.x % (D / 4) * 4;
+  const int n = found, col = threadIdx.x % COLS * 4, slice = threadIdx.x / COLS % SLICES;
   const int64_t size = (int64_t)k.sh.rows * (D + 2);
   const float *parts = (const float *)(k.a.work + k.sh.parts);
-  for (int r = blockIdx.y * ROWS + threadIdx.x / (D / 4); r < t.rows; r += ROWS * gridDim.y) {
-    float m = -INFINITY;  // (the row's threads look at a part each)
-    for (int i = threadIdx.x % (D / 4); i < n; i += D / 4) m = fmaxf(m, parts[of[i] * size + 2 * r]);
-#pragma unroll
-    for (int o = D / 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    const float ref = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f;
+  for (int r0 = blockIdx.y * ROWS; r0 < t.rows; r0 += ROWS * gridDim.y) {
+    const int r = r0 + threadIdx.x / (COLS * SLICES), row = min(r, t.rows - 1);
+    float m = -INFINITY, l = 0.0f;
     v4f acc = {};
-#pragma unroll 16
-    for (int i = 0; i < n; i++) {
-      const float *part = parts + of[i] * size;
-      const float f = exp2_of(part[2 * r] - ref);
-      l += part[2 * r + 1] * f;
-      acc += *(const v4f *)(part + 2 * k.sh.rows + r * D + col) * f;
+    for (int i0 = slice; i0 < n; i0 += 4 * SLICES) {
+      float2 ml[4];
+      v4f v[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const float *part = parts + of[min(i0 + SLICES * j, n - 1)] * size;
+        ml[j] = *(const float2 *)(part + 2 * row);
+        v[j] = *(const v4f *)(part + 2 * k.sh.rows + row * D + col);
+      }
+      float most = m;
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (i0 + SLICES * j < n) most = fmaxf(most, ml[j].x);
+      const float ref = most == -INFINITY ? 0.0f : most, was = exp2_of(m - ref);
+      m = most, l *= was, acc *= was;
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (i0 + SLICES * j < n) {
+          const float f = exp2_of(ml[j].x - ref);
+          l += ml[j].y * f;
+          acc += v[j] * f;
+        }
     }
+    if (SLICES > 1) {
+      __syncthreads();  // (the rows before)
+      sums[threadIdx.x] = acc, stats[threadIdx.x] = make_float2(m, l);
+      __syncthreads();
+      if (slice) continue;
+      for (int i = 1; i < SLICES; i++) m = fmaxf(m, stats[threadIdx.x + COLS * i].x);
+      const float ref = m == -INFINITY ? 0.0f : m;
+      l = 0.0f, acc = v4f{};
+      for (int i = 0; i < SLICES; i++) {
+        const float2 other = stats[threadIdx.x + COLS * i];
+        const float f = exp2_of(other.x - ref);
+        l += other.y * f;
+        acc += sums[threadIdx.x + COLS * i] * f;
+      }
+    }
+    if (r >= t.rows) continue;
     const int32_t i0 = token_of(k.sh, t.r0 + r), g = t.r0 + r - i0 * k.sh.group;
     float *out = (float *)(k.a.out + (t.begin + i0) * k.a.out_stride) + (int64_t)(t.h * k.sh.group + g) * k.c.dim;
     if (col < k.c.dim) *(v4f *)(out + col) = l != 0.0f ? acc / l : v4f{0.f, 0.f, 0.f, 0.f};
@@ -807,18 +840,17 @@ __global__ __launch_bounds__(1024) void plan_kernel(Call k) {
   for (int32_t i = threadIdx.x; i <= sh.blocks; i += 1024) {
     int32_t at = share_start(all, i, sh.blocks), first, size;
     if (at < all) {
-      find(at, first, size);
-      if (at - first <= near) at = first;
-      else if (first + size - at <= near) at = first + size;
+      Start o = find(at, first, size);
+      if (at - first <= near) {
+        at = first, o.step = 0;
+      } else if (first + size - at <= near) {
+        at = first + size;
+        if (at < all) o = find(at, first, size);
+      }
+      if (i < sh.blocks) p.first[i] = o;
     }
     p.edge[i] = at;
-  }
-  __syncthreads();
-  for (int32_t i = threadIdx.x; i < sh.blocks; i += 1024) {
-    int32_t first, size;
-    p.tail[i].last = -1;
-    if (p.edge[i] >= p.edge[i + 1]) continue;
-    p.first[i] = find(p.edge[i], first, size);
+    if (i < sh.blocks) p.tail[i].last = -1;
   }
 }
 
@@ -1289,9 +1321,13 @@ hipError_t launch(const Attention &a, const Cache &c, const Batch &b, hipStream_
     else
       hipLaunchKernelGGL((c.f16 ? rows_kernel<D, 1, false> : rows_kernel<D, 0, false>), blocks, dim3(256), 0, s, call);
   }
-  // (a block of join_kernel takes 1024 / D rows at a time)
-  const dim3 join(call.sh.blocks, std::min(call.sh.rows * D / 1024, 8));
-  if (call.sh.shared) hipLaunchKernelGGL(join_kernel<D>, join, dim3(256), 0, s, call, edge);
+  // (few rows: their parts sliced)
+  constexpr int SLICES = 4;
+  const int64_t rows = std::min<int64_t>((int64_t)b.longest * call.sh.group, call.sh.rows);
+  if (call.sh.shared && rows <= 4)
+    hipLaunchKernelGGL((join_kernel<D, SLICES>), dim3(call.sh.blocks, (rows * D * SLICES + 1023) / 1024), dim3(256), 0, s, call, edge);
+  else if (call.sh.shared)
+    hipLaunchKernelGGL((join_kernel<D, 1>), dim3(call.sh.blocks, std::min<int64_t>((rows * D + 1023) / 1024, 8)), dim3(256), 0, s, call, edge);
   return hipGetLastError();
 }
 
