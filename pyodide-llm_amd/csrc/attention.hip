@@ -1284,13 +1284,17 @@ Share share_of(const Cache &c, const Batch &b, int32_t heads, int32_t a_cu, int3
   sh.countable = tiles * c.heads * steps < INT32_MAX && rows * sh.group < (int64_t)1 << 32;
   return sh;
 }
-// Where a sequence has room for four steps at most, a block takes a tile whole: two launches, the shares and their join cost more
-// than three more steps (a head of 128 int8: 1.2 us a step alone; measured over 16 to 4096 positions).
+// Where a sequence has room for four steps at most, a block takes a tile whole: the shares and the second launch that joins them
+// cost more than three more steps.  For eight, where the sequences and heads alone give every compute unit a block.  Measured, whole /
+// shared (us), one token a sequence, heads of 128 int8 (a step: 256 positions), 8 of keys: 250 positions of 1 sequence 10.2 / 13.3, of
+// 32 sequences 12.0 / 16.6; 500 of 32 12.7 / 19.8; 1000 of 32 16.7 / 23.0; 1800 of 1 20.4 / 13.6, of 8 22.3 / 18.9, of 32 30.1 / 34.8,
+// of 100 87.7 / 90.6.  (Longer ones gain 2 us and more, too, but lose as much as 15 where one sequence is longer than the others.)
 constexpr int kWholeSteps = 4;
 Share few_share(const Cache &c, const Batch &b, int32_t heads) {
   const int32_t d = padded(c.dim);
   Share sh = share_of(c, b, heads, few_blocks_a_cu(d, c.f16), kFewRows, few_np(d, c.f16) == 16 ? 8 : 7, false);
-  if (((int64_t)b.width << c.shift) <= (int64_t)kWholeSteps << sh.log && b.sequences < 1 << 20) {
+  const int64_t most = (int64_t)b.sequences * c.heads >= cu_count() ? 2 * kWholeSteps : kWholeSteps;
+  if (((int64_t)b.width << c.shift) <= most << sh.log && b.sequences < 1 << 20) {
     sh.whole = (b.longest * sh.group + kFewRows - 1) / kFewRows;
     sh.shared = false;
   }

@@ -185,6 +185,19 @@ def test_few_rows_or_many(pkg, arena, form, dim, new, lengths, width):
     check(p, queries(rng, p, 8))
 
 
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("sequences, longest, dim", [(20, 900, 64), (32, 1900, 128), (33, 1000, 64)])
+def test_many_sequences(pkg, arena, form, sequences, longest, dim):
+    """a token each of many sequences of all lengths, with 8 heads of keys: a block a tile from as many on as the GPU has
+    compute units"""
+    rng = np.random.default_rng(sequences)
+    arena.reset()
+    lengths = [1 + i * (longest - 1) // (sequences - 1) for i in range(sequences)]
+    p = Paged(pkg, arena, rng, form, 8, dim, 64, lengths, [1] * sequences, extra_width=0, longest=1)
+    p.fill(rng)
+    check(p, queries(rng, p, 8 if dim == 128 else 16))
+
+
 @pytest.mark.parametrize("starts", [[0, 5, 3, 9], [-4, 2, 100, 9], [3, 3, 8, 9], [0, 9, 0, 9]])
 @pytest.mark.parametrize("longest", [0, 1])
 def test_contradicting_starts(pkg, arena, starts, longest):
