@@ -294,7 +294,11 @@ struct Elements {
 };
 
 // ---- a few rows: 16 a block, the positions split over its waves and over blocks ----------------------------------------
-// Bound by the cache's bytes.  A wave takes 4 NP positions a step: lane l (m = l % 16, q = l / 16) holds 16 dimensions of a key
+// Bound by the cache's bytes.  A token each of 32 sequences of 1200 to 8000 positions (32 query heads, 8 of keys, 128 values, int8:
+// 320 MB) 69 us, one token over 131072 positions in float16 (545 MB) 100 us: 6.1 TB/s while all blocks run, where reading alone
+// reaches 7.1, after 9 us until the first scores are there; 5 tokens each of 8 sequences of 4100 positions (71 MB, each read for
+// two tiles) 28 us.  A second block's worth of loads a compute unit hides neither more nor less (half the positions a step: 78 us for
+// the 72 that the first took then; twice the shares: 81 for 75), nor does another priority.  A wave takes 4 NP positions a step: lane l (m = l % 16, q = l / 16) holds 16 dimensions of a key
 // at a time (row m of an instruction is the position NP (m / 4) + 4 t + m % 4 of its t-th 16, so that the lane's scores are those
 // of the NP positions from NP q on), and of dimension 16 d + m the values of those NP positions.  Everything goes from
 // memory to registers: the waves share nothing, and the next step's keys are on their way while this one's weights are formed.
@@ -700,7 +704,9 @@ __global__ __launch_bounds__(256) void join_kernel(Call k, const int32_t *edge) 
 }
 
 // ---- prompts: 128 rows a block, 32 a wave, over 64 positions a step -----------------------------------------------------
-// Bound by the matrix cores.  A wave's 32 rows are the columns of 32 x 32 x 16 instructions: lane l (row l % 32, h = l / 32) holds
+// Bound by the matrix cores and the softmax's vector instructions, whose times add up here.  2048 tokens behind 6144 (32 query heads, 8
+// of keys, 128 values, int8) 565 us: 425 TFLOP/s of the formula's products, twice that of the instructions' (a library's float16 matrix
+// product reaches 1271); a batch of prompts with heads of 64 float16 values 83 us, 254 TFLOP/s.  A wave's 32 rows are the columns of 32 x 32 x 16 instructions: lane l (row l % 32, h = l / 32) holds
 // of the step's scores those of the positions 32 k + 16 c + 8 h + e (e < 8), which are its operand of the second product for the
 // positions 32 k + 16 c .. + 15.  The block's keys and values go through LDS as float16, two steps' room, each element widened
 // once a block; keys in rows whose number has bits 2 and 3 swapped (the instruction's row 8 j + 4 h + i is position

@@ -6,6 +6,9 @@
 // The sum of squares, its root and y are held in 64 bits and y rounded once to float32: the products of two float32 are exact
 // there, so whatever order the lanes add them in, y is the same float32 but for one value in some 10^8, and an int8 does not
 // depend on how many tokens a launch has.  The 64-bit operations run at float32's rate here.
+//
+// Bound by memory: a block takes a row, whose values stay in registers between the sum and the products.  2048 rows of 4096 values
+// with a residual, readied: 110 MB in 25.5 us, 4.3 TB/s (a copy reaches 5.2); a row of 288 values 2.6 us, a launch.
 #include "common.hpp"
 #include "launch.hpp"
 #include "ready.hpp"
