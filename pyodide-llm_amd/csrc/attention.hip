@@ -724,12 +724,12 @@ struct Start {
 // neighbours together take about the same time and a share of one tile's size ends near every second tile's end.
 HQ_DEV int32_t tile_at(int32_t k, int32_t tiles) { return k & 1 ? tiles - 1 - (k >> 1) : k >> 1; }
 // the plan, in a call's workspace: the shares' tails, their edges (blocks + 1 numbers), the place of each share's first step, and the
-// steps of one head: of all sequences up to s, of the tiles up to a tile of its sequence (tiles from base[s] on)
+// steps of one head: of all sequences up to s, of the tiles up to a tile of its sequence (tiles[s] of them from base[s] on)
 struct Plan {
   Tail *tail;
   int32_t *edge;
   Start *first;
-  int32_t *upto, *base, *tile;
+  int32_t *upto, *base, *tiles, *tile;
 };
 __host__ __device__ inline Plan plan_of(char *work, int32_t blocks, int32_t sequences) {
   Plan p;
@@ -738,21 +738,18 @@ __host__ __device__ inline Plan plan_of(char *work, int32_t blocks, int32_t sequ
   p.edge = (int32_t *)(p.first + blocks);
   p.upto = p.edge + blocks + 1;
   p.base = p.upto + sequences;
-  p.tile = p.base + sequences;
+  p.tiles = p.base + sequences;
+  p.tile = p.tiles + sequences;
   return p;
 }
 int64_t plan_bytes(int64_t blocks, int64_t sequences, int64_t tiles) {
-  return blocks * (int64_t)(sizeof(Tail) + sizeof(Start)) + (blocks + 1 + 2 * sequences + tiles) * 4;
+  return blocks * (int64_t)(sizeof(Tail) + sizeof(Start)) + (blocks + 1 + 3 * sequences + tiles) * 4;
 }
 
 // inclusive sums over a block of 1024 threads
-HQ_DEV int64_t sum_upto(int64_t v, int64_t *wave_sums) {
+HQ_DEV int64_t sum_upto(int32_t each, int64_t *wave_sums) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int64_t w = __shfl_up(v, o, 64);
-    if (lane >= o) v += w;
-  }
+  int64_t v = wave_sums_of(each);
   __syncthreads();
   if (lane == 63) wave_sums[wave] = v;
   __syncthreads();
@@ -766,11 +763,11 @@ __global__ __launch_bounds__(1024) void plan_kernel(Call k) {
   const Cache &c = k.c;
   const Batch &b = k.b;
   __shared__ int64_t wave_sums[16], carry;
-  __shared__ int32_t near_upto[kPlanSequences], near_base[kPlanSequences], near_tile[kPlanTiles];
+  __shared__ int32_t near_upto[kPlanSequences], near_base[kPlanSequences], near_tiles[kPlanSequences], near_tile[kPlanTiles];
   Plan p = plan_of(k.a.work, sh.blocks, b.sequences);
   const int32_t group = sh.group, n = b.sequences;
   // the sums, which only this kernel reads, in LDS where they fit: the searches below are chains of loads
-  if (n <= kPlanSequences && sh.tiles <= kPlanTiles) p.upto = near_upto, p.base = near_base, p.tile = near_tile;
+  if (n <= kPlanSequences && sh.tiles <= kPlanTiles) p.upto = near_upto, p.base = near_base, p.tiles = near_tiles, p.tile = near_tile;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   // a sequence's first tile
   if (threadIdx.x == 0) carry = 0;
@@ -780,7 +777,7 @@ __global__ __launch_bounds__(1024) void plan_kernel(Call k) {
     const int32_t tiles = s < n ? (sequence_of(b, s).count * group + sh.rows - 1) / sh.rows : 0;
     const int64_t upto = sum_upto(tiles, wave_sums) + carry;
     // (sequences that overlap could have more tiles than there is room for: those past it have none)
-    if (s < n) p.base[s] = upto <= sh.tiles ? (int32_t)upto - tiles : -1;
+    if (s < n) p.base[s] = (int32_t)upto - tiles, p.tiles[s] = upto <= sh.tiles ? tiles : 0;
     __syncthreads();
     if (threadIdx.x == 1023) carry = upto;
     __syncthreads();
@@ -788,17 +785,12 @@ __global__ __launch_bounds__(1024) void plan_kernel(Call k) {
   // a tile's steps and those of the sequence's before it, a wave a sequence
   for (int32_t s = wave; s < n; s += 16) {
     const Sequence q = sequence_of(b, s);
-    const int32_t tiles = p.base[s] < 0 ? 0 : (q.count * group + sh.rows - 1) / sh.rows;
+    const int32_t tiles = p.tiles[s];
     int32_t before = 0;
     for (int32_t t0 = 0; t0 < tiles; t0 += 64) {
-      int32_t v = t0 + lane < tiles ? tile_of(k, q, tile_at(t0 + lane, tiles)).steps : 0;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int32_t w = __shfl_up(v, o, 64);
-        if (lane >= o) v += w;
-      }
+      const int32_t v = wave_sums_of(t0 + lane < tiles ? tile_of(k, q, tile_at(t0 + lane, tiles)).steps : 0);
       if (t0 + lane < tiles) p.tile[p.base[s] + t0 + lane] = before + v;
-      before += __shfl(v, 63, 64);
+      before += __builtin_amdgcn_readlane(v, 63);
     }
     if (lane == 0) p.upto[s] = before;
   }
@@ -834,7 +826,7 @@ __global__ __launch_bounds__(1024) void plan_kernel(Call k) {
     o.h = rest / total;
     rest -= o.h * total;
     const int32_t *tile = p.tile + p.base[lo];
-    int32_t t0 = 0, t1 = (sequence_of(b, lo).count * group + sh.rows - 1) / sh.rows - 1;
+    int32_t t0 = 0, t1 = p.tiles[lo] - 1;
     while (t0 < t1) {
       const int32_t mid = (t0 + t1) >> 1;
       if (tile[mid] > rest) t1 = mid;
