@@ -8,7 +8,9 @@
 // depend on how many tokens a launch has.  The 64-bit operations run at float32's rate here.
 //
 // Bound by memory: a block takes a row, whose values stay in registers between the sum and the products.  2048 rows of 4096 values
-// with a residual, readied: 110 MB in 25.5 us, 4.3 TB/s (a copy reaches 5.2); a row of 288 values 2.6 us, a launch.
+// with a residual, readied: 110 MB in 21.7 us, 5.1 TB/s (a copy reaches 5.2); a row of 288 values 2.6 us, a launch.
+#include <algorithm>
+
 #include "common.hpp"
 #include "launch.hpp"
 #include "ready.hpp"
@@ -83,9 +85,10 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormRows a, int32_t n, float
 
 template <int MODE>
 hipError_t launch_norm_mode(const NormRows &a, int32_t n, float eps, int32_t bias, hipStream_t s) {
-  // as few passes as 1024 threads of 4 values allow, and as few threads as those passes need: by the row alone, so that
-  // a token's sums run in one order however many tokens there are
-  const int32_t lanes = (n + 3) / 4, passes = (lanes + 1023) / 1024;
+  // 256 threads of 4 values and up to kNormKeep passes, then up to 1024 threads: several blocks a compute unit, so that some load
+  // while others store (2048 rows of 4096 values: 21.7 us, in one pass of 1024 threads 25.9; of 2048 values 13.4, in one of 512
+  // 14.7; a single row 8.2 us either way).  By the row alone, so that a token's sums run in one order however many tokens there are
+  const int32_t lanes = (n + 3) / 4, passes = std::max((lanes + 1023) / 1024, std::min((lanes + 255) / 256, kNormKeep));
   const int32_t threads = ((lanes + passes - 1) / passes + 63) / 64 * 64;
   const uint32_t wide = a.count < 65536 ? (uint32_t)a.count : 65536u;
   hipLaunchKernelGGL(norm_kernel<MODE>, dim3(wide, ((uint32_t)a.count + wide - 1) / wide), dim3(threads), 0, s, a, n, eps,
