@@ -706,7 +706,7 @@ __global__ __launch_bounds__(256) void join_kernel(Call k, const int32_t *edge) 
 // ---- prompts: 128 rows a block, 32 a wave, over 64 positions a step -----------------------------------------------------
 // Bound by the matrix cores and the softmax's vector instructions, whose times add up here.  2048 tokens behind 6144 (32 query heads, 8
 // of keys, 128 values, int8) 565 us: 425 TFLOP/s of the formula's products, twice that of the instructions' (a library's float16 matrix
-// product reaches 1271); a batch of prompts with heads of 64 float16 values 83 us, 254 TFLOP/s.  A wave's 32 rows are the columns of 32 x 32 x 16 instructions: lane l (row l % 32, h = l / 32) holds
+// product reaches 1271); a batch of prompts with heads of 64 float16 values 82 us, 257 TFLOP/s.  A wave's 32 rows are the columns of 32 x 32 x 16 instructions: lane l (row l % 32, h = l / 32) holds
 // of the step's scores those of the positions 32 k + 16 c + 8 h + e (e < 8), which are its operand of the second product for the
 // positions 32 k + 16 c .. + 15.  The block's keys and values go through LDS as float16, two steps' room, each element widened
 // once a block; keys in rows whose number has bits 2 and 3 swapped (the instruction's row 8 j + 4 h + i is position
