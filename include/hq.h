@@ -321,9 +321,9 @@ typedef struct hq_cache {
  * starts[s]` of lengths[s] positions; position p is on page table[s width + p / page].  starts, lengths and table are
  * device memory and are read when the call's kernels run (a captured call can be replayed with other contents).  An entry
  * of the table outside 0 .. pages - 1 is no page: what would be written there is left out, what is there reads as zeros
- * and is not attended to, as is a position past the table's end or before position 0.  width page is at most 2^30.  Rows
- * that no sequence has are left alone.  longest: no sequence has more new tokens (0: not known), a hint: the results do not
- * depend on it. */
+ * and is not attended to, as is a position past the table's end or before position 0.  Rows that no sequence has are left
+ * alone.  At most 2^24 tokens, 2^22 sequences and 2^30 positions a table.  longest: no sequence has more new tokens (0: not
+ * known), a hint: the results do not depend on it. */
 typedef struct hq_batch {
   const void *starts, *lengths, *table;
   int32_t sequences, tokens, longest, width;

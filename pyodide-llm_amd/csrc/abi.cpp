@@ -435,6 +435,8 @@ int32_t paged_of(const char *who, const hq_cache *cache, const hq_batch *batch, 
   if (((int64_t)batch->width << shift) > 1 << 30)
     return fail(HQ_ERR_ARGUMENT, "%s: a table of %d pages of %d positions", who, batch->width, cache->page);
   if (batch->tokens > (1 << 24)) return fail(HQ_ERR_ARGUMENT, "%s: tokens = %d", who, batch->tokens);
+  // (a launch of two blocks a sequence stays below 2^32 threads)
+  if (batch->sequences > (1 << 22)) return fail(HQ_ERR_ARGUMENT, "%s: sequences = %d", who, batch->sequences);
   c = hq::Cache{(char *)cache->k, (char *)cache->v, (float *)cache->ks, (float *)cache->vs, cache->form == HQ_CACHE_F16,
                 cache->pages, shift, cache->heads, cache->dim};
   const int32_t longest = batch->longest && batch->longest < batch->tokens ? batch->longest : batch->tokens;

@@ -107,6 +107,15 @@ def test_work_bytes_need_no_memory(pkg, L):
     assert L.hq_attention_work_bytes(c, b, 4) == L.hq_attention_work_bytes(*paged(pkg), 4) >= 0
 
 
+def test_too_many(pkg, L):
+    """what a launch's grid or 32-bit positions could not count is refused, a table that covers 2^30 positions is not"""
+    for wrong, words in ((dict(sequences=(1 << 22) + 1), "sequences = "), (dict(sequences=2 ** 31 - 1), "sequences = "),
+                         (dict(width=(1 << 26) + 1), "a table of")):
+        assert L.hq_cache_write_ex(*paged(pkg, **wrong), 4096, 4096, 512, 512, None) == 1
+        assert words in L.hq_last_error_message().decode()
+    assert L.hq_cache_write_ex(*paged(pkg, width=1 << 26, tokens=0), 4096, 4096, 512, 512, None) == 0
+
+
 @pytest.mark.parametrize("none", [dict(tokens=0), dict(sequences=0)])
 def test_calls_without_tokens(pkg, L, none):
     c, b = paged(pkg, starts=None, lengths=None, table=None, **none)
