@@ -343,7 +343,8 @@ int32_t hq_cache_read_ex(const hq_cache *cache, const hq_batch *batch, void *k, 
  * its own among them, where window > 0):
  *   out = sum_j e^(s_j) v_j / sum_j e^(s_j)     s_j = scale q.k_j    (cap > 0: cap tanh(scale q.k_j / cap))
  * and zeros where no position is seen; laid out as q.  To float32's accuracy: sums in float32, products of float32 values
- * held to 22 bits.  Results do not depend on what pages hold at positions that nobody sees, but for a page's positions
+ * held to 22 bits, a weighted value to 2^-25 of the row's largest weight times scale, whatever sizes the values are of that other
+ * rows, or this one with no weight, see (a weight below 2^-126 of the row's largest may count as none).  Results do not depend on what pages hold at positions that nobody sees, but for a page's positions
  * below lengths[s], which the cache's writes have filled.  work: hq_attention_work_bytes bytes (-1: bad arguments), 256-byte
  * aligned, of any content; calls that share it on one stream follow each other, on two they race.  scale > 0. */
 int64_t hq_attention_work_bytes(const hq_cache *cache, const hq_batch *batch, int32_t heads);

@@ -11,9 +11,14 @@
 // rounding of what is left: 22 bits), two instructions a product.  A row of queries is first scaled by the power of two that
 // brings its largest |value| into [2^13, 2^14), so that the second half keeps its bits.  A position's scales multiply its score and
 // its weight.  One pass over the positions holds a running maximum m and sum l of a softmax in base 2:
-//   p_j = 2^(u_j - m + 6),  u_j = s_j log2(e),   l = sum p_j,   acc = sum (p_j vs_j 2^-E) v_j
-// m moves only where a score passes it by 8 (p_j stays below 2^14), so that acc is seldom rescaled; E, the largest exponent of
-// a position's scale so far, keeps a weight times its scale within float16's range whatever the values' size.
+//   p_j = 2^(u_j - m + 7),  u_j = s_j log2(e),   l = sum p_j,   acc = sum (p_j vs_j 2^-E) v_j
+// m, a whole number, moves only where a score passes it by 7 (p_j stays below 2^14), so that acc is seldom rescaled.
+//
+// A weight times its scale has to lie high in float16's range: below 1 its second half, of 2^-24 at least, holds less than 24 bits.
+// While the scales of all positions loaded so far lie within 2^4 of each other, E is the largest one's exponent, the same for all
+// rows: a row's largest p_j vs_j 2^-E is at least 2^2 then, and each is held to 2^-25 of the row's largest and better.  Where they
+// lie further apart, or one is 0 (kApart), a row has an exponent of its own, from the largest p_j vs_j that it sees itself: what a row
+// does not see, or gives no weight, takes nothing from it.  That costs a logarithm a weight more (apart_weights).
 //
 // Layout.  S^T = K Q^T and out^T = V^T P^T: rows are the instructions' columns, so that a lane holds one row's scores (lane % 16)
 // and its maximum, sum and rescaling need no layout change, and the scores' registers are, with the keys taken in the right
@@ -34,8 +39,12 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kFewRows = 16;       // a tile's rows
-constexpr float kRoom = 8.0f, kShift = 6.0f;  // how far a score may pass the maximum; p = 2^(u - m + kShift)
-constexpr int kLeast = -100;  // the exponent of the smallest scale a cache stores (and E's start)
+constexpr float kRoom = 7.0f, kShift = 7.0f;  // how far a score may pass the maximum; p = 2^(u - m + kShift)
+constexpr int kBand = 4;          // how far the exponents of the scales that share one E may lie apart
+constexpr int kNoScale = -101;    // E before the first scale (a cache stores 2^-100 and more)
+constexpr int kMostScale = 126;   // E's largest (2^-E is a float32)
+constexpr int kApart = INT_MAX;   // in E's place: every row has its own
+constexpr int kHeld = 14;         // powers of 2 that leave p and l at an item's end: l counts positions then, acc stays below their values' sum
 
 // ---- rows, positions and shares ---------------------------------------------------------------------------------
 struct Share {
@@ -187,6 +196,18 @@ HQ_DEV float sum_pair(float v) {
   pair32(v, x, y);
   return x + y;
 }
+// the bits of the scales from which on, and below which, a scale is outside [2^low, 2^(high + 1))
+HQ_DEV uint32_t above_bits(int high) { return (uint32_t)(high + 128) << 23; }
+HQ_DEV uint32_t below_bits(int low) { return (uint32_t)(low + 127) << 23; }
+// 2^e, for whatever e came of: 0 below its range
+HQ_DEV float power_within(float e) { return __builtin_amdgcn_ldexpf(1.0f, (int)fminf(fmaxf(e, -300.0f), 100.0f)); }
+// x 2^(from - to + e), from and to whole numbers or -infinity, in one step: neither factor alone need be a float32
+HQ_DEV v4f shifted(v4f x, float from, float to, int e) {
+  const int by = (int)fmaxf(from - to, -1000.0f) + e;
+  return v4f{__builtin_amdgcn_ldexpf(x[0], by), __builtin_amdgcn_ldexpf(x[1], by), __builtin_amdgcn_ldexpf(x[2], by),
+             __builtin_amdgcn_ldexpf(x[3], by)};
+}
+
 // over the lanes l, l ^ 16, l ^ 32, l ^ 48: a row's
 HQ_DEV float max_row(float v) {
   float x, y;
@@ -277,6 +298,46 @@ HQ_DEV void halves_of(const float *x, v8h &hi, v8h &lo) {
   }
 }
 
+// A row whose positions' scales lie apart: its weights are p vs 2^-x, and top is log2 of the largest p vs so far, as p counts now
+struct Apart {
+  float top;
+  int32_t x;
+};
+// ... where all shared E until now: whoever made m had p of 2^(kShift - 1) and more, and a scale of 2^(E - kBand) and more
+HQ_DEV Apart apart_from(int exponent, float m) {
+  return {m == -INFINITY || exponent == kNoScale ? -INFINITY : (float)(exponent + (int)kShift - 1 - kBand), exponent};
+}
+// N scores p (-infinity: not seen; times rowf in base 2) of such a row, whose scales vs are, enter: m, l and the row's exponent move, and
+// its sums are to be multiplied by what comes back.  most: the row's largest score; row_most: the largest over the row's lanes.
+template <int N, class RowMost>
+HQ_DEV float apart_moves(const float (&p)[N], const float (&vs)[N], float rowf, float most, float &m, float &l, Apart &own, RowMost row_most) {
+  const float was = m;
+  if (most > m + kRoom) m = fmaxf(m, ceilf(most));
+  const float drop = was == -INFINITY ? 0.0f : m - was, less = (m == -INFINITY ? 0.0f : m) - kShift;
+  l *= exp2_of(-drop);
+  float top = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < N; e++)
+    top = fmaxf(top, __builtin_fmaf(p[e], rowf, -less) + __builtin_amdgcn_logf(vs[e]));  // (log2; of 0 it is -infinity)
+  own.top = fmaxf(own.top - drop, row_most(top));
+  const float over = own.top - (float)own.x;
+  const int x = own.x;
+  // the largest weight to 2^7, and again only where it has left [1, 2^13]  (a top below -240: all weights are 0 in float32 anyway)
+  if (own.top >= -240.0f && (over > 13.0f || over < 0.0f)) own.x = (int)rintf(own.top) - 7;
+  return power_within((float)(x - own.x) - drop);
+}
+// ... and become weights p vs 2^-x
+template <int N>
+HQ_DEV void apart_weights(float (&p)[N], const float (&vs)[N], float rowf, float m, float &l, int32_t x) {
+  const float less = (m == -INFINITY ? 0.0f : m) - kShift;
+#pragma unroll
+  for (int e = 0; e < N; e++) {
+    p[e] = exp2_of(__builtin_fmaf(p[e], rowf, -less));
+    l += p[e];
+    p[e] = vs[e] == 0.0f ? 0.0f : __builtin_amdgcn_ldexpf(p[e], -x) * vs[e];
+  }
+}
+
 // N consecutive elements of the cache (16 or 8)
 template <int F16, int N>
 struct Elements {
@@ -311,6 +372,7 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
   constexpr int ES = F16 ? 2 : 1, DB = D / 64, DT = D / 16, PITCH = D + 4, NP = few_np(D, F16), WK = 4 * NP, STEP = 4 * WK;
   __shared__ float sums[4][kFewRows][PITCH];
   __shared__ float stats[2][4][kFewRows];
+  __shared__ Apart apart[4][kFewRows];
   __shared__ int32_t parked[4][14];  // a wave's numbers that its steps do not need
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m16 = lane & 15, q4 = lane >> 4;
@@ -435,7 +497,7 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
       for (int i = 0; i < 13; i++) parked[wave][i] = now[i];
     }
     float m = -INFINITY, l = 0.0f;
-    int exponent = kLeast;
+    int exponent = kNoScale, low = kNoScale;  // the largest and the smallest scale's
     v4f acc[DT] = {};
     if (base < stop) {
       while (true) {
@@ -467,14 +529,15 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
         const bool edge = base + WK > every_to || base < every_from || __any(page2 < 0);
         uint32_t seen = ~0u;
         if (edge) {
-          // what the row does not see has no score; what no row sees may hold anything: its scale and values become zeros
+          // what the row does not see has no score; what no row sees may hold anything: its scale becomes one of the others', its values 0
           const int32_t at = base + NP * q4;
           seen = page2 < 0 ? 0u : bits_between(from - at, to - at);
           const uint32_t any = page2 < 0 ? 0u : bits_between(o.t.from - at, o.t.to - at);
+          const uint32_t other = (uint32_t)((exponent == kApart ? 0 : exponent) + 127) << 23;
 #pragma unroll
           for (int e = 0; e < NP; e++) {
             p[e] = kept(p[e], seen, e, 0xff800000u);
-            vs[e] = kept(vs[e], any, e, 0u);
+            vs[e] = kept(vs[e], any, e, other);
           }
           if (F16) {
 #pragma unroll
@@ -486,31 +549,62 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
           }
         }
         // ---- the running maximum and the scales' exponent
-        float most = p[0], wide = vs[0];
+        float most = p[0];
+        uint32_t most_scale = __float_as_uint(vs[0]), least_scale = most_scale;
 #pragma unroll
-        for (int e = 1; e < NP; e++) most = fmaxf(most, p[e]), wide = fmaxf(wide, vs[e]);
-        most = max_row(most) * rowf, wide = max_row(wide);
-        if (__any(most > m + kRoom)) {  // (the first that is seen too: m is -infinity before it)
-          const float m1 = fmaxf(m, most);
-          const float alpha = m1 == -INFINITY ? 0.0f : exp2_of(m - m1);
-          m = m1;
-          l *= alpha;
-#pragma unroll
-          for (int d = 0; d < DT; d++) acc[d] *= alpha;
+        for (int e = 1; e < NP; e++) {
+          most = fmaxf(most, p[e]);
+          most_scale = max(most_scale, __float_as_uint(vs[e])), least_scale = min(least_scale, __float_as_uint(vs[e]));
         }
-        const int e1 = __builtin_amdgcn_readfirstlane((int)(__float_as_uint(wide) >> 23) - 127);
-        if (e1 > exponent && e1 < 128) {  // (128: nothing but NaN)
-          const float by = power_of_2(max(exponent - e1, -126));
+        most = max_row(most) * rowf;
+        if (exponent != kApart && __any(most_scale >= above_bits(exponent) || least_scale < below_bits(low))) {
+          // a scale outside those so far (or a NaN, which says nothing)
+          float high = 0.0f, least = INFINITY;
 #pragma unroll
-          for (int d = 0; d < DT; d++) acc[d] *= by;
-          exponent = e1;
+          for (int e = 0; e < NP; e++) high = fmaxf(high, vs[e]), least = fminf(least, vs[e]);
+          high = max_row(high), least = -max_row(-least);
+          if (least <= high) {
+            const int h1 = max(__builtin_amdgcn_readfirstlane((int)(__float_as_uint(high) >> 23) - 127), exponent);
+            const int l0 = __builtin_amdgcn_readfirstlane((int)(__float_as_uint(least) >> 23) - 127);
+            const int l1 = exponent == kNoScale ? l0 : min(l0, low);
+            if (h1 - l1 <= kBand && h1 <= kMostScale) {
+              if (h1 > exponent) {
+                const float by = power_of_2(max(exponent - h1, -126));
+#pragma unroll
+                for (int d = 0; d < DT; d++) acc[d] *= by;
+              }
+              exponent = h1, low = l1;
+            } else {
+              apart[wave][m16] = apart_from(exponent, m);
+              exponent = kApart;
+            }
+          }
         }
-        const float less = (m == -INFINITY ? 0.0f : m) - kShift, by = power_of_2(-exponent);
+        if (exponent == kApart) {
+          Apart own = apart[wave][m16];
+          const float rescale = apart_moves(p, vs, rowf, most, m, l, own, [](float v) { return max_row(v); });
+          apart[wave][m16] = own;
+          if (__any(rescale != 1.0f)) {
 #pragma unroll
-        for (int e = 0; e < NP; e++) {
-          p[e] = exp2_of(__builtin_fmaf(p[e], rowf, -less));
-          l += p[e];
-          p[e] = p[e] * (vs[e] * by);
+            for (int d = 0; d < DT; d++) acc[d] *= rescale;
+          }
+          apart_weights(p, vs, rowf, m, l, own.x);
+        } else {
+          if (__any(most > m + kRoom)) {  // (the first that is seen too: m is -infinity before it)
+            const float m1 = fmaxf(m, ceilf(most));
+            const float alpha = m1 == -INFINITY ? 0.0f : exp2_of(m - m1);
+            m = m1;
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < DT; d++) acc[d] *= alpha;
+          }
+          const float less = (m == -INFINITY ? 0.0f : m) - kShift, by = power_of_2(-exponent);
+#pragma unroll
+          for (int e = 0; e < NP; e++) {
+            p[e] = exp2_of(__builtin_fmaf(p[e], rowf, -less));
+            l += p[e];
+            p[e] = p[e] * (vs[e] * by);
+          }
         }
         if (edge) {
 #pragma unroll
@@ -541,7 +635,8 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
         next = after_next, next1 = after1, next2 = after2;
       }
     }
-    l = sum_row(l);
+    l = __builtin_amdgcn_ldexpf(sum_row(l), -kHeld);
+    const int own_exponent = (exponent == kApart ? apart[wave][m16].x : exponent) - kHeld;
     // ---- the four waves together
     const Call *after = call_again();
     const int32_t heads = after->c.heads, shared = after->sh.group;
@@ -556,13 +651,11 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
     __syncthreads();
     const float m0 = stats[0][0][m16], m1 = stats[0][1][m16], m2 = stats[0][2][m16], m3 = stats[0][3][m16];
     const float mm = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)), ref = mm == -INFINITY ? 0.0f : mm;
-    const float f = exp2_of(m - ref) * power_of_2(exponent);
     const float ll = stats[1][0][m16] * exp2_of(m0 - ref) + stats[1][1][m16] * exp2_of(m1 - ref) +
                      stats[1][2][m16] * exp2_of(m2 - ref) + stats[1][3][m16] * exp2_of(m3 - ref);
 #pragma unroll
     for (int d = 0; d < DT; d++) {
-      const v4f v = acc[d] * f;
-      *(v4f *)&sums[wave][m16][d * 16 + q4 * 4] = v;
+      *(v4f *)&sums[wave][m16][d * 16 + q4 * 4] = shifted(acc[d], m, ref, own_exponent);
     }
     __syncthreads();
     const int32_t slot = o.step > 0 ? 0 : 1;
@@ -671,14 +764,15 @@ __global__ __launch_bounds__(256) void join_kernel(Call k, const int32_t *edge) 
 #pragma unroll
       for (int j = 0; j < 4; j++)
         if (i0 + SLICES * j < n) most = fmaxf(most, ml[j].x);
-      const float ref = most == -INFINITY ? 0.0f : most, was = exp2_of(m - ref);
-      m = most, l *= was, acc *= was;
+      // (a part's sums can be as large as its weight is small: they are moved in one step)
+      const float ref = most == -INFINITY ? 0.0f : most;
+      l *= exp2_of(m - ref), acc = shifted(acc, m, ref, 0);
+      m = most;
 #pragma unroll
       for (int j = 0; j < 4; j++)
         if (i0 + SLICES * j < n) {
-          const float f = exp2_of(ml[j].x - ref);
-          l += ml[j].y * f;
-          acc += v[j] * f;
+          l += ml[j].y * exp2_of(ml[j].x - ref);
+          acc += shifted(v[j], ml[j].x, ref, 0);
         }
     }
     if (SLICES > 1) {
@@ -691,9 +785,8 @@ __global__ __launch_bounds__(256) void join_kernel(Call k, const int32_t *edge) 
       l = 0.0f, acc = v4f{};
       for (int i = 0; i < SLICES; i++) {
         const float2 other = stats[threadIdx.x + COLS * i];
-        const float f = exp2_of(other.x - ref);
-        l += other.y * f;
-        acc += sums[threadIdx.x + COLS * i] * f;
+        l += other.y * exp2_of(other.x - ref);
+        acc += shifted(sums[threadIdx.x + COLS * i], other.x, ref, 0);
       }
     }
     if (r >= t.rows) continue;
@@ -880,8 +973,9 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
   constexpr bool BOTH = D <= 128;      // whether the registers hold a step's keys and values at once
   __shared__ __align__(16) char keys[2][kPositions * D * 2];
   __shared__ __align__(16) char values[2][kPositions * D * 2];
-  __shared__ __align__(16) float scales[2][2][kPositions];  // of keys, of values (times 2^-exponent)
-  __shared__ int32_t info[2][2];                            // the exponent, which 16 positions are on a page
+  __shared__ __align__(16) float scales[2][2][kPositions];  // of keys, of values (times 2^-exponent, or as they are: kApart)
+  __shared__ int32_t info[2][2];                            // the exponent or kApart, which 16 positions are on a page
+  __shared__ Apart apart[kRows];
   __shared__ int32_t parked[4][10];                         // a wave's numbers that its steps do not need
   // neighbouring shares on one XCD (blocks go round its 8): they read the same keys and values
   int32_t block, u, end;
@@ -1042,7 +1136,8 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
         }
       }
     };
-    int exponent_run = kLeast;  // (wave 1's)
+    // (wave 1's, in one scalar register: the exponent of the largest scale times 8, and how far below it the smallest's is)
+    int band_run = kNoScale * 8;
     const auto store_values = [&](int buf) {
       const uint32_t tid = opaque_lane(threadIdx.x), ln = tid & 63, part = tid % PARTS;
       const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1069,9 +1164,22 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
       sreg = __uint_as_float(__float_as_uint(sreg) & scale_bits);
       if (wave == 0) scales[buf][0][ln] = sreg;
       if (wave == 1) {
-        if (__any(sreg >= power_of_2(exponent_run + 1)))  // (a NaN is not)
-          exponent_run = (int)(wave_max(sreg == sreg ? __float_as_uint(sreg) : 0u) >> 23) - 127;
-        scales[buf][1][ln] = sreg * power_of_2(-exponent_run);
+        const uint32_t bits = __float_as_uint(sreg);
+        if (band_run != kApart) {
+          const int run = band_run >> 3, low = run - (band_run & 7);
+          if (__any(bits >= above_bits(run) || (bits < below_bits(low) && scale_bits))) {
+            // a scale outside those so far (or a NaN, which says nothing)
+            const bool finite = scale_bits && bits < 0x7f800000u;
+            const uint32_t high = wave_max(finite ? bits : 0u), least = ~wave_max(finite ? ~bits : 0u);
+            if (least <= high) {
+              const int h1 = max((int)(high >> 23) - 127, run), l0 = (int)(least >> 23) - 127;
+              const int l1 = run == kNoScale ? l0 : min(l0, low);
+              band_run = h1 - l1 <= kBand && h1 <= kMostScale ? 8 * h1 + (h1 - l1) : kApart;
+            }
+          }
+        }
+        const int exponent_run = band_run == kApart ? kApart : band_run >> 3;
+        scales[buf][1][ln] = exponent_run == kApart ? sreg : sreg * power_of_2(-exponent_run);
         if (ln == 0) info[buf][0] = exponent_run, info[buf][1] = on_page;
       }
     };
@@ -1082,7 +1190,7 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
     }
     // ---- the steps
     float m = -INFINITY, l = 0.0f;
-    int exponent = kLeast;
+    int exponent = kNoScale;
     v16f acc[DT] = {};
     int32_t base = (tile.first + o.step) * kPositions;
     const int32_t stop = base < tile.to ? base + steps * kPositions : base;  // (rows that see nothing: a step without positions)
@@ -1146,38 +1254,60 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
 #pragma unroll
           for (int e = 1; e < 16; e++) most = fmaxf(most, p[e]);
           most = max_pair(most) * rowf;
-          if (__any(most > m + kRoom)) {
-            const float m1 = fmaxf(m, most);
-            const float alpha = m1 == -INFINITY ? 0.0f : exp2_of(m - m1);
-            m = m1;
-            l *= alpha;
-#pragma unroll
-            for (int d = 0; d < DT; d++) acc[d] *= alpha;
-          }
           const int e1 = __builtin_amdgcn_readfirstlane(info[buf][0]);
-          if (e1 > exponent) {
-            const float by = power_of_2(max(exponent - e1, -126));
+          const auto value_scales = [&](float (&vs)[16]) {
 #pragma unroll
-            for (int d = 0; d < DT; d++) acc[d] *= by;
+            for (int i = 0; i < 2; i++) {
+              const v4f v0 = *(const v4f *)(sc + kPositions + 16 * i), v1 = *(const v4f *)(sc + kPositions + 16 * i + 4);
+#pragma unroll
+              for (int e = 0; e < 8; e++) vs[8 * i + e] = e < 4 ? v0[e & 3] : v1[e & 3];
+            }
+          };
+          if (__any(most > m + kRoom) || e1 != exponent || e1 == kApart) {
+            float rescale = 1.0f;
+            if (e1 == kApart) {
+              Apart own = exponent == kApart ? apart[32 * wave + m32] : apart_from(exponent, m);
+              float vs[16];
+              value_scales(vs);
+              rescale = apart_moves(p, vs, rowf, most, m, l, own, [](float v) { return max_pair(v); });
+              apart[32 * wave + m32] = own;
+            } else {
+              if (__any(most > m + kRoom)) {
+                const float m1 = fmaxf(m, ceilf(most));
+                rescale = m1 == -INFINITY ? 0.0f : exp2_of(m - m1);
+                m = m1;
+                l *= rescale;
+              }
+              rescale *= power_of_2(max(exponent - e1, -126));
+            }
+#pragma unroll
+            for (int d = 0; d < DT; d++) acc[d] *= rescale;
             exponent = e1;
           }
-          const float less = (m == -INFINITY ? 0.0f : m) - kShift;
+          if (e1 == kApart) {
+            float vs[16];
+            value_scales(vs);
+            apart_weights(p, vs, rowf, m, l, apart[32 * wave + m32].x);
+          } else {
+            const float less = (m == -INFINITY ? 0.0f : m) - kShift;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              const v4f v0 = *(const v4f *)(sc + kPositions + 16 * i), v1 = *(const v4f *)(sc + kPositions + 16 * i + 4);
+#pragma unroll
+              for (int e = 0; e < 8; e++) {
+                const float w = exp2_of(__builtin_fmaf(p[8 * i + e], rowf, -less));
+                l += w;
+                p[8 * i + e] = w * (e < 4 ? v0[e & 3] : v1[e & 3]);
+              }
+            }
+          }
+          if (edge) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) p[e] = kept(p[e], seen, e, 0u);  // (a NaN scale that others see)
+          }
           v8h ph[2], pl[2];
 #pragma unroll
-          for (int i = 0; i < 2; i++) {
-            const v4f v0 = *(const v4f *)(sc + kPositions + 16 * i), v1 = *(const v4f *)(sc + kPositions + 16 * i + 4);
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-              const float w = exp2_of(__builtin_fmaf(p[8 * i + e], rowf, -less));
-              l += w;
-              p[8 * i + e] = w * (e < 4 ? v0[e & 3] : v1[e & 3]);
-            }
-            if (edge) {
-#pragma unroll
-              for (int e = 0; e < 8; e++) p[8 * i + e] = kept(p[8 * i + e], seen, 8 * i + e, 0u);  // (a NaN scale that others see)
-            }
-            halves_of(p + 8 * i, ph[i], pl[i]);
-          }
+          for (int i = 0; i < 2; i++) halves_of(p + 8 * i, ph[i], pl[i]);
           // ---- out += weights times values
           const uint32_t vat = opaque_lane(m32 * (kPositions * 2) + 16 * ((4 * t + h2) ^ (m32 & 7)));
 #pragma unroll
@@ -1202,7 +1332,7 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
       }
       __syncthreads();
     }
-    l = sum_pair(l);
+    l = __builtin_amdgcn_ldexpf(sum_pair(l), -kHeld);
     // ---- the rows out, or to be joined
     const Call *after = call_again();
     int32_t kept_back[10];
@@ -1213,10 +1343,10 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
     const bool whole = done == kept_back[6];
     if (live) {
       const int thread = opaque_lane(threadIdx.x), m32 = thread & 31, h2 = (thread >> 5) & 1, wave = thread >> 6;
-      const float by = power_of_2(exponent);
+      const int own_exponent = (exponent == kApart ? apart[32 * wave + m32].x : exponent) - kHeld;
       if (whole) {
         const int32_t shared = after->sh.group, dim = after->c.dim;
-        const float per = l != 0.0f ? by / l : 0.0f;
+        const float per = l != 0.0f ? 1.0f / l : 0.0f;
         float *out = (float *)(after->a.out + (begin + token) * after->a.out_stride) + (int64_t)(o.h * shared + g) * dim;
 #pragma unroll
         for (int d = 0; d < DT; d++)
@@ -1224,7 +1354,7 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
           for (int j = 0; j < 4; j++) {
             const int at = 32 * d + 8 * j + 4 * h2;
             v4f v = {acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]};
-            if (32 * d + 8 * j < dim) *(v4f *)(out + at) = v * per;
+            if (32 * d + 8 * j < dim) *(v4f *)(out + at) = shifted(v * per, 0.0f, 0.0f, own_exponent);
           }
       } else {
         float *part = (float *)(after->a.work + after->sh.parts) + (int64_t)(block * 2 + (o.step > 0 ? 0 : 1)) * kRows * (D + 2);
@@ -1235,7 +1365,7 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
 #pragma unroll
           for (int j = 0; j < 4; j++) {
             v4f v = {acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]};
-            *(v4f *)(part + kRows * 2 + r * D + 32 * d + 8 * j + 4 * h2) = v * by;
+            *(v4f *)(part + kRows * 2 + r * D + 32 * d + 8 * j + 4 * h2) = shifted(v, 0.0f, 0.0f, own_exponent);
           }
       }
     }
