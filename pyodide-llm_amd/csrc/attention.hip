@@ -9,8 +9,9 @@
 // Arithmetic.  An element of the cache, int8 or float16, is exact as a float16, so the products run on the float16 matrix
 // instructions with float32 sums; what multiplies it, a query value or a weight, is held as two float16 (its rounding and the
 // rounding of what is left: 22 bits), two instructions a product.  A row of queries is first scaled by the power of two that
-// brings its largest |value| into [2^13, 2^14), so that the second half keeps its bits.  A position's scales multiply its score and
-// its weight.  One pass over the positions holds a running maximum m and sum l of a softmax in base 2:
+// brings its largest |value| into [2^13, 2^14), so that the second half keeps its bits.  A position's scales multiply its score (up to
+// 2^38 before) and its weight; the row's power of two is taken back before the key's scale multiplies (many rows: in steps with a scale
+// of 2^64 and more, else with the rest of the score's factor), so that a score of ordinary size stays one whatever its factors' size.  One pass over the positions holds a running maximum m and sum l of a softmax in base 2:
 //   p_j = 2^(u_j - m + 7),  u_j = s_j log2(e),   l = sum p_j,   acc = sum (p_j vs_j 2^-E) v_j
 // m, a whole number, moves only where a score passes it by 7 (p_j stays below 2^14), so that acc is seldom rescaled.
 //
@@ -44,6 +45,7 @@ constexpr int kBand = 4;          // how far the exponents of the scales that sh
 constexpr int kNoScale = -101;    // E before the first scale (a cache stores 2^-100 and more)
 constexpr int kMostScale = 126;   // E's largest (2^-E is a float32)
 constexpr int kApart = INT_MAX;   // in E's place: every row has its own
+constexpr uint32_t kLargeScale = (uint32_t)(64 + 127) << 23;  // 2^64's bits
 constexpr int kHeld = 14;         // powers of 2 that leave p and l at an item's end: l counts positions then, acc stays below their values' sum
 
 // ---- rows, positions and shares ---------------------------------------------------------------------------------
@@ -298,6 +300,14 @@ HQ_DEV void halves_of(const float *x, v8h &hi, v8h &lo) {
   }
 }
 
+// A row's products (times 2^up) take 2^-up first, then a key's scale, so that nothing passes a float32 that the score itself does not
+// pass: `first`, and the rest of the row's factor (with a large query's power of two: there the score does), in base 2 or a cap's.
+HQ_DEV float first_of_large(int32_t up) { return power_of_2(-max(up, 0)); }
+HQ_DEV float factor_of_large(int32_t up, float scale, float cap) {
+  const float rowf = scale * power_of_2(-min(up, 0));
+  return cap > 0.0f ? rowf / cap : rowf * kLog2e;
+}
+
 // A row whose positions' scales lie apart: its weights are p vs 2^-x, and top is log2 of the largest p vs so far, as p counts now
 struct Apart {
   float top;
@@ -373,6 +383,7 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
   __shared__ float sums[4][kFewRows][PITCH];
   __shared__ float stats[2][4][kFewRows];
   __shared__ Apart apart[4][kFewRows];
+  __shared__ float firsts[4][kFewRows];  // first_of_large of the rows
   __shared__ int32_t parked[4][14];  // a wave's numbers that its steps do not need
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m16 = lane & 15, q4 = lane >> 4;
@@ -473,7 +484,7 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
       most = max_row(most);
       const int up = most > 0.0f ? min(140 - (int)(__float_as_uint(most) >> 23), 126) : 0;
       const float by = power_of_2(up);
-      rowf = a.scale * power_of_2(-up);
+      firsts[wave][m16] = first_of_large(up), rowf = factor_of_large(up, a.scale, a.cap);
 #pragma unroll
       for (int d = 0; d < DB; d++)
 #pragma unroll
@@ -483,9 +494,8 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
           halves_of(e, qh[d][i], ql[d][i]);
         }
     }
-    // a score is its product times rowf, in base 2; with a cap row_cap comes before the tanh instead
-    const float cap = a.cap, row_cap = rowf / cap;
-    rowf = cap > 0.0f ? 1.0f : rowf * kLog2e;
+    // a score is its product times first, its key's scale and rowf, in base 2; with a cap that is the tanh's argument
+    const float cap = a.cap;
     const int32_t sees = before + token + 1;
     const int32_t to = min(sees, reach), from = a.window ? sees - a.window : 0;  // the lane's row's own positions
     // the positions that every row sees lie in [every_from, every_to)
@@ -519,12 +529,15 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
         load_keys(next, page_in(b, c, next1, next + NP * (m16 >> 2)));
         const int32_t next_page2 = page_in(b, c, next2, next + NP * q4);
         float p[NP];
+        float by_row = rowf;
+        const float first = firsts[wave][m16];
 #pragma unroll
-        for (int e = 0; e < NP; e++) p[e] = s[e >> 2][e & 3] * ks[e];
+        for (int e = 0; e < NP; e++) p[e] = s[e >> 2][e & 3] * first * ks[e];
         if (cap > 0.0f) {
           const float bend = opaque(0.55f), twice = opaque(2.0f * kLog2e);
 #pragma unroll
-          for (int e = 0; e < NP; e++) p[e] = cap * kLog2e * tanh_of(p[e] * row_cap, bend, twice);
+          for (int e = 0; e < NP; e++) p[e] = cap * kLog2e * tanh_of(p[e] * by_row, bend, twice);
+          by_row = 1.0f;
         }
         const bool edge = base + WK > every_to || base < every_from || __any(page2 < 0);
         uint32_t seen = ~0u;
@@ -556,7 +569,7 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
           most = fmaxf(most, p[e]);
           most_scale = max(most_scale, __float_as_uint(vs[e])), least_scale = min(least_scale, __float_as_uint(vs[e]));
         }
-        most = max_row(most) * rowf;
+        most = max_row(most) * by_row;
         if (exponent != kApart && __any(most_scale >= above_bits(exponent) || least_scale < below_bits(low))) {
           // a scale outside those so far (or a NaN, which says nothing)
           float high = 0.0f, least = INFINITY;
@@ -582,13 +595,13 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
         }
         if (exponent == kApart) {
           Apart own = apart[wave][m16];
-          const float rescale = apart_moves(p, vs, rowf, most, m, l, own, [](float v) { return max_row(v); });
+          const float rescale = apart_moves(p, vs, by_row, most, m, l, own, [](float v) { return max_row(v); });
           apart[wave][m16] = own;
           if (__any(rescale != 1.0f)) {
 #pragma unroll
             for (int d = 0; d < DT; d++) acc[d] *= rescale;
           }
-          apart_weights(p, vs, rowf, m, l, own.x);
+          apart_weights(p, vs, by_row, m, l, own.x);
         } else {
           if (__any(most > m + kRoom)) {  // (the first that is seen too: m is -infinity before it)
             const float m1 = fmaxf(m, ceilf(most));
@@ -601,7 +614,7 @@ __global__ __launch_bounds__(256, few_blocks_a_cu(D, F16)) void few_kernel(Call)
           const float less = (m == -INFINITY ? 0.0f : m) - kShift, by = power_of_2(-exponent);
 #pragma unroll
           for (int e = 0; e < NP; e++) {
-            p[e] = exp2_of(__builtin_fmaf(p[e], rowf, -less));
+            p[e] = exp2_of(__builtin_fmaf(p[e], by_row, -less));
             l += p[e];
             p[e] = p[e] * (vs[e] * by);
           }
@@ -807,7 +820,7 @@ __global__ __launch_bounds__(256) void join_kernel(Call k, const int32_t *edge) 
 //
 // Which block does what is worked out once a call (plan_kernel): steps of all (sequence, head, row tile) in a row, shared evenly,
 // a share's end moved to an item's end that is near, so that few items are shared and their parts joined (join_kernel).
-constexpr int kRows = 128, kPositions = 64;
+constexpr int kRows = 128, kPositions = 64, kAnyLarge = 16;
 
 // where in the row of all steps: sequence, row tile, head and step of the item
 struct Start {
@@ -974,8 +987,9 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
   __shared__ __align__(16) char keys[2][kPositions * D * 2];
   __shared__ __align__(16) char values[2][kPositions * D * 2];
   __shared__ __align__(16) float scales[2][2][kPositions];  // of keys, of values (times 2^-exponent, or as they are: kApart)
-  __shared__ int32_t info[2][2];                            // the exponent or kApart, which 16 positions are on a page
+  __shared__ int32_t info[2][2];  // the exponent or kApart; a bit for each 16 positions on a page, and one where a key's scale is large
   __shared__ Apart apart[kRows];
+  __shared__ int32_t ups[kRows];  // the power of two that a row's queries are multiplied by
   __shared__ int32_t parked[4][10];                         // a wave's numbers that its steps do not need
   // neighbouring shares on one XCD (blocks go round its 8): they read the same keys and values
   int32_t block, u, end;
@@ -1029,6 +1043,7 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
       const int up = most > 0.0f ? min(140 - (int)(__float_as_uint(most) >> 23), 126) : 0;
       const float by = live ? power_of_2(up) : 0.0f;
       rowf = a.scale * power_of_2(-up);
+      ups[32 * wave + m32] = up;
 #pragma unroll
       for (int k = 0; k < KS; k++) {
         const int at = 16 * k + 8 * h2;
@@ -1039,8 +1054,8 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
       }
     }
     // (as in few_kernel)
-    const float cap = a.cap, row_cap = rowf / cap;
-    rowf = cap > 0.0f ? 1.0f : rowf * kLog2e;
+    const float cap = a.cap;
+    rowf = cap > 0.0f ? rowf / cap : rowf * kLog2e;
     // ---- staging: the wave's 16 keys (consecutive in memory), the thread's 16 (8) positions of some dimensions, a scale a lane
     // (what the thread's number gives is formed anew in every step: registers are what the rows leave few of)
     constexpr int ROW = D * ES / 16, PARTS = F16 ? 8 : 4, EACH = kPositions / PARTS;
@@ -1162,7 +1177,11 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
         }
       }
       sreg = __uint_as_float(__float_as_uint(sreg) & scale_bits);
-      if (wave == 0) scales[buf][0][ln] = sreg;
+      if (wave == 0) {
+        scales[buf][0][ln] = sreg;
+        const bool any_large = __any(__float_as_uint(sreg) >= kLargeScale);  // (or a NaN)
+        if (ln == 0) info[buf][1] = on_page | (any_large ? kAnyLarge : 0);
+      }
       if (wave == 1) {
         const uint32_t bits = __float_as_uint(sreg);
         if (band_run != kApart) {
@@ -1180,7 +1199,7 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
         }
         const int exponent_run = band_run == kApart ? kApart : band_run >> 3;
         scales[buf][1][ln] = exponent_run == kApart ? sreg : sreg * power_of_2(-exponent_run);
-        if (ln == 0) info[buf][0] = exponent_run, info[buf][1] = on_page;
+        if (ln == 0) info[buf][0] = exponent_run;
       }
     };
     {
@@ -1228,18 +1247,27 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
             s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, qh[k], s, 0, 0, 0);
           }
           float p[16];
-          const int32_t pages_here = __builtin_amdgcn_readfirstlane(info[buf][1]) >> (2 * t) & 3;
+          const int32_t flags = __builtin_amdgcn_readfirstlane(info[buf][1]), pages_here = flags >> (2 * t) & 3;
           const float *sc = &scales[buf][0][32 * t + 8 * h2];
+          float by_row = rowf;
+          v4f ks[4];
 #pragma unroll
-          for (int i = 0; i < 2; i++) {
-            const v4f k0 = *(const v4f *)(sc + 16 * i), k1 = *(const v4f *)(sc + 16 * i + 4);
+          for (int i = 0; i < 4; i++) ks[i] = *(const v4f *)(sc + 16 * (i >> 1) + 4 * (i & 1));
+          if (flags & kAnyLarge) {
+            const int32_t up = ups[32 * wave + m32];
+            const float first = first_of_large(up);
 #pragma unroll
-            for (int e = 0; e < 8; e++) p[8 * i + e] = s[8 * i + e] * (e < 4 ? k0[e & 3] : k1[e & 3]);
+            for (int e = 0; e < 16; e++) p[e] = s[e] * first * ks[e >> 2][e & 3];
+            by_row = factor_of_large(up, call_again()->a.scale, cap);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; e++) p[e] = s[e] * ks[e >> 2][e & 3];
           }
           if (cap > 0.0f) {
             const float bend = opaque(0.55f), twice = opaque(2.0f * kLog2e);
 #pragma unroll
-            for (int e = 0; e < 16; e++) p[e] = cap * kLog2e * tanh_of(p[e] * row_cap, bend, twice);
+            for (int e = 0; e < 16; e++) p[e] = cap * kLog2e * tanh_of(p[e] * by_row, bend, twice);
+            by_row = 1.0f;
           }
           const bool edge = at32 + 32 > every_to || at32 < every_from || pages_here != 3;
           uint32_t seen = ~0u;
@@ -1253,7 +1281,7 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
           float most = p[0];
 #pragma unroll
           for (int e = 1; e < 16; e++) most = fmaxf(most, p[e]);
-          most = max_pair(most) * rowf;
+          most = max_pair(most) * by_row;
           const int e1 = __builtin_amdgcn_readfirstlane(info[buf][0]);
           const auto value_scales = [&](float (&vs)[16]) {
 #pragma unroll
@@ -1269,7 +1297,7 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
               Apart own = exponent == kApart ? apart[32 * wave + m32] : apart_from(exponent, m);
               float vs[16];
               value_scales(vs);
-              rescale = apart_moves(p, vs, rowf, most, m, l, own, [](float v) { return max_pair(v); });
+              rescale = apart_moves(p, vs, by_row, most, m, l, own, [](float v) { return max_pair(v); });
               apart[32 * wave + m32] = own;
             } else {
               if (__any(most > m + kRoom)) {
@@ -1287,7 +1315,7 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
           if (e1 == kApart) {
             float vs[16];
             value_scales(vs);
-            apart_weights(p, vs, rowf, m, l, apart[32 * wave + m32].x);
+            apart_weights(p, vs, by_row, m, l, apart[32 * wave + m32].x);
           } else {
             const float less = (m == -INFINITY ? 0.0f : m) - kShift;
 #pragma unroll
@@ -1295,7 +1323,7 @@ __global__ __launch_bounds__(256, rows_blocks_a_cu(D)) void rows_kernel(Call) {
               const v4f v0 = *(const v4f *)(sc + kPositions + 16 * i), v1 = *(const v4f *)(sc + kPositions + 16 * i + 4);
 #pragma unroll
               for (int e = 0; e < 8; e++) {
-                const float w = exp2_of(__builtin_fmaf(p[8 * i + e], rowf, -less));
+                const float w = exp2_of(__builtin_fmaf(p[8 * i + e], by_row, -less));
                 l += w;
                 p[8 * i + e] = w * (e < 4 ? v0[e & 3] : v1[e & 3]);
               }

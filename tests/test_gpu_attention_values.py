@@ -200,3 +200,58 @@ def test_not_a_number_among_sizes(pkg, arena, form, new):
     p.send()
     got = p.run_attention(q, 0.125)
     assert np.isnan(got[-1]).all() and (np.abs(got - want)[:-1] <= far[:-1]).all()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("new", NEW)
+@pytest.mark.parametrize("keys, asks, cap", [(1e35, 1e-35, 0.0), (1e37, 1e-37, 0.0), (1e35, 1e-35, 5.0), (1e20, 1e-20, 0.0),
+                                             (1e-28, 1e28, 0.0), (1e-25, 1e25, 3.0)])
+def test_large_keys_small_queries(pkg, arena, form, new, keys, asks, cap):
+    """scores of ordinary size whose factors are near the ends of float32"""
+    rng = np.random.default_rng(15)
+    p = made(pkg, arena, rng, form, [300], [new])
+    for j in range(300):
+        k, v, _ = p.vectors(0, [j])
+        p.put(0, j, (k[0] * keys).astype(F), v[0].astype(F))
+    p.send()
+    check(p, queries(rng, p, 2) * F(asks), cap=cap)
+
+
+def check_seen(p, q, at):
+    """rows that do not see position `at`, or give it nothing, are the mean of the values they see, whose scores are all near 0 (below
+    2^-40); rows that it takes are the caller's to check"""
+    got = p.run_attention(q, 1 / np.sqrt(p.dim))
+    assert np.isfinite(got).all()
+    k, v, there = p.vectors(0, range(p.lengths[0]))
+    for t, s, position in p.positions():
+        for h in range(q.shape[1]):
+            if position >= at and h == 0:
+                continue
+            seen = np.array([j for j in range(position + 1) if j != at])
+            mean = v[seen, 0].mean(0)
+            assert (np.abs(got[t, h] - mean) <= np.abs(v[seen, 0]).mean(0) * (2.0 ** -20 + np.sqrt(seen.size) * 2.0 ** -22)).all()
+    return got
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("new", [1, 8, 100])
+@pytest.mark.parametrize("others", [1.0, 1e-20, 0.0])
+def test_one_large_key(pkg, arena, form, new, others):
+    """a key of 1e35 among small ones or zeros: 1e-30 times it takes all or nothing, by its sign, and what does not see it is as ever"""
+    rng = np.random.default_rng(16)
+    p = made(pkg, arena, rng, form, [300], [new])
+    at = 299 - new // 2
+    for j in range(300):
+        k, v, _ = p.vectors(0, [j])
+        k = k[0] * others
+        if j == at:
+            k[:] = 0
+            k[0, 3] = 1e35
+        p.put(0, j, k.astype(F), v[0].astype(F))
+    p.send()
+    q = queries(rng, p, 2) * F(1e-30)
+    q[:, 0, 3], q[:, 1, 3] = 1e-30, -1e-30
+    got = check_seen(p, q, at)
+    value = p.vectors(0, [at])[1][0, 0]
+    first = at - (300 - new)
+    assert (np.abs(got[first:, 0] - value) <= 2.0 ** -20 * np.abs(value)).all()
