@@ -1472,7 +1472,9 @@ bool few_rows(const Cache &c, const Batch &b, int32_t heads) {
 template <int D>
 hipError_t launch(const Attention &a, const Cache &c, const Batch &b, hipStream_t s) {
   const bool few = few_rows(c, b, a.heads);
-  const Call call{a, c, b, few ? few_share(c, b, a.heads) : rows_share(c, b, a.heads)};
+  Call call{a, c, b, few ? few_share(c, b, a.heads) : rows_share(c, b, a.heads)};
+  // (a window past all positions is none; a position less the window then stays above 32 bits' lowest, 2^24 before the first too)
+  call.a.window = std::min(a.window, kMostPositions);
   const dim3 blocks = call.sh.whole ? dim3(b.sequences, call.sh.whole, c.heads) : dim3(call.sh.blocks);
   const int32_t *edge = nullptr;
   if (few) {
