@@ -85,13 +85,17 @@ class Forward:
         token's row (a buffer of this object's)."""
         torch, lib, ck, s = self.torch, self.lib, self.ck, self.ck.shape
         count, sequences = x.shape[0], lengths.shape[0]
-        if not (0 < count <= self.tokens and 0 < sequences <= self.sequences and x.shape[1] == s.dim and x.is_contiguous()
-                and tuple(table.shape) == (sequences, self.width) and starts.shape[0] == sequences + 1):
-            raise ValueError(f"refused: {tuple(x.shape)} embeddings, a table of {tuple(table.shape)} and {starts.shape[0]} "
-                             f"starts for steps of {self.tokens} tokens, {self.sequences} sequences of {self.width} pages")
-        for name, t in (("starts", starts), ("lengths", lengths), ("table", table)):
-            if t.dtype != torch.int32 or not t.is_contiguous() or t.device != x.device:
-                raise ValueError(f"refused: {name} is not int32 beside the embeddings, in one piece")
+        if not (x.dim() == 2 and 0 < count <= self.tokens and 0 < sequences <= self.sequences and x.shape[1] == s.dim
+                and tuple(table.shape) == (sequences, self.width) and tuple(starts.shape) == (sequences + 1,)
+                and lengths.dim() == 1):
+            raise ValueError(f"refused: {tuple(x.shape)} embeddings, a table of {tuple(table.shape)}, {tuple(starts.shape)} starts "
+                             f"and {tuple(lengths.shape)} lengths for steps of {self.tokens} tokens, {self.sequences} sequences "
+                             f"of {self.width} pages")
+        # the calls take addresses: what lies there has to be what they read (and write: x is the residual stream)
+        for name, t, kind in (("x", x, torch.float32), ("starts", starts, torch.int32), ("lengths", lengths, torch.int32),
+                              ("table", table, torch.int32)):
+            if t.dtype != kind or not t.is_contiguous() or t.device != self.y.device:
+                raise ValueError(f"refused: {name} is {t.dtype} on {t.device}, not {kind} on {self.y.device} in one piece")
         stream = torch.cuda.current_stream()
         batch = Batch(starts.data_ptr(), lengths.data_ptr(), table.data_ptr(), sequences, count, longest, self.width)
         needed = lib.hq_attention_work_bytes(self.caches[0], batch, s.heads)
