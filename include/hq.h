@@ -300,7 +300,9 @@ int32_t hq_job_path(int32_t kind, int32_t n, int32_t count, int64_t frame, int64
  * interleave's planes and sums (ternary, binary) or sums_x's sums (llama.cpp's blocks), to the bit what those give for y.
  * d, r, y and xq (with xs) may be NULL: r then is not stored (it has to be where d is given), y not stored, or nothing
  * readied.  r may be x; nothing else may overlap.  n a multiple of 32, 128 (planes) or 256 (sums); x, d, w, r, y and their
- * strides 16-byte aligned, frame a multiple of 16, xq and xs 4-byte aligned; eps >= 0. */
+ * strides 16-byte aligned, frame a multiple of 16, xq and xs 4-byte aligned; eps >= 0.  Rows that are written may not reach into
+ * others: x_stride (with r) and y_stride are 4 n and more, frame n and more; activations and scales (with what follows them: n / 8
+ * bytes a token, n / 4 with planes, n / 2 with sums) may share frames side by side. */
 enum { HQ_READY_BIASED = 0, HQ_READY_PLAIN = 1, HQ_READY_PLANES = 2, HQ_READY_SUMS = 3 };
 int32_t hq_norm_ready_ex(void *xq, void *xs, void *y, void *r, const void *x, const void *d, const void *w, int32_t n,
                          float eps, int32_t ready, int32_t count, int32_t frame, int32_t x_stride, int32_t d_stride,

@@ -796,6 +796,20 @@ int32_t hq_norm_ready_ex(void *xq, void *xs, void *y, void *r, const void *x, co
     if (x_stride < 0 || x_stride % 16 || (d && (d_stride < 0 || d_stride % 16)) || (y && (y_stride < 0 || y_stride % 16)))
       return fail(HQ_ERR_ALIGNMENT, "norm_ready: a token stride is not a multiple of 16");
     if (xq && (frame < 0 || frame % 16)) return fail(HQ_ERR_ALIGNMENT, "norm_ready: frame = %d is not a multiple of 16", frame);
+    // (rows that are written must not reach into the next: blocks write them at the same time)
+    const int64_t row = 4 * (int64_t)n;
+    if ((r && x_stride < row) || (y && y_stride < row))
+      return fail(HQ_ERR_ARGUMENT, "norm_ready: x_stride = %d (with r) or y_stride = %d (with y), a token's row takes %lld", x_stride,
+                  y_stride, (long long)row);
+    if (xq && frame < n) return fail(HQ_ERR_ARGUMENT, "norm_ready: frame = %d, a token's activations take %d", frame, n);
+  }
+  if (xq) {
+    // activations and scales in one frame: each token's side by side
+    const int64_t scales = ready == HQ_READY_PLANES ? n / 4 : ready == HQ_READY_SUMS ? n / 2 : n / 8, others = (count - 1) * (int64_t)frame;
+    const int64_t apart = (int64_t)((intptr_t)xs - (intptr_t)xq), at = count > 1 ? (apart % frame + frame) % frame : 0;
+    if (apart < others + n && -apart < others + scales && (at < n || at + scales > frame))
+      return fail(HQ_ERR_ARGUMENT, "norm_ready: xs %lld bytes past xq, frame = %d: activations of %d bytes and scales of %lld overlap",
+                  (long long)apart, frame, n, (long long)scales);
   }
   if (int32_t st = ensure_device()) return st;
   const hq::NormRows a{(char *)xq, (char *)xs, (char *)y, (char *)r, (const char *)x, (const char *)d, (const char *)w,

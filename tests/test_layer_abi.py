@@ -33,6 +33,28 @@ def test_norm_refusals(L, wrong, code, words):
     assert L.hq_last_error() == code and words in L.hq_last_error_message().decode()
 
 
+@pytest.mark.parametrize("wrong, words", [
+    (dict(x_stride=1008), "x_stride = 1008"), (dict(x_stride=0), "x_stride = 0"), (dict(x_stride=1008, d=None), "x_stride = 1008"),
+    (dict(y=4096, y_stride=1008), "y_stride = 1008"), (dict(y=4096, y_stride=0), "y_stride = 0"), (dict(frame=240), "frame = 240"),
+    (dict(frame=0), "frame = 0"),
+])
+def test_norm_rows_that_overlap(L, wrong, words):
+    """rows of several tokens that are written may not reach into each other"""
+    assert norm(L, **wrong) == 1
+    assert L.hq_last_error() == 1 and words in L.hq_last_error_message().decode()
+
+
+@pytest.mark.parametrize("wrong", [
+    dict(xs=4096 + 256, frame=256), dict(xs=4096 + 256, frame=272), dict(xs=4096 + 256, frame=304, ready=2),
+    dict(xs=4096 + 256, frame=368, ready=3), dict(xs=4096), dict(xs=4096 + 252), dict(xs=4096 - 16), dict(xs=4096 + 320, frame=320),
+    dict(xs=4096 + 128, count=1), dict(xs=4096 - 16, count=1),
+])
+def test_norm_scales_that_overlap(L, wrong):
+    """scales (n / 8 bytes; with planes n / 4, with sums n / 2) may lie in the activations' frames, beside them"""
+    assert norm(L, **wrong) == 1
+    assert L.hq_last_error() == 1 and "overlap" in L.hq_last_error_message().decode()
+
+
 def test_norm_without_tokens(L):
     assert norm(L, x=None, count=0) == 0
 
