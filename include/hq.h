@@ -325,7 +325,9 @@ typedef struct hq_cache {
  * of the table outside 0 .. pages - 1 is no page: what would be written there is left out, what is there reads as zeros
  * and is not attended to, as is a position past the table's end or before position 0.  Rows that no sequence has are left
  * alone.  At most 2^24 tokens, 2^22 sequences and 2^30 positions a table.  longest: no sequence has more new tokens (0: not
- * known), a hint: the results do not depend on it. */
+ * known), a hint that only speed and rounding depend on: attention takes its kernel for a few rows or the prompts' by it, whose sums run
+ * in different orders, so that a last bit may differ.  Not known counts as all tokens: a token each of 32 sequences then takes
+ * the prompts' kernel, twice as long. */
 typedef struct hq_batch {
   const void *starts, *lengths, *table;
   int32_t sequences, tokens, longest, width;

@@ -11,7 +11,9 @@
 // rounding of what is left: 22 bits), two instructions a product.  A row of queries is first scaled by the power of two that
 // brings its largest |value| into [2^13, 2^14), so that the second half keeps its bits.  A position's scales multiply its score (up to
 // 2^38 before) and its weight; the row's power of two is taken back before the key's scale multiplies (many rows: in steps with a scale
-// of 2^64 and more, else with the rest of the score's factor), so that a score of ordinary size stays one whatever its factors' size.  One pass over the positions holds a running maximum m and sum l of a softmax in base 2:
+// of 2^64 and more, else with the rest of the score's factor), so that a score of ordinary size stays one whatever its factors' size.
+//
+// One pass over the positions holds a running maximum m and sum l of a softmax in base 2:
 //   p_j = 2^(u_j - m + 7),  u_j = s_j log2(e),   l = sum p_j,   acc = sum (p_j vs_j 2^-E) v_j
 // m, a whole number, moves only where a score passes it by 7 (p_j stays below 2^14), so that acc is seldom rescaled.
 //
@@ -46,7 +48,7 @@ constexpr int kNoScale = -101;    // E before the first scale (a cache stores 2^
 constexpr int kMostScale = 126;   // E's largest (2^-E is a float32)
 constexpr int kApart = INT_MAX;   // in E's place: every row has its own
 constexpr uint32_t kLargeScale = (uint32_t)(64 + 127) << 23;  // 2^64's bits
-constexpr int kHeld = 14;         // powers of 2 that leave p and l at an item's end: l counts positions then, acc stays below their values' sum
+constexpr int kHeld = 14;         // powers of 2 that p and l lose at an item's end: acc is then no larger than the values' sum
 
 // ---- rows, positions and shares ---------------------------------------------------------------------------------
 struct Share {
@@ -366,7 +368,7 @@ struct Elements {
 
 // ---- a few rows: 16 a block, the positions split over its waves and over blocks ----------------------------------------
 // Bound by the cache's bytes.  A token each of 32 sequences of 1200 to 8000 positions (32 query heads, 8 of keys, 128 values, int8:
-// 320 MB) 69 us, one token over 131072 positions in float16 (545 MB) 100 us: 6.1 TB/s while all blocks run, where reading alone
+// 320 MB) 70 us, one token over 131072 positions in float16 (545 MB) 100 us: 6.1 TB/s while all blocks run, where reading alone
 // reaches 7.1, after 9 us until the first scores are there; 5 tokens each of 8 sequences of 4100 positions (71 MB, each read for
 // two tiles) 28 us.  A second block's worth of loads a compute unit hides neither more nor less (half the positions a step: 78 us for
 // the 72 that the first took then; twice the shares: 81 for 75), nor does another priority.  A wave takes 4 NP positions a step: lane l (m = l % 16, q = l / 16) holds 16 dimensions of a key
@@ -811,10 +813,13 @@ __global__ __launch_bounds__(256) void join_kernel(Call k, const int32_t *edge) 
 
 // ---- prompts: 128 rows a block, 32 a wave, over 64 positions a step -----------------------------------------------------
 // Bound by the matrix cores and the softmax's vector instructions, whose times add up here.  2048 tokens behind 6144 (32 query heads, 8
-// of keys, 128 values, int8) 565 us: 425 TFLOP/s of the formula's products, twice that of the instructions' (a library's float16 matrix
-// product reaches 1271); a batch of prompts with heads of 64 float16 values 82 us, 257 TFLOP/s.  A wave's 32 rows are the columns of 32 x 32 x 16 instructions: lane l (row l % 32, h = l / 32) holds
-// of the step's scores those of the positions 32 k + 16 c + 8 h + e (e < 8), which are its operand of the second product for the
-// positions 32 k + 16 c .. + 15.  The block's keys and values go through LDS as float16, two steps' room, each element widened
+// of keys, 128 values, int8): a call takes 520 us back to back, this kernel all of it but the plan's and the join's 22 (579 us in a
+// profiled run, whose clock is lower): 480 TFLOP/s of the formula's products, twice that of the instructions' (a library's float16 matrix
+// product reaches 1271).  A batch of prompts with heads of 64 float16 values: a call takes 94 us, 224 TFLOP/s (85 us of this kernel in a
+// profiled run).  Where value scales lie apart in every step: 654 and 112 us for 529 and 93 in the same run.
+//
+// A wave's 32 rows are the columns of 32 x 32 x 16 instructions: lane l (row l % 32, h = l / 32) holds of the step's scores those of the
+// positions 32 k + 16 c + 8 h + e (e < 8), which are its operand of the second product for the positions 32 k + 16 c .. + 15.  The block's keys and values go through LDS as float16, two steps' room, each element widened
 // once a block; keys in rows whose number has bits 2 and 3 swapped (the instruction's row 8 j + 4 h + i is position
 // 16 (j / 2) + 8 h + 4 (j % 2) + i), 16-byte chunks XORed with the row so that 8 lanes read 8 bank quads.
 //

@@ -8,7 +8,8 @@
 // depend on how many tokens a launch has.  The 64-bit operations run at float32's rate here.
 //
 // Bound by memory: a block takes a row, whose values stay in registers between the sum and the products.  2048 rows of 4096 values
-// with a residual, readied: 110 MB in 21.7 us, 5.1 TB/s (a copy reaches 5.2); a row of 288 values 2.6 us, a launch.
+// with a residual, readied: 110 MB in 21.4 us a call back to back, 5.2 TB/s, as a copy (22.6 us in a profiled run, whose clock is
+// lower); a row of 288 values 2.8 us of the GPU's time, 7.8 of the host's for the call.
 #include <algorithm>
 
 #include "common.hpp"
@@ -86,8 +87,8 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormRows a, int32_t n, float
 template <int MODE>
 hipError_t launch_norm_mode(const NormRows &a, int32_t n, float eps, int32_t bias, hipStream_t s) {
   // 256 threads of 4 values and up to kNormKeep passes, then up to 1024 threads: several blocks a compute unit, so that some load
-  // while others store (2048 rows of 4096 values: 21.7 us, in one pass of 1024 threads 25.9; of 2048 values 13.4, in one of 512
-  // 14.7; a single row 8.2 us either way).  By the row alone, so that a token's sums run in one order however many tokens there are
+  // while others store (calls back to back, 2048 rows of 4096 values: 21.7 us, in one pass of 1024 threads 25.9; of 2048 values 13.4,
+  // in one of 512 14.7; a single row 8.2 us either way).  By the row alone, so that a token's sums run in one order however many tokens there are
   const int32_t lanes = (n + 3) / 4, passes = std::max((lanes + 1023) / 1024, std::min((lanes + 255) / 256, kNormKeep));
   const int32_t threads = ((lanes + passes - 1) / passes + 63) / 64 * 64;
   const uint32_t wide = a.count < 65536 ? (uint32_t)a.count : 65536u;

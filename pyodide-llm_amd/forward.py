@@ -81,8 +81,9 @@ class Forward:
 
     def step(self, x, starts, lengths, table, longest=0):
         """x: the new tokens' embeddings (float32, on the device), which become the residual stream; starts, lengths and
-        table: hq_batch's, int32 on the device, lengths with the new tokens among them.  Returns the final norm of every new
-        token's row (a buffer of this object's)."""
+        table: hq_batch's, int32 on the device, lengths with the new tokens among them; longest: the most new tokens that a
+        sequence has (0: not known, which makes a step of single tokens slower).  Returns the final norm of every new token's row
+        (a buffer of this object's)."""
         torch, lib, ck, s = self.torch, self.lib, self.ck, self.ck.shape
         count, sequences = x.shape[0], lengths.shape[0]
         if not (x.dim() == 2 and 0 < count <= self.tokens and 0 < sequences <= self.sequences and x.shape[1] == s.dim
