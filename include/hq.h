@@ -356,6 +356,83 @@ int32_t hq_attention_ex(void *out, const void *q, int32_t heads, int32_t out_str
                         const hq_cache *cache, const hq_batch *batch, float scale, int32_t window, float cap, void *work,
                         int64_t work_bytes, void *stream);
 
+/* ---- a serving step around its layers (no counterpart among the reference's kernels) ------------------------------ */
+
+/* Embeddings of token ids: row t of out (dim float32, out_stride bytes apart) = row ids[t] of a packed table of `vocab` rows of
+ * `dim` weights, each widened as float32(value x its group's scale) and multiplied by `scale` (one more rounding); an id
+ * outside 0 .. vocab - 1 gives zeros.  ids: `count` int32 in device memory.  packing: HQ_PACK_* with values and scales as the
+ * loader keeps them (hq_outlier_columns_ex's), or HQ_PACK_BLOCKS + a block type (a row is what sb_row gives; values the blocks,
+ * scales sb_tables's area).  values 16-byte aligned (int6 8, blocks 2), scales 4 (ternary and binary 2, blocks 16), out and its
+ * stride 16, a stride at least 4 dim. */
+enum { HQ_PACK_BLOCKS = 256 };
+int32_t hq_embed_ex(void *out, const void *ids, const void *values, const void *scales, int32_t packing, int32_t vocab,
+                    int32_t dim, float scale, int32_t count, int32_t out_stride, void *stream);
+
+/* The pages that nobody uses, as a stack in device memory: `free` holds up to `pages` page numbers (int32), of which the word at
+ * `count` says how many there are (the last is on top); a call writes how many are left at `left` (which may be `count`) and, where
+ * `missing` is not NULL, how many pages it lacked.  A page is `page` positions (16, 32, 64, 128 or 256).  All 4-byte aligned. */
+typedef struct hq_pool {
+  void *free;
+  const void *count;
+  void *left, *missing;
+  int32_t pages, page;
+} hq_pool;
+/* What a step's new tokens make of a batch, on the device: sequence s has held[s] positions and gets fresh[s] new tokens
+ * (negative numbers count as 0; what would pass the batch's `tokens` rows is left out, from the last sequences).  Written:
+ *   batch->starts    sums of the new tokens before each sequence, and after the last
+ *   batch->lengths   held + new (may be held)
+ *   batch->table     the pages of positions that begin on a new page, from the top of the stack, in order of sequences and
+ *                    positions; where the stack is empty, -1, and past the table's width nothing.  Other entries stay as they are
+ * and for each of the `tokens` rows, each where it is not NULL: sequence and position (int32) and slot (int64: its page times
+ * `page` plus its place there, -1 without a page), all -1 for rows that no sequence has.  4-byte aligned, slot 8.
+ * Nothing else that is written may overlap what is read. */
+int32_t hq_batch_plan_ex(const hq_batch *batch, const hq_pool *pool, const void *held, const void *fresh, void *sequence,
+                         void *position, void *slot, void *stream);
+/* Pages given back: of the table's row s (width entries) those from from[s] up to to[s] (int32; NULL: 0 and the width) that are
+ * pages go onto the stack, in order of rows and entries, and become -1.  Where the stack is full (a page was given back twice:
+ * two entries that are the same page are both put on it) the rest is dropped.  pool->missing is not touched. */
+int32_t hq_pages_give_ex(const hq_pool *pool, void *table, int32_t sequences, int32_t width, const void *from, const void *to,
+                         void *stream);
+
+/* Low-rank adapters beside a projection: a[adapters][rank][n] and b[adapters][rows][rank] (float16 or bfloat16), and for each
+ * token t of sequence s with adapter w = which[s]
+ *   y[t] = from[t] + scales[w] b[w] (a[w] x[t])        (no adapter: y[t] = from[t])
+ * (float32 rows, from_stride and y_stride bytes apart; from NULL: zeros; from may be y). */
+typedef struct hq_adapter {
+  const void *a, *b, *from;
+  void *y;
+  int32_t rows, from_stride, y_stride;
+} hq_adapter;
+/* `count` projections (up to 8) of one input x (tokens x n float32, x_stride bytes apart) with the adapters of the batch's
+ * sequences, after the products themselves: which (int32, device) is a sequence's adapter, none where it is outside 0 .. adapters
+ * - 1; scales (float32, device; NULL: 1) an adapter's scale, the same for all projections; form HQ_ADAPTER_*.  Of the batch only
+ * starts, sequences, tokens and longest are read.  Rows that no sequence has are left alone.  Products and sums in float32
+ * (a x to 2^-22 of its terms), the sum of a row in an order of this library's that may depend on `longest`.  rank a multiple of 8 up to
+ * 256, n a multiple of 32; a, b, x, from, y and their strides 16-byte aligned.  work: hq_adapters_work_bytes bytes (-1: bad
+ * arguments), 256-byte aligned, of any content; calls that share it on one stream follow each other, on two they race. */
+enum { HQ_ADAPTER_F16 = 1, HQ_ADAPTER_BF16 = 2 };
+int64_t hq_adapters_work_bytes(int32_t count, int32_t rank, int32_t tokens);
+int32_t hq_adapters_ex(const hq_adapter *targets, int32_t count, const void *x, int32_t x_stride, int32_t n, int32_t rank,
+                       int32_t adapters, int32_t form, const void *scales, const void *which, const hq_batch *batch, void *work,
+                       int64_t work_bytes, void *stream);
+
+/* The next token of each of `rows` rows of logits (vocab float32, stride bytes apart), drawn with the number u[row] of [0, 1):
+ *   w_i = e^((l_i - max l) / temperature), in 64 bits          (temperature not above 0: the largest alone, the lowest index of these)
+ *   kept: of all tokens by falling l, then rising index, the first top_k (0 or less: all);
+ *         of these each before which less than top_p of their sum of w lies, the first in any case (1 or more: all);
+ *         of these those with w >= min_p (0 or less: all; more than 1 counts as 1)
+ *   the first i, by rising index, whose kept w up to and with it are more than u times the sum of all kept
+ * into tokens (int32), and w_i over that sum into chance (float32, may be NULL).  -infinity and NaN logits are never drawn (a row
+ * of nothing else: token -1, chance 0); +infinity ones have all the weight.  temperature, top_p, min_p and u (float32) and top_k
+ * (int32) are a number a row in device memory; each but u may be NULL (temperature 1, the others off), and NaN is off as well.  u below 0 or NaN counts as
+ * 0, and where u is 1 or more the last kept token is drawn.  Sums behind top_p are of w in steps of 2^-42 or finer, in any order; the last sum
+ * is in 64 bits by rising index: the same numbers always draw the same token.  logits and stride 4-byte aligned; vocab at most
+ * 2^20, rows too.  work: hq_sample_work_bytes bytes (-1: bad arguments), 256-byte aligned, of any content, as hq_attention_ex's. */
+int64_t hq_sample_work_bytes(int32_t rows, int32_t vocab);
+int32_t hq_sample_ex(void *tokens, void *chance, const void *logits, const void *u, const void *temperature, const void *top_k,
+                     const void *top_p, const void *min_p, int32_t rows, int32_t vocab, int32_t stride, void *work,
+                     int64_t work_bytes, void *stream);
+
 /* The ceilings the kernels are measured against (no counterpart on this path: the reference's CPU ceiling loops,
  * kernels/ceilings.ts:12-25 and ceilings_relaxed.ts:34-52, are its model).  hq_ceiling_read reads every byte of
  * [p, p + bytes) once (bytes a multiple of 16): time it for the achievable HBM read bandwidth of a buffer past the

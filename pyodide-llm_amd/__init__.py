@@ -18,6 +18,7 @@ raises.
 import ctypes
 import os
 
+from . import adapters  # (a projection's low-rank adapters)
 from . import cache  # (the paged cache's and a batch's descriptions)
 from . import jobs  # noqa: F401  (the jobs.ts mirror)
 
@@ -25,8 +26,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIBRARY = os.path.join(HERE, "libhq.so")
 
 HQ_OK, HQ_ERR_ARGUMENT, HQ_ERR_ALIGNMENT, HQ_ERR_NULL, HQ_ERR_HIP, HQ_ERR_KIND, HQ_ERR_DEVICE = range(7)
-# the packings of hq_outlier_columns_ex (include/hq.h)
+# the packings of hq_outlier_columns_ex and hq_embed_ex (include/hq.h); hq_embed_ex takes HQ_PACK_BLOCKS + a block type as well
 HQ_PACK = {"int8": 0, "int6": 1, "ternary": 2, "binary": 3}
+HQ_PACK_BLOCKS = 256
 
 
 class HQError(RuntimeError):
@@ -36,7 +38,7 @@ class HQError(RuntimeError):
 
 
 p, i32, f32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_float
-pcache, pbatch = ctypes.POINTER(cache.Cache), ctypes.POINTER(cache.Batch)
+pcache, pbatch, ppool = (ctypes.POINTER(kind) for kind in (cache.Cache, cache.Batch, cache.Pool))
 
 # the reference's kernels, by name: src/runtime/jobs.ts:101-140 (Arguments), src/python/engine/kernels.py:42-51
 REFERENCE_SIGNATURES = {
@@ -119,6 +121,14 @@ OWN_SIGNATURES = {
     "hq_cache_read_ex": ([pcache, pbatch, p, p, i32, i32, p], i32),
     "hq_attention_work_bytes": ([pcache, pbatch, i32], ctypes.c_int64),
     "hq_attention_ex": ([p, p, i32, i32, i32, pcache, pbatch, f32, i32, f32, p, ctypes.c_int64, p], i32),
+    "hq_embed_ex": ([p, p, p, p, i32, i32, i32, f32, i32, i32, p], i32),
+    "hq_batch_plan_ex": ([pbatch, ppool, p, p, p, p, p, p], i32),
+    "hq_pages_give_ex": ([ppool, p, i32, i32, p, p, p], i32),
+    "hq_adapters_work_bytes": ([i32, i32, i32], ctypes.c_int64),
+    "hq_adapters_ex": ([ctypes.POINTER(adapters.Target), i32, p, i32, i32, i32, i32, i32, p, p, pbatch, p, ctypes.c_int64, p],
+                       i32),
+    "hq_sample_work_bytes": ([i32, i32], ctypes.c_int64),
+    "hq_sample_ex": ([p, p, p, p, p, p, p, p, i32, i32, i32, p, ctypes.c_int64, p], i32),
     "hq_ceiling_read": ([p, ctypes.c_int64, p, p], i32),
     "hq_ceiling_mfma": ([i32, i32, p, p], i32),
     "hq_ceiling_epilogue": ([i32, i32, i32, p, p], i32),

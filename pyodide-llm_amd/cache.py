@@ -1,5 +1,6 @@
 """What a layer's operators between its products take: the descriptions of a paged key/value cache and of a batch of new
-tokens (hq_cache and hq_batch of include/hq.h), and the forms hq_norm_ready_ex readies activations in.
+tokens (hq_cache and hq_batch of include/hq.h), of the pages that nobody uses (hq_pool), and the forms hq_norm_ready_ex readies
+activations in.
 
 A cache's arrays and a batch's are device memory of the caller's; the descriptions hold their addresses, and are read
 when a call is made (ctypes passes them by reference: `lib.hq_cache_write_ex(cache, batch, ...)`).
@@ -27,6 +28,12 @@ class Batch(ctypes.Structure):
     _fields_ = [("starts", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("table", ctypes.c_void_p),
                 ("sequences", ctypes.c_int32), ("tokens", ctypes.c_int32), ("longest", ctypes.c_int32),
                 ("width", ctypes.c_int32)]
+
+
+class Pool(ctypes.Structure):
+    """free, count, left, missing (device addresses of int32), pages, page"""
+    _fields_ = [("free", ctypes.c_void_p), ("count", ctypes.c_void_p), ("left", ctypes.c_void_p), ("missing", ctypes.c_void_p),
+                ("pages", ctypes.c_int32), ("page", ctypes.c_int32)]
 
 
 def shapes(form, pages, page, heads, dim):

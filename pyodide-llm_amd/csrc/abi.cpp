@@ -415,28 +415,62 @@ int32_t group_of(int32_t packing, int32_t dim) {
   while (size > 1 && dim % size) size >>= 1;
   return size;
 }
+// a batch's sizes (table: whether its table is used), with pages of 1 << shift positions
+int32_t batch_sizes_of(const char *who, const hq_batch *batch, int32_t shift, bool table = true) {
+  if (batch->sequences < 0 || batch->tokens < 0 || batch->longest < 0 || batch->width < 0)
+    return fail(HQ_ERR_ARGUMENT, "%s: sequences = %d, tokens = %d, longest = %d, width = %d", who, batch->sequences,
+                batch->tokens, batch->longest, batch->width);
+  if (table && ((int64_t)batch->width << shift) > 1 << 30)
+    return fail(HQ_ERR_ARGUMENT, "%s: a table of %d pages of %d positions", who, batch->width, 1 << shift);
+  if (batch->tokens > (1 << 24)) return fail(HQ_ERR_ARGUMENT, "%s: tokens = %d", who, batch->tokens);
+  // (a launch of two blocks a sequence stays below 2^32 threads)
+  if (batch->sequences > (1 << 22)) return fail(HQ_ERR_ARGUMENT, "%s: sequences = %d", who, batch->sequences);
+  return HQ_OK;
+}
+// the positions of a page as a shift (-1: no page size)
+int32_t page_shift_of(int32_t page) {
+  int32_t shift = 4;
+  while (shift < 8 && (1 << shift) != page) shift++;
+  return (1 << shift) == page ? shift : -1;
+}
+// a pool, checked
+int32_t pool_of(const char *who, const hq_pool *pool, hq::Pool &p) {
+  if (!pool) return fail(HQ_ERR_NULL, "%s: pool NULL", who);
+  const int32_t shift = page_shift_of(pool->page);
+  if (shift < 0) return fail(HQ_ERR_ARGUMENT, "%s: page = %d is none of 16, 32, 64, 128, 256", who, pool->page);
+  if (pool->pages < 0) return fail(HQ_ERR_ARGUMENT, "%s: pages = %d", who, pool->pages);
+  if ((pool->pages && !pool->free) || !pool->count || !pool->left)
+    return fail(HQ_ERR_NULL, "%s: the pool's free, count or left NULL", who);
+  if (!aligned(pool->free, 4) || !aligned(pool->count, 4) || !aligned(pool->left, 4) || !aligned(pool->missing, 4))
+    return fail(HQ_ERR_ALIGNMENT, "%s: the pool's free, count, left or missing not 4-byte aligned", who);
+  p = hq::Pool{(int32_t *)pool->free, (const int32_t *)pool->count, (int32_t *)pool->left, (int32_t *)pool->missing, pool->pages,
+               shift};
+  return HQ_OK;
+}
+int32_t adapters_sizes_of(const char *who, int32_t count, int32_t rank, int32_t tokens) {
+  if (count < 0 || count > hq::kMaxTargets) return fail(HQ_ERR_ARGUMENT, "%s: count = %d projections (at most %d)", who, count, hq::kMaxTargets);
+  if (rank <= 0 || rank % 8 || rank > 256) return fail(HQ_ERR_ARGUMENT, "%s: rank = %d is not a multiple of 8 up to 256", who, rank);
+  if (tokens < 0 || tokens > (1 << 24)) return fail(HQ_ERR_ARGUMENT, "%s: tokens = %d", who, tokens);
+  return HQ_OK;
+}
+int32_t sample_sizes_of(const char *who, int32_t rows, int32_t vocab) {
+  if (rows < 0 || rows > (1 << 20)) return fail(HQ_ERR_ARGUMENT, "%s: rows = %d (at most 2^20)", who, rows);
+  if (vocab <= 0 || vocab > hq::kMostVocab) return fail(HQ_ERR_ARGUMENT, "%s: vocab = %d is not 1 to 2^20", who, vocab);
+  return HQ_OK;
+}
 // the cache and the batch of a call, checked (memory: whether their device pointers are)
 int32_t paged_of(const char *who, const hq_cache *cache, const hq_batch *batch, hq::Cache &c, hq::Batch &b,
                  bool memory = true) {
   if (!cache || !batch) return fail(HQ_ERR_NULL, "%s: cache or batch NULL", who);
   if (cache->form != HQ_CACHE_INT8 && cache->form != HQ_CACHE_F16)
     return fail(HQ_ERR_ARGUMENT, "%s: form %d is neither int8 nor float16", who, cache->form);
-  int32_t shift = 4;
-  while (shift < 8 && (1 << shift) != cache->page) shift++;
-  if ((1 << shift) != cache->page)
-    return fail(HQ_ERR_ARGUMENT, "%s: page = %d is none of 16, 32, 64, 128, 256", who, cache->page);
+  const int32_t shift = page_shift_of(cache->page);
+  if (shift < 0) return fail(HQ_ERR_ARGUMENT, "%s: page = %d is none of 16, 32, 64, 128, 256", who, cache->page);
   if (cache->dim <= 0 || cache->dim % 16 || cache->dim > 256)
     return fail(HQ_ERR_ARGUMENT, "%s: dim = %d is not a multiple of 16 up to 256", who, cache->dim);
   if (cache->heads <= 0 || cache->heads > 1024) return fail(HQ_ERR_ARGUMENT, "%s: heads = %d", who, cache->heads);
   if (cache->pages < 0) return fail(HQ_ERR_ARGUMENT, "%s: pages = %d", who, cache->pages);
-  if (batch->sequences < 0 || batch->tokens < 0 || batch->longest < 0 || batch->width < 0)
-    return fail(HQ_ERR_ARGUMENT, "%s: sequences = %d, tokens = %d, longest = %d, width = %d", who, batch->sequences,
-                batch->tokens, batch->longest, batch->width);
-  if (((int64_t)batch->width << shift) > 1 << 30)
-    return fail(HQ_ERR_ARGUMENT, "%s: a table of %d pages of %d positions", who, batch->width, cache->page);
-  if (batch->tokens > (1 << 24)) return fail(HQ_ERR_ARGUMENT, "%s: tokens = %d", who, batch->tokens);
-  // (a launch of two blocks a sequence stays below 2^32 threads)
-  if (batch->sequences > (1 << 22)) return fail(HQ_ERR_ARGUMENT, "%s: sequences = %d", who, batch->sequences);
+  if (int32_t st = batch_sizes_of(who, batch, shift)) return st;
   c = hq::Cache{(char *)cache->k, (char *)cache->v, (float *)cache->ks, (float *)cache->vs, cache->form == HQ_CACHE_F16,
                 cache->pages, shift, cache->heads, cache->dim};
   const int32_t longest = batch->longest && batch->longest < batch->tokens ? batch->longest : batch->tokens;
@@ -879,6 +913,164 @@ int32_t hq_attention_ex(void *out, const void *q, int32_t heads, int32_t out_str
   if (int32_t st = ensure_device()) return st;
   const hq::Attention a{(char *)out, (const char *)q, (char *)work, out_stride, q_stride, heads, window, scale, cap};
   return hip_status(hq::launch_attention(a, c, b, stream_of(stream)), "attention");
+}
+
+// ---- a serving step around its layers -----------------------------------------------------------------------------
+int32_t hq_embed_ex(void *out, const void *ids, const void *values, const void *scales, int32_t packing, int32_t vocab,
+                    int32_t dim, float scale, int32_t count, int32_t out_stride, void *stream) {
+  g_error = HQ_OK;
+  const int32_t type = packing - HQ_PACK_BLOCKS;
+  const bool blocks = hq::sb_block_bytes(type) > 0;
+  if (!blocks && (packing < HQ_PACK_INT8 || packing > HQ_PACK_BINARY))
+    return fail(HQ_ERR_ARGUMENT, "embed: packing %d is none of int8, int6, ternary, binary, nor a block type", packing);
+  if (vocab <= 0 || dim <= 0) return fail(HQ_ERR_ARGUMENT, "embed: vocab = %d, dim = %d", vocab, dim);
+  const int32_t group = blocks ? 256 : group_of(packing, dim);
+  if (dim % group) return fail(HQ_ERR_ARGUMENT, "embed: dim = %d is not whole groups of %d", dim, group);
+  if (std::isnan(scale) || std::isinf(scale)) return fail(HQ_ERR_ARGUMENT, "embed: scale = %g", (double)scale);
+  if (count < 0) return fail(HQ_ERR_ARGUMENT, "embed: count = %d", count);
+  if (count == 0) return HQ_OK;
+  if (!out || !ids || !values || !scales) return fail(HQ_ERR_NULL, "embed: a NULL pointer");
+  const uintptr_t va = blocks ? 2 : packing == HQ_PACK_INT6 ? 8 : 16;
+  const uintptr_t sa = blocks ? 16 : packing == HQ_PACK_TERNARY || packing == HQ_PACK_BINARY ? 2 : 4;
+  if (!aligned(values, va) || !aligned(scales, sa))
+    return fail(HQ_ERR_ALIGNMENT, "embed: values not %d-byte aligned or scales not %d-byte aligned", (int)va, (int)sa);
+  if (!aligned(out, 16) || !aligned(ids, 4)) return fail(HQ_ERR_ALIGNMENT, "embed: out not 16- or ids not 4-byte aligned");
+  if (count > 1) {
+    if (out_stride < 0 || out_stride % 16)
+      return fail(HQ_ERR_ALIGNMENT, "embed: out_stride = %d is not a multiple of 16", out_stride);
+    if (out_stride < 4 * (int64_t)dim)
+      return fail(HQ_ERR_ARGUMENT, "embed: out_stride = %d, a row takes %lld", out_stride, 4 * (long long)dim);
+  }
+  if (int32_t st = ensure_device()) return st;
+  const hq::Embed e{(char *)out, (const int32_t *)ids, (const char *)values, (const char *)scales, out_stride, vocab, dim, count,
+                    scale};
+  return hip_status(blocks ? hq::launch_embed_blocks(type, e, stream_of(stream))
+                           : hq::launch_embed(packing, e, group, stream_of(stream)), "embed");
+}
+
+int32_t hq_batch_plan_ex(const hq_batch *batch, const hq_pool *pool, const void *held, const void *fresh, void *sequence,
+                         void *position, void *slot, void *stream) {
+  g_error = HQ_OK;
+  if (!batch) return fail(HQ_ERR_NULL, "batch_plan: batch NULL");
+  hq::Pool p;
+  if (int32_t st = pool_of("batch_plan", pool, p)) return st;
+  if (int32_t st = batch_sizes_of("batch_plan", batch, p.shift)) return st;
+  if (!batch->starts) return fail(HQ_ERR_NULL, "batch_plan: starts NULL");
+  if (batch->sequences && (!batch->lengths || !held || !fresh || (batch->width && !batch->table)))
+    return fail(HQ_ERR_NULL, "batch_plan: lengths, table, held or fresh NULL");
+  const void *words[] = {batch->starts, batch->lengths, batch->table, held, fresh, sequence, position};
+  for (const void *w : words)
+    if (!aligned(w, 4)) return fail(HQ_ERR_ALIGNMENT, "batch_plan: an array of int32 is not 4-byte aligned");
+  if (!aligned(slot, 8)) return fail(HQ_ERR_ALIGNMENT, "batch_plan: slot not 8-byte aligned");
+  if (int32_t st = ensure_device()) return st;
+  const hq::Plan a{(const int32_t *)held, (const int32_t *)fresh, (int32_t *)batch->starts, (int32_t *)batch->lengths,
+                   (int32_t *)batch->table, (int32_t *)sequence, (int32_t *)position, (int64_t *)slot, batch->sequences,
+                   batch->tokens, batch->width};
+  return hip_status(hq::launch_plan(a, p, stream_of(stream)), "batch_plan");
+}
+
+int32_t hq_pages_give_ex(const hq_pool *pool, void *table, int32_t sequences, int32_t width, const void *from, const void *to,
+                         void *stream) {
+  g_error = HQ_OK;
+  hq::Pool p;
+  if (int32_t st = pool_of("pages_give", pool, p)) return st;
+  const hq_batch sizes{nullptr, nullptr, table, sequences, 0, 0, width};
+  if (int32_t st = batch_sizes_of("pages_give", &sizes, p.shift)) return st;
+  if (sequences && width && !table) return fail(HQ_ERR_NULL, "pages_give: table NULL");
+  if (!aligned(table, 4) || !aligned(from, 4) || !aligned(to, 4))
+    return fail(HQ_ERR_ALIGNMENT, "pages_give: table, from or to not 4-byte aligned");
+  if (int32_t st = ensure_device()) return st;
+  return hip_status(hq::launch_give(p, (int32_t *)table, sequences, width, (const int32_t *)from, (const int32_t *)to,
+                                    stream_of(stream)), "pages_give");
+}
+
+int64_t hq_adapters_work_bytes(int32_t count, int32_t rank, int32_t tokens) {
+  g_error = HQ_OK;
+  if (adapters_sizes_of("adapters_work_bytes", count, rank, tokens)) return -1;
+  return hq::adapters_work_bytes(count, rank, tokens);
+}
+
+int32_t hq_adapters_ex(const hq_adapter *targets, int32_t count, const void *x, int32_t x_stride, int32_t n, int32_t rank,
+                       int32_t adapters, int32_t form, const void *scales, const void *which, const hq_batch *batch, void *work,
+                       int64_t work_bytes, void *stream) {
+  g_error = HQ_OK;
+  if (!batch) return fail(HQ_ERR_NULL, "adapters: batch NULL");
+  if (int32_t st = batch_sizes_of("adapters", batch, 4, false)) return st;
+  if (int32_t st = adapters_sizes_of("adapters", count, rank, batch->tokens)) return st;
+  if (n <= 0 || n % 32) return fail(HQ_ERR_ARGUMENT, "adapters: n = %d is not a positive multiple of 32", n);
+  if (adapters < 0) return fail(HQ_ERR_ARGUMENT, "adapters: adapters = %d", adapters);
+  if (form != HQ_ADAPTER_F16 && form != HQ_ADAPTER_BF16)
+    return fail(HQ_ERR_ARGUMENT, "adapters: form %d is neither float16 nor bfloat16", form);
+  if (count && !targets) return fail(HQ_ERR_NULL, "adapters: targets NULL");
+  hq::Adapters a{};
+  for (int32_t i = 0; i < count; i++)
+    if (targets[i].rows < 0) return fail(HQ_ERR_ARGUMENT, "adapters: target %d has %d rows", i, targets[i].rows);
+  if (count == 0 || batch->tokens == 0 || batch->sequences == 0) return HQ_OK;
+  if (!batch->starts || !which || (adapters && !x)) return fail(HQ_ERR_NULL, "adapters: starts, which or x NULL");
+  if (!aligned(batch->starts, 4) || !aligned(which, 4) || !aligned(scales, 4))
+    return fail(HQ_ERR_ALIGNMENT, "adapters: starts, which or scales not 4-byte aligned");
+  if (!aligned(x, 16) || (batch->tokens > 1 && (x_stride < 0 || x_stride % 16)))
+    return fail(HQ_ERR_ALIGNMENT, "adapters: x or x_stride not 16-byte aligned");
+  if (batch->tokens > 1 && x_stride < 4 * (int64_t)n)
+    return fail(HQ_ERR_ARGUMENT, "adapters: x_stride = %d, a token's row takes %lld", x_stride, 4 * (long long)n);
+  for (int32_t i = 0; i < count; i++) {
+    const hq_adapter &t = targets[i];
+    if (t.rows == 0) continue;
+    if (!t.y || (adapters && (!t.a || !t.b))) return fail(HQ_ERR_NULL, "adapters: target %d's a, b or y NULL", i);
+    if (!aligned(t.a, 16) || !aligned(t.b, 16) || !aligned(t.from, 16) || !aligned(t.y, 16))
+      return fail(HQ_ERR_ALIGNMENT, "adapters: target %d's a, b, from or y not 16-byte aligned", i);
+    if (batch->tokens > 1) {
+      const int64_t row = 4 * (int64_t)t.rows;
+      if (t.y_stride < 0 || t.y_stride % 16 || (t.from && (t.from_stride < 0 || t.from_stride % 16)))
+        return fail(HQ_ERR_ALIGNMENT, "adapters: target %d's stride is not a multiple of 16", i);
+      if (t.y_stride < row || (t.from && t.from_stride < row))
+        return fail(HQ_ERR_ARGUMENT, "adapters: target %d's strides %d and %d, a token's row takes %lld", i, t.from_stride,
+                    t.y_stride, (long long)row);
+    }
+    a.target[a.count++] = hq::Target{(const char *)t.a, (const char *)t.b, (const char *)t.from, (char *)t.y, t.rows,
+                                     t.from_stride, t.y_stride};
+  }
+  const int64_t need = hq::adapters_work_bytes(count, rank, batch->tokens);
+  if (work_bytes < need)
+    return fail(HQ_ERR_ARGUMENT, "adapters: a workspace of %lld bytes, %lld are needed", (long long)work_bytes, (long long)need);
+  if (need && !work) return fail(HQ_ERR_NULL, "adapters: work NULL");
+  if (!aligned(work, 256)) return fail(HQ_ERR_ALIGNMENT, "adapters: work not 256-byte aligned");
+  if (int32_t st = ensure_device()) return st;
+  a.x = (const char *)x, a.scales = (const float *)scales, a.which = (const int32_t *)which, a.work = (float *)work;
+  a.x_stride = x_stride, a.n = n, a.rank = rank, a.adapters = adapters, a.bf16 = form == HQ_ADAPTER_BF16;
+  const int32_t longest = batch->longest && batch->longest < batch->tokens ? batch->longest : batch->tokens;
+  const hq::Batch b{(const int32_t *)batch->starts, nullptr, nullptr, batch->sequences, batch->tokens, longest, 0};
+  return hip_status(hq::launch_adapters(a, b, stream_of(stream)), "adapters");
+}
+
+int64_t hq_sample_work_bytes(int32_t rows, int32_t vocab) {
+  g_error = HQ_OK;
+  if (sample_sizes_of("sample_work_bytes", rows, vocab)) return -1;
+  return hq::sample_work_bytes(rows, vocab);
+}
+
+int32_t hq_sample_ex(void *tokens, void *chance, const void *logits, const void *u, const void *temperature, const void *top_k,
+                     const void *top_p, const void *min_p, int32_t rows, int32_t vocab, int32_t stride, void *work,
+                     int64_t work_bytes, void *stream) {
+  g_error = HQ_OK;
+  if (int32_t st = sample_sizes_of("sample", rows, vocab)) return st;
+  if (rows == 0) return HQ_OK;
+  if (!tokens || !logits || !u) return fail(HQ_ERR_NULL, "sample: tokens, logits or u NULL");
+  const void *words[] = {tokens, chance, logits, u, temperature, top_k, top_p, min_p};
+  for (const void *w : words)
+    if (!aligned(w, 4)) return fail(HQ_ERR_ALIGNMENT, "sample: an array is not 4-byte aligned");
+  if (rows > 1 && (stride < 0 || stride % 4)) return fail(HQ_ERR_ALIGNMENT, "sample: stride = %d is not a multiple of 4", stride);
+  if (rows > 1 && stride < 4 * (int64_t)vocab)
+    return fail(HQ_ERR_ARGUMENT, "sample: stride = %d, a row takes %lld", stride, 4 * (long long)vocab);
+  const int64_t need = hq::sample_work_bytes(rows, vocab);
+  if (work_bytes < need)
+    return fail(HQ_ERR_ARGUMENT, "sample: a workspace of %lld bytes, %lld are needed", (long long)work_bytes, (long long)need);
+  if (need && !work) return fail(HQ_ERR_NULL, "sample: work NULL");
+  if (!aligned(work, 256)) return fail(HQ_ERR_ALIGNMENT, "sample: work not 256-byte aligned");
+  if (int32_t st = ensure_device()) return st;
+  const hq::Sample a{(int32_t *)tokens, (float *)chance, (const char *)logits, (const float *)u, (const float *)temperature,
+                     (const float *)top_p, (const float *)min_p, (const int32_t *)top_k, (char *)work, stride, rows, vocab};
+  return hip_status(hq::launch_sample(a, stream_of(stream)), "sample");
 }
 
 // ---- a phase of jobs in the reference's table form ------------------------------------------------------------

@@ -1039,14 +1039,13 @@ hipError_t launch_tile_type(const Job &j, hipStream_t s) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// sb_row: a row as float32 (row.ts), a chunk of 16 weights a thread
+// sb_row: a row as float32 (row.ts), a chunk of 16 weights a thread; embeddings: a row of a table each
 // ---------------------------------------------------------------------------------------------------------------
-template <int TY>
-__global__ __launch_bounds__(256) void sb_row_kernel(float *out, const char *w, const uint8_t *tab, int32_t n) {
+// chunk i of the row at w (block i / 16, h = i % 16) as float32, times `times`, to its 16 values at `to`
+template <int TY, bool TIMES>
+HQ_DEV void row_chunk(float *to, const char *w, const uint8_t *tab, int32_t i, float times) {
   constexpr int BYTES = sb_block_bytes(TY);
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;  // chunk: block i / 16, h = i % 16
-  if (i >= (int64_t)(n >> 4)) return;
-  const int b = (int)(i >> 4), h = (int)(i & 15);
+  const int b = i >> 4, h = i & 15;
   BlockBytes<BYTES> B;
   B.load(w + (int64_t)b * BYTES);
   uint32_t iq4[4] = {0u, 0u, 0u, 0u};
@@ -1065,7 +1064,6 @@ __global__ __launch_bounds__(256) void sb_row_kernel(float *out, const char *w, 
   const float scale = (TY == IQ2_XXS || TY == IQ2_XS || TY == IQ2_S) ? fmul(fmul(d, fadd(0.5f, s)), 0.25f)
                     : TY == IQ3_XXS ? fmul(fmul(d, fadd(0.5f, s)), 0.5f) : fmul(d, (float)c.S);
   const float least = has_minimums<TY>() ? fmul(fm, (float)c.M) : 0.0f;
-  float *to = out + 16 * i;
 #pragma unroll
   for (int j = 0; j < 16; j++) {
     const int32_t byte = (int32_t)(int8_t)((c.mag[j >> 2] >> (8 * (j & 3))) & 0xff);
@@ -1083,7 +1081,30 @@ __global__ __launch_bounds__(256) void sb_row_kernel(float *out, const char *w, 
     }
     float x = fmul(scale, v);
     if (has_minimums<TY>()) x = fsub(x, least);
-    to[j] = x;
+    to[j] = TIMES ? fmul(x, times) : x;
+  }
+}
+
+template <int TY>
+__global__ __launch_bounds__(256) void sb_row_kernel(float *out, const char *w, const uint8_t *tab, int32_t n) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (int64_t)(n >> 4)) return;
+  row_chunk<TY, false>(out + 16 * i, w, tab, (int32_t)i, 1.0f);
+}
+
+template <int TY>
+__global__ __launch_bounds__(256) void embed_blocks_kernel(Embed e) {
+  const int32_t i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= (e.dim >> 4)) return;
+  for (int64_t t = blockIdx.y; t < e.count; t += gridDim.y) {
+    float *to = (float *)(e.out + t * e.out_stride) + 16 * i;
+    const int32_t id = e.ids[t];
+    if ((uint32_t)id < (uint32_t)e.vocab) {
+      row_chunk<TY, true>(to, e.values + (int64_t)id * (e.dim >> 8) * sb_block_bytes(TY), (const uint8_t *)e.scales, i, e.scale);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; j++) to[j] = 0.0f;
+    }
   }
 }
 
@@ -1219,6 +1240,28 @@ hipError_t launch_sb_tile(const Job &j, hipStream_t s) {
   case IQ1_S: return launch_tile_type<IQ1_S>(j, s);
   case IQ1_M: return launch_tile_type<IQ1_M>(j, s);
   case IQ4_XS: return launch_tile_type<IQ4_XS>(j, s);
+  default: return hipErrorInvalidValue;
+  }
+}
+
+hipError_t launch_embed_blocks(int32_t type, const Embed &e, hipStream_t s) {
+  if (e.count <= 0 || e.dim <= 0) return hipSuccess;
+  const dim3 grid((uint32_t)(((e.dim >> 4) + 255) / 256), (uint32_t)(e.count < 65535 ? e.count : 65535));
+  const auto run = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, e);
+    return hipGetLastError();
+  };
+  switch (type) {
+  case Q2_K: return run(embed_blocks_kernel<Q2_K>);
+  case Q4_K: return run(embed_blocks_kernel<Q4_K>);
+  case IQ2_XXS: return run(embed_blocks_kernel<IQ2_XXS>);
+  case IQ2_XS: return run(embed_blocks_kernel<IQ2_XS>);
+  case IQ2_S: return run(embed_blocks_kernel<IQ2_S>);
+  case IQ3_XXS: return run(embed_blocks_kernel<IQ3_XXS>);
+  case IQ3_S: return run(embed_blocks_kernel<IQ3_S>);
+  case IQ1_S: return run(embed_blocks_kernel<IQ1_S>);
+  case IQ1_M: return run(embed_blocks_kernel<IQ1_M>);
+  case IQ4_XS: return run(embed_blocks_kernel<IQ4_XS>);
   default: return hipErrorInvalidValue;
   }
 }

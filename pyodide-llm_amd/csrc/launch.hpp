@@ -172,6 +172,71 @@ struct Attention {
 int64_t attention_work_bytes(const Cache &c, const Batch &b, int32_t heads);
 hipError_t launch_attention(const Attention &a, const Cache &c, const Batch &b, hipStream_t s);
 
+// embeddings (embed.hip; blocks.hip for the block types): row t of out, out_stride bytes apart, is row ids[t] of the table
+struct Embed {
+  char *out;
+  const int32_t *ids;
+  const char *values, *scales;  // (block types: the blocks and sb_tables's area)
+  int64_t out_stride;
+  int32_t vocab, dim, count;
+  float scale;
+};
+hipError_t launch_embed(int32_t packing, const Embed &e, int32_t group, hipStream_t s);
+hipError_t launch_embed_blocks(int32_t type, const Embed &e, hipStream_t s);
+
+// a batch's plan and its pages (plan.hip): hq_pool and hq_batch checked; a page is 1 << shift positions
+struct Pool {
+  int32_t *free;
+  const int32_t *count;
+  int32_t *left, *missing;
+  int32_t pages, shift;
+};
+struct Plan {
+  const int32_t *held, *fresh;
+  int32_t *starts, *lengths, *table;
+  int32_t *sequence, *position;
+  int64_t *slot;
+  int32_t sequences, tokens, width;
+};
+hipError_t launch_plan(const Plan &a, const Pool &p, hipStream_t s);
+hipError_t launch_give(const Pool &p, int32_t *table, int32_t sequences, int32_t width, const int32_t *from, const int32_t *to,
+                       hipStream_t s);
+
+// low-rank adapters (adapters.hip)
+constexpr int kMaxTargets = 8;
+struct Target {
+  const char *a, *b, *from;
+  char *y;
+  int32_t rows;
+  int64_t from_stride, y_stride;
+};
+struct Adapters {
+  Target target[kMaxTargets];
+  const char *x;
+  const float *scales;
+  const int32_t *which;
+  float *work;
+  int64_t x_stride;
+  int32_t count, n, rank, adapters, bf16;
+};
+int64_t adapters_work_bytes(int32_t count, int32_t rank, int32_t tokens);
+hipError_t launch_adapters(const Adapters &a, const Batch &b, hipStream_t s);
+
+// sampling (sample.hip)
+struct Sample {
+  int32_t *tokens;
+  float *chance;
+  const char *logits;
+  const float *u, *temperature, *top_p, *min_p;
+  const int32_t *top_k;
+  char *work;
+  int64_t stride;
+  int32_t rows, vocab;
+};
+constexpr int32_t kMostVocab = 1 << 20;
+int64_t sample_work_bytes(int32_t rows, int32_t vocab);
+hipError_t launch_sample(const Sample &a, hipStream_t s);
+
 // the ceilings (ceilings.hip): every byte of [p, p + bytes) read once; `iterations` x 8 MFMAs a wave of `blocks`
 // blocks of 4 waves.  sink: 256 words that are almost never written
 hipError_t launch_ceiling_read(const char *p, int64_t bytes, uint32_t *sink, hipStream_t s);
