@@ -27,6 +27,7 @@ constexpr int kBatch = 8;                // steps whose loads are on their way t
 constexpr int kHeld = 32768, kSmall = 8192;  // the longest rows that a block holds in LDS (alone on its compute unit, beside others)
 constexpr int kHand = 128;               // logits that a wave of the first launch can hand on
 constexpr int kList = 7680;              // and what the second launch takes of a row (two blocks a compute unit)
+constexpr int kFew = 64;                 // keys that one wave finishes with
 constexpr uint32_t kLowest = 0x00800000u;  // the key of the lowest finite number
 
 HQ_DEV uint32_t key_of(float v) {
@@ -88,63 +89,113 @@ struct Settings {
   HQ_DEV bool whole_sum() const { return !top_k && (top_p < 1.0 || !(min_p > 0.0)); }  // the row's whole sum is needed
 };
 HQ_DEV Settings settings_of(const Sample &a, int64_t row) {
+  // (all of them loaded before the first is looked at: an array that is not there is u's)
+  const float u = a.u[row], temperature = (a.temperature ? a.temperature : a.u)[row];
+  const float top_p = (a.top_p ? a.top_p : a.u)[row], min_p = (a.min_p ? a.min_p : a.u)[row];
+  const int32_t top_k = (a.top_k ? a.top_k : (const int32_t *)a.u)[row];
   Settings o;
-  o.temperature = a.temperature ? a.temperature[row] : 1.0f;
-  o.top_k = a.top_k ? max(a.top_k[row], 0) : 0;
-  if (o.top_k >= a.vocab) o.top_k = 0;
-  o.top_p = a.top_p ? a.top_p[row] : 1.0f;
-  o.min_p = a.min_p ? a.min_p[row] : 0.0f;
-  o.min_p = o.min_p > 0.0 ? fmin(o.min_p, 1.0) : 0.0;
-  o.u = a.u[row];
-  if (!(o.u >= 0.0)) o.u = 0.0;
+  o.temperature = a.temperature ? temperature : 1.0f;
+  o.top_k = a.top_k && top_k > 0 && top_k < a.vocab ? top_k : 0;
+  o.top_p = a.top_p ? top_p : 1.0f;
+  o.min_p = a.min_p && min_p > 0.0f ? fminf(min_p, 1.0f) : 0.0f;
+  o.u = u >= 0.0f ? u : 0.0f;
   if (!(o.temperature > 0.0)) o.temperature = 1.0, o.top_k = 1;
   return o;
 }
 
+// ---- over a wave's lanes, by moves between registers ---------------------------------------------------------------
+template <int CTRL, int ROWS, typename T>
+HQ_DEV T moved(T v) {  // (0 for lanes that nothing comes to)
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int32_t, v), CTRL, ROWS, 0xf, true));
+  } else {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int32_t)(uint32_t)u, CTRL, ROWS, 0xf, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int32_t)(uint32_t)(u >> 32), CTRL, ROWS, 0xf, true);
+    return __builtin_bit_cast(T, (uint64_t)lo | (uint64_t)hi << 32);
+  }
+}
+// What lanes give each other is computed here, with all lanes, and not moved to where a few of them use it
+template <typename T>
+HQ_DEV T here(T v) {
+  if constexpr (sizeof(T) == 4) {
+    uint32_t u = __builtin_bit_cast(uint32_t, v);
+    asm volatile("" : "+v"(u));
+    return __builtin_bit_cast(T, u);
+  } else {
+    uint64_t u = __builtin_bit_cast(uint64_t, v);
+    asm volatile("" : "+v"(u));
+    return __builtin_bit_cast(T, u);
+  }
+}
+// the sum over the lanes up to and with this one, in rows of 16, then the rows before
+template <typename T>
+HQ_DEV T sum_row(T v) {
+  v += moved<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+  v += moved<0x112, 0xf>(v);
+  v += moved<0x114, 0xf>(v);
+  v += moved<0x118, 0xf>(v);
+  return here(v);
+}
+template <typename T>
+HQ_DEV T sum_up_to(T v) {
+  v = sum_row(v);
+  v += moved<0x142, 0xa>(v);  // row_bcast 15 into rows 1 and 3, row_bcast 31 into rows 2 and 3
+  v += moved<0x143, 0xc>(v);
+  return here(v);
+}
+// lane l's value (l the same in all lanes)
+template <typename T>
+HQ_DEV T from_lane(T v, int l) {
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int32_t, v), l));
+  } else {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int32_t)(uint32_t)u, l);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int32_t)(uint32_t)(u >> 32), l);
+    return __builtin_bit_cast(T, (uint64_t)lo | (uint64_t)hi << 32);
+  }
+}
+template <typename T>
+HQ_DEV T wave_sum(T v) { return from_lane(sum_up_to(v), 63); }
+HQ_DEV uint32_t wave_most(uint32_t v) {
+  v = max(v, moved<0x111, 0xf>(v));
+  v = max(v, moved<0x112, 0xf>(v));
+  v = max(v, moved<0x114, 0xf>(v));
+  v = max(v, moved<0x118, 0xf>(v));
+  v = max(v, moved<0x142, 0xa>(v));
+  v = max(v, moved<0x143, 0xc>(v));
+  return from_lane(here(v), 63);
+}
+
 // ---- sums over a block ----------------------------------------------------------------------------------------------
 // (every thread calls; `part`: kWaves doublewords of LDS that nothing else uses)
-template <typename T, typename Op>
-HQ_DEV T block_all(T v, T *part, Op op) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = op(v, (T)__shfl_xor(v, o, 64));
+template <typename T>
+HQ_DEV T block_sum(T v, T *part) {
+  v = wave_sum(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
   __syncthreads();
-  v = part[threadIdx.x & (kWaves - 1)];
-#pragma unroll
-  for (int o = kWaves / 2; o > 0; o >>= 1) v = op(v, (T)__shfl_xor(v, o, kWaves));
-  return v;
+  return from_lane(sum_row(part[threadIdx.x & (kWaves - 1)]), kWaves - 1);
 }
-struct Add {
-  template <typename T> HQ_DEV T operator()(T x, T y) const { return x + y; }
-};
-struct Most {
-  template <typename T> HQ_DEV T operator()(T x, T y) const { return x > y ? x : y; }
-};
-
+HQ_DEV uint32_t block_most(uint32_t v, uint32_t *part) {
+  v = wave_most(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return wave_most(part[threadIdx.x & (kWaves - 1)]);
+}
 // the sum over the threads before this one
 template <typename T>
 HQ_DEV T sum_before(T v, T *part, T &total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  T sum = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const T other = __shfl_up(sum, o, 64);
-    if (lane >= o) sum += other;
-  }
+  const int wave = threadIdx.x >> 6;
+  const T sum = sum_up_to(v);
   __syncthreads();
-  if (lane == 63) part[wave] = sum;
+  if ((threadIdx.x & 63) == 63) part[wave] = sum;
   __syncthreads();
-  // (a lane a wave: the sums up to each)
-  T waves = part[lane & (kWaves - 1)];
-#pragma unroll
-  for (int o = 1; o < kWaves; o <<= 1) {
-    const T other = __shfl_up(waves, o, kWaves);
-    if ((lane & (kWaves - 1)) >= o) waves += other;
-  }
-  total = __shfl(waves, kWaves - 1, kWaves);
-  const T before = wave ? __shfl(waves, wave - 1, kWaves) : (T)0;
-  return before + (sum - v);
+  const T waves = sum_row(part[threadIdx.x & (kWaves - 1)]);  // (a lane a wave: the sums up to each)
+  total = from_lane(waves, kWaves - 1);
+  return (wave ? from_lane(waves, wave - 1) : (T)0) + (sum - v);
 }
 
 struct Scratch {
@@ -154,12 +205,17 @@ struct Scratch {
       uint64_t weight[kBins];
       uint32_t count[kBins], some[kBins];  // (a key of the bin)
     };
-    uint32_t offset[4 * kBins];  // (the second launch: a step's place in the list)
+    uint32_t offset[4 * kBins + 1];  // (the second launch: a step's place in the list)
   };
   uint64_t part[kWaves];
+  uint32_t part2[kWaves];
   uint64_t found[4];
   double sums[kWaves];
   uint32_t ties[kWaves];
+  uint32_t few, few_keys[kFew];  // keys that a wave can finish with, their indexes, and how many
+  int32_t few_at[kFew];
+  uint64_t ahead[kFew];
+  uint32_t rank[kFew], place[kFew];
 };
 
 // ---- where a row's keys are -----------------------------------------------------------------------------------------
@@ -262,111 +318,163 @@ HQ_DEV uint32_t first_key(uint32_t lo, uint32_t hi, F holds) {
   return lo;
 }
 
-// The first key, from the top downward, up to and with whose equals the count (the weight) of the keys is `target` or more; those below
-// lo do not count.  Not reached: the smallest key there is.  The first round's bins lie evenly over `range` below the
-// largest value, the rest in the last (logits on both sides of 0 would crowd a few bins of keys), those after it evenly over the keys.
-template <bool WEIGHT, typename Source>
-HQ_DEV Line line_of(const Source &source, const Weights &w, uint32_t lo, float range, double target, Scratch &m) {
-  uint32_t hi = w.top;
-  Line o{hi, 0, 0};
-  const float most = (float)w.most, per = (kBins - 0.5f) / range;
-  bool values = most < __builtin_huge_valf() && range > 0.0f && per > 0.0f && per < __builtin_huge_valf();
-  const auto value_bin = [&](uint32_t key) { return (int)fminf((most - value_of(key)) * per, kBins - 1.0f); };
-  while (true) {
-    const int shift = max(22 - (int)__builtin_clz((hi - lo) | 1u), 0);  // hi - lo in 10 bits
+// A search for the line: rounds of histograms over the keys of lo .. hi, each in the bin of the one before in which the line lies.  The
+// first round's bins lie evenly over `range` below the largest value, the rest in the last (logits on both sides of 0 would
+// crowd a few bins of keys), those after it evenly over the keys.
+struct Search {
+  const Weights &w;
+  uint32_t lo, hi;
+  float most, per;
+  bool values;
+  int shift;
+  // of the round: the line's bin, the count (weight) before it and in it, its keys and those before it too, one of them
+  int bin;
+  uint64_t before = 0, own;
+  uint32_t equal, through, some;
+
+  HQ_DEV Search(const Weights &w_, uint32_t lo_, float range) : w(w_), lo(lo_), hi(w_.top), most((float)w_.most), per((kBins - 0.5f) / range) {
+    values = most < __builtin_huge_valf() && range > 0.0f && per > 0.0f && per < __builtin_huge_valf();
+  }
+  HQ_DEV int value_bin(uint32_t key) const { return (int)fminf((most - value_of(key)) * per, kBins - 1.0f); }
+  HQ_DEV int bin_of(uint32_t key) const { return values ? value_bin(key) : (int)((hi - key) >> shift); }
+  HQ_DEV bool inside(uint32_t key) const { return key >= lo && key <= hi; }
+
+  // false: there is no key
+  template <bool WEIGHT, typename Source>
+  HQ_DEV bool round(const Source &source, double target, Scratch &m) {
+    shift = max(22 - (int)__builtin_clz((hi - lo) | 1u), 0);  // hi - lo in 10 bits
     __syncthreads();
     m.count[threadIdx.x] = 0;
     if (WEIGHT) m.weight[threadIdx.x] = 0;
-    if (threadIdx.x == 0) m.found[0] = 0;
     __syncthreads();
     source.sweep([&](const uint32_t keys[4], int32_t) {
 #pragma unroll
       for (int c = 0; c < 4; c++) {
-        const uint32_t key = keys[c];
-        if (key < lo || key > hi) continue;
-        const int bin = values ? value_bin(key) : (int)((hi - key) >> shift);
-        atomicAdd(&m.count[bin], 1u);
-        if (WEIGHT) atomicAdd((unsigned long long *)&m.weight[bin], (unsigned long long)w.steps(key));
-        m.some[bin] = key;
+        if (!inside(keys[c])) continue;
+        const int b = bin_of(keys[c]);
+        atomicAdd(&m.count[b], 1u);
+        if (WEIGHT) atomicAdd((unsigned long long *)&m.weight[b], (unsigned long long)w.steps(keys[c]));
+        m.some[b] = keys[c];
       }
       return true;
     });
     __syncthreads();
     const uint32_t count = m.count[threadIdx.x];
-    uint64_t all;
-    const uint64_t before = o.before + sum_before(WEIGHT ? m.weight[threadIdx.x] : (uint64_t)count, m.part, all);
+    const uint64_t mine = WEIGHT ? m.weight[threadIdx.x] : (uint64_t)count;
+    // the sums over the bins before this thread's, of the line's measure and of keys
+    const int wave = threadIdx.x >> 6;
+    const uint64_t sum = sum_up_to(mine);
+    const uint32_t keys = sum_up_to(count);
+    if ((threadIdx.x & 63) == 63) m.part[wave] = sum, m.part2[wave] = keys;
+    __syncthreads();
+    const uint64_t sums = sum_row(m.part[threadIdx.x & (kWaves - 1)]);
+    const uint32_t all = sum_row(m.part2[threadIdx.x & (kWaves - 1)]);
+    const uint64_t ahead = before + (wave ? from_lane(sums, wave - 1) : 0) + (sum - mine);
+    const uint32_t up_to = (wave ? from_lane(all, wave - 1) : 0) + keys;
     // the last bin with anything in it that begins before the line
-    if (count && (double)before < target) atomicMax((unsigned long long *)&m.found[0], (unsigned long long)threadIdx.x + 1);
+    const uint64_t begun = __ballot(count && (double)ahead < target);
+    if ((threadIdx.x & 63) == 0) m.ties[wave] = begun ? threadIdx.x + 64 - __clzll((long long)begun) : 0;
     __syncthreads();
-    const int bin = (int)m.found[0] - 1;
-    if (bin < 0) return o;
-    if ((int)threadIdx.x == bin) m.found[1] = before;
+    bin = (int)wave_most(m.ties[threadIdx.x & (kWaves - 1)]) - 1;
+    if ((int)threadIdx.x == bin) m.found[1] = ahead, m.found[2] = up_to;
     __syncthreads();
-    o.before = m.found[1];
-    o.equal = m.count[bin];
-    o.key = m.some[bin];
-    if (o.equal == 1) return o;
+    if (bin < 0) return false;
+    before = m.found[1], own = WEIGHT ? m.weight[bin] : (uint64_t)m.count[bin];
+    through = (uint32_t)m.found[2], equal = m.count[bin], some = m.some[bin];
+    return true;
+  }
+
+  // a key that none of the round's bin or before it lies below (the bins' edge, and a bin's width for what rounding does)
+  HQ_DEV uint32_t edge() const {
+    if (!values) return max(lo, hi - min(hi, ((uint32_t)bin << shift) | ((1u << shift) - 1)));
+    return bin >= kBins - 1 ? lo : max(lo, key_of(most - (float)(bin + 2) / per));
+  }
+
+  // the round's bin as the next round's keys; false: it is one key
+  HQ_DEV bool narrow() {
     if (values) {
       const uint32_t from = first_key(lo, hi, [&](uint32_t key) { return value_bin(key) <= bin; });
       if (bin > 0) hi = first_key(lo, hi, [&](uint32_t key) { return value_bin(key) < bin; }) - 1;
       lo = from;
       values = false;
     } else {
-      if (shift == 0) return o;
+      if (shift == 0) return false;
       const uint32_t top = hi - ((uint32_t)bin << shift), width = (1u << shift) - 1;
       lo = top - lo > width ? top - width : lo;
       hi = top;
     }
-    if (lo == hi) return o;
+    return lo < hi;
+  }
+};
+
+// the keys from `edge` on that `takes` says, up to kFew of them, in any order
+template <typename Source, typename F>
+HQ_DEV uint32_t gather(const Source &source, uint32_t edge, Scratch &m, F takes) {
+  __syncthreads();
+  if (threadIdx.x == 0) m.few = 0;
+  __syncthreads();
+  source.sweep([&](const uint32_t keys[4], int32_t i) {
+    if (!__any(max(max(keys[0], keys[1]), max(keys[2], keys[3])) >= edge)) return true;
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      if (keys[c] < edge || !takes(keys[c])) continue;
+      const uint32_t to = atomicAdd(&m.few, 1u);
+      if (to < kFew) m.few_keys[to] = keys[c], m.few_at[to] = source.index(i + c);
+    }
+    return true;
+  });
+  __syncthreads();
+  return m.few;
+}
+
+// Of each of the n gathered keys, a few of them a wave: the measure (a count, or steps of weight) of those before it in falling order
+// (of equals: by index), how many these are, and its place by index, in m.ahead, m.rank and m.place
+template <bool WEIGHT>
+HQ_DEV void order(const Weights &w, int n, Scratch &m) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t key = lane < n ? m.few_keys[lane] : 0u;
+  const int32_t at = lane < n ? m.few_at[lane] : INT32_MAX;
+  const uint64_t mine = WEIGHT && lane < n ? w.steps(key) : 0;
+  for (int i = threadIdx.x >> 6; i < n; i += kWaves) {
+    const uint32_t its = m.few_keys[i];
+    const int32_t its_at = m.few_at[i];
+    const bool first = key > its || (key == its && at < its_at);
+    const uint32_t rank = (uint32_t)__popcll(__ballot(first)), place = (uint32_t)__popcll(__ballot(at < its_at));
+    const uint64_t ahead = WEIGHT ? wave_sum(first ? mine : 0) : rank;
+    if (lane == 0) m.rank[i] = rank, m.place[i] = place, m.ahead[i] = ahead;
+  }
+  __syncthreads();
+}
+
+// The line, the search's first round done: up to and with the equals of its key the count (the weight) of the keys is `target` or more.
+// Not reached: the smallest key there is.
+template <bool WEIGHT, typename Source>
+HQ_DEV Line line_of(const Source &source, Search &f, double target, Scratch &m) {
+  while (true) {
+    if (f.equal == 1) return Line{f.some, f.before, 1};
+    if (f.equal <= kFew) {
+      const int n = (int)gather(source, f.edge(), m, [&](uint32_t key) { return f.inside(key) && f.bin_of(key) == f.bin; });
+      order<WEIGHT>(f.w, n, m);
+      const int lane = threadIdx.x & 63;
+      const uint32_t key = lane < n ? m.few_keys[lane] : 0u;
+      const uint64_t ahead = f.before + (lane < n ? m.ahead[lane] : 0);
+      // (of equals the first begins before the line when any does)
+      const uint32_t least = ~wave_most(lane < n && (double)ahead < target ? ~key : 0u);
+      const uint64_t equal = __ballot(lane < n && key == least);
+      const uint32_t before = ~wave_most(lane < n && key == least ? ~m.rank[lane] : 0u);
+      const uint64_t first = __ballot(lane < n && key == least && m.rank[lane] == before);
+      return Line{least, from_lane(ahead, __ffsll((unsigned long long)first) - 1), (uint32_t)__popcll(equal)};
+    }
+    if (!f.narrow()) return Line{f.some, f.before, f.equal};
+    if (!f.template round<WEIGHT>(source, target, m)) return Line{f.some, f.before, f.equal};
   }
 }
 
 // what top-k, top-p and min-p leave: keys above t, and the first `ties` of those equal to it; weights below min_p not
 struct Kept {
   uint32_t t, ties;
-  bool known;  // (false: t may lie below the keys that the source has)
 };
 constexpr uint32_t kAllTies = UINT32_MAX;
-
-// lo: the source has all of the row's keys from lo on, `keys` of them (lo 1: all there are); sum: the row's whole sum of weights
-// (below 0: not known, the source has all)
-template <typename Source>
-HQ_DEV Kept kept_of(const Source &source, const Weights &w, const Settings &set, uint32_t lo, int64_t keys, double sum, Scratch &m) {
-  Kept o{lo, kAllTies, true};
-  if (set.top_k == 1) return Kept{w.top, 1, true};
-  const float range = (float)fmin(40.0 * 92.332482616893656877 / w.slope, 3e38);
-  if (set.top_k) {
-    if (keys < set.top_k && lo > 1) return Kept{0, 0, false};
-    const Line k = line_of<false>(source, w, lo, range, (double)set.top_k, m);
-    o.t = k.key, o.ties = (uint32_t)min((uint64_t)set.top_k - k.before, (uint64_t)k.equal);
-  }
-  // nothing that the source lacks can have min_p or more
-  const bool low = lo <= 1 || set.top_k || w.of(lo) < set.min_p;
-  if (!(set.top_p < 1.0)) return Kept{o.t, o.ties, low};
-  double steps = sum * w.by;
-  if (set.top_k || sum < 0.0) {
-    uint64_t all = 0;
-    source.sweep([&](const uint32_t k[4], int32_t) {
-#pragma unroll
-      for (int c = 0; c < 4; c++) all += k[c] > o.t || (k[c] == o.t && o.ties == kAllTies) ? w.steps(k[c]) : 0;
-      return true;
-    });
-    all = block_all(all, m.part, Add());
-    if (o.ties != kAllTies) all += o.ties * w.steps(o.t);
-    steps = (double)all;
-  }
-  // (the first token is kept whatever its share)
-  const double target = fmax(set.top_p * steps, 0.5);
-  const Line p = line_of<true>(source, w, max(o.t, 1u), range, target, m);
-  const uint32_t equal = p.key == o.t ? min(p.equal, o.ties) : p.equal;
-  const uint64_t each = w.steps(p.key);
-  if (lo > 1 && !set.top_k && (double)(p.before + equal * each) < target) return Kept{o.t, o.ties, low};  // (all of the source is kept)
-  // ties j = 0, 1, .. with before + j each < target
-  const double room = (target - (double)p.before) / (double)each;
-  uint32_t ties = room < (double)equal ? (uint32_t)ceil(room) : equal;
-  while (ties > 1 && !((double)p.before + (double)(ties - 1) * (double)each < target)) ties--;
-  return Kept{p.key, max(ties, 1u), true};
-}
 
 // ---- the token ------------------------------------------------------------------------------------------------------
 // The first by index whose kept weights up to it are more than u times all.  Each wave sums its part, then the wave in whose part the
@@ -392,16 +500,16 @@ HQ_DEV void draw(const Source &source, const Weights &w, const Settings &set, co
     }
     return true;
   });
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64), tied += __shfl_xor(tied, o, 64);
+  sum = wave_sum(sum), tied = wave_sum(tied);
   __syncthreads();
   if (lane == 0) m.sums[wave] = sum, m.ties[wave] = tied;
   __syncthreads();
-  double total = 0.0;
+  double total = 0.0, of_wave[kWaves];
   uint32_t seen = 0;
+#pragma unroll
   for (int i = 0; i < kWaves; i++) {
-    total += m.sums[i] + (double)min(m.ties[i], most - min(most, seen)) * edge;
-    seen += m.ties[i];
+    of_wave[i] = m.sums[i] + (double)min(m.ties[i], most - min(most, seen)) * edge;
+    total += of_wave[i], seen += m.ties[i];
   }
   const double target = set.u * total;
   // the wave whose sum passes the target (none: the last that has any)
@@ -410,13 +518,13 @@ HQ_DEV void draw(const Source &source, const Weights &w, const Settings &set, co
   int which = -1;
   bool passed = false;
   seen = 0;
+#pragma unroll
   for (int i = 0; i < kWaves; i++) {
-    const double own = m.sums[i] + (double)min(m.ties[i], most - min(most, seen)) * edge;
-    if (!passed && own > 0.0) {
+    if (!passed && of_wave[i] > 0.0) {
       which = i, run = before, tied_before = seen;
-      passed = before + own > target;
+      passed = before + of_wave[i] > target;
     }
-    before += own, seen += m.ties[i];
+    before += of_wave[i], seen += m.ties[i];
   }
   if (wave != which) return;
   int32_t last = -1;
@@ -436,12 +544,7 @@ HQ_DEV void draw(const Source &source, const Weights &w, const Settings &set, co
       if (k[c] == kept.t && k[c]) mine[c] = rank++ < most ? edge : 0.0;
       sum += mine[c];
     }
-    double up_to = sum;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const double other = __shfl_up(up_to, o, 64);
-      if (lane >= o) up_to += other;
-    }
+    const double up_to = sum_up_to(sum);
     // the lane in whose four the target is passed, or the last that has any
     const uint64_t over = __ballot(sum > 0.0 && run + up_to > target), any = __ballot(sum > 0.0);
     if (over || any) {
@@ -455,11 +558,11 @@ HQ_DEV void draw(const Source &source, const Weights &w, const Settings &set, co
         if (mine[c] > 0.0 && (c_at < 0 || !over || !(at > target))) c_at = c, w_at = mine[c];
         at += mine[c];
       }
-      last = __shfl(i + c_at, l, 64);
-      last_chance = (float)(__shfl(w_at, l, 64) / total);
+      last = from_lane(i + c_at, l);
+      last_chance = (float)(from_lane(w_at, l) / total);
       if (over) return false;
     }
-    run += __shfl(up_to, 63, 64);
+    run += from_lane(up_to, 63);
 #pragma unroll
     for (int c = 0; c < 4; c++) tied_before += __popcll(equal[c]);
     return true;
@@ -468,6 +571,127 @@ HQ_DEV void draw(const Source &source, const Weights &w, const Settings &set, co
     *token = last < 0 ? -1 : source.index(last);
     if (chance) *chance = last_chance;
   }
+}
+
+// The same of up to 64 gathered keys that are the first of the row in falling order (all that can be kept among them), by one wave:
+// target: the weight that top-p keeps (0: of what top-k leaves)
+HQ_DEV void draw_few(const Weights &w, const Settings &set, uint32_t n, double target, int32_t *token, float *chance, Scratch &m) {
+  order<true>(w, (int)n, m);
+  if (threadIdx.x >= 64) return;
+  const int lane = threadIdx.x;
+  const bool there = lane < (int)n;
+  const uint32_t key = there ? m.few_keys[lane] : 0u, rank = there ? m.rank[lane] : 0u;
+  const uint64_t ahead = there ? m.ahead[lane] : 0;
+  const double x = there ? w.of(key) : 0.0;
+  const uint64_t mine = (uint64_t)(x * w.by + 0.5);
+  bool kept = there && (!set.top_k || rank < (uint32_t)set.top_k);
+  if (set.top_p < 1.0) {
+    const uint64_t all = wave_sum(kept ? mine : 0);
+    if (!(target > 0.0)) target = fmax(set.top_p * (double)all, 0.5);
+    kept = kept && ((double)ahead < target || rank == 0);
+  }
+  kept = kept && (x >= set.min_p || key == w.top);
+  // by index (what is not kept as 0)
+  const int to = there ? (int)m.place[lane] : lane;
+  const uint64_t bits = __builtin_bit_cast(uint64_t, kept ? x : 0.0);
+  const uint32_t lo = here((uint32_t)__builtin_amdgcn_ds_permute(4 * to, (int32_t)(uint32_t)bits));
+  const uint32_t hi = here((uint32_t)__builtin_amdgcn_ds_permute(4 * to, (int32_t)(uint32_t)(bits >> 32)));
+  const int32_t place = here(__builtin_amdgcn_ds_permute(4 * to, there ? m.few_at[lane] : -1));
+  const double own = __builtin_bit_cast(double, (uint64_t)lo | (uint64_t)hi << 32);
+  const double up_to = sum_up_to(own), total = from_lane(up_to, 63), line = set.u * total;
+  const uint64_t over = __ballot(own > 0.0 && up_to > line), any = __ballot(own > 0.0);
+  const int l = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)any);
+  if (lane == l) {
+    *token = place;
+    if (chance) *chance = (float)(own / total);
+  }
+}
+
+// A row's token from a source that has all of the row's keys from lo on, `keys` of them (lo 1: all there are); sum: the row's whole
+// sum of weights (below 0: not known, the source has all).  false: what is kept may lie below lo.
+template <typename Source>
+HQ_DEV bool answer(const Source &source, const Weights &w, const Settings &set, uint32_t lo, uint32_t keys, double sum, int32_t *token,
+                   float *chance, Scratch &m) {
+  if (set.top_k == 1) {  // the lowest index of the largest
+    uint32_t first = 0;
+    source.sweep([&](const uint32_t k[4], int32_t i) {
+#pragma unroll
+      for (int c = 0; c < 4; c++)
+        if (k[c] == w.top) first = max(first, ~(uint32_t)source.index(i + c));
+      return true;
+    });
+    first = ~block_most(first, (uint32_t *)m.part);
+    if (threadIdx.x == 0) {
+      *token = (int32_t)first;
+      if (chance) *chance = 1.0f;
+    }
+    return true;
+  }
+  Kept kept{lo, kAllTies};
+  const float range = (float)fmin(40.0 * 92.332482616893656877 / w.slope, 3e38);
+  bool cut = false;  // top-k or top-p leave something out
+  if (set.top_k) {
+    if (keys < (uint32_t)set.top_k && lo > 1) return false;
+    Search f(w, lo, range);
+    f.template round<false>(source, set.top_k, m);
+    if (f.through <= kFew) {
+      const uint32_t n = gather(source, f.edge(), m, [&](uint32_t key) { return f.inside(key) && f.bin_of(key) <= f.bin; });
+      draw_few(w, set, n, 0.0, token, chance, m);
+      return true;
+    }
+    const Line k = line_of<false>(source, f, set.top_k, m);
+    kept = Kept{k.key, (uint32_t)min((uint64_t)set.top_k - k.before, (uint64_t)k.equal)};
+    cut = true;
+  }
+  if (set.top_p < 1.0) {
+    double steps = sum * w.by;
+    if (set.top_k || sum < 0.0) {
+      uint64_t all = 0;
+      source.sweep([&](const uint32_t k[4], int32_t) {
+#pragma unroll
+        for (int c = 0; c < 4; c++) all += k[c] > kept.t || (k[c] == kept.t && kept.ties == kAllTies) ? w.steps(k[c]) : 0;
+        return true;
+      });
+      all = block_sum(all, m.part);
+      if (kept.ties != kAllTies) all += kept.ties * w.steps(kept.t);
+      steps = (double)all;
+    }
+    // (the first token is kept whatever its share)
+    const double target = fmax(set.top_p * steps, 0.5);
+    Search f(w, max(kept.t, 1u), range);
+    f.template round<true>(source, target, m);
+    // (the source ends before the line: all of it is kept)
+    if (lo <= 1 || set.top_k || (double)(f.before + f.own) >= target) {
+      if (f.through <= kFew) {
+        const uint32_t n = gather(source, f.edge(), m, [&](uint32_t key) { return f.inside(key) && f.bin_of(key) <= f.bin; });
+        draw_few(w, set, n, target, token, chance, m);
+        return true;
+      }
+      const Line p = line_of<true>(source, f, target, m);
+      const uint32_t equal = p.key == kept.t ? min(p.equal, kept.ties) : p.equal;
+      // ties j = 0, 1, .. with before + j each < target
+      const double each = (double)w.steps(p.key), room = (target - (double)p.before) / each;
+      uint32_t ties = room < (double)equal ? (uint32_t)ceil(room) : equal;
+      while (ties > 1 && !((double)p.before + (double)(ties - 1) * each < target)) ties--;
+      kept = Kept{p.key, max(ties, 1u)};
+      cut = true;
+    }
+  }
+  if (!cut && lo > 1 && !(w.of(lo) < set.min_p)) return false;  // (what the source lacks may have min_p)
+  if (!cut && set.min_p > 0.0) {
+    // (no float below this has it: a logarithm's and the difference's roundings are far below a millionth)
+    const float least = (float)(w.most + (log(set.min_p) * 1.000001 - 1e-6) * 92.332482616893656877 / w.slope);
+    const uint32_t edge = least > -3e38f && w.most < 3e38 ? max(key_of(least - fabsf(least) * 1e-6f), 1u) : 1u;
+    const uint32_t n = gather(source, edge, m, [&](uint32_t key) { return key && (w.of(key) >= set.min_p || key == w.top); });
+    if (n <= kFew) {
+      Settings none = set;
+      none.top_p = 1.0;  // (all of these are within it)
+      draw_few(w, none, n, 0.0, token, chance, m);
+      return true;
+    }
+  }
+  draw(source, w, set, kept, token, chance, m);
+  return true;
 }
 
 // ---- a row a block --------------------------------------------------------------------------------------------------
@@ -492,12 +716,11 @@ __global__ __launch_bounds__(kThreads) void row_kernel(Sample a, double by) {
     top = max(max(top, max(k[0], k[1])), max(k[2], k[3]));
     return true;
   });
-  top = (uint32_t)block_all((uint64_t)top, m.part, Most());
+  top = block_most(top, (uint32_t *)m.part);
   if (!top) return none(a, row);
   const List<true> source(keys, nullptr, a.vocab);
   const Weights w{top, (double)value_of(top), slope_of(set.temperature), by, m.roots};
-  const Kept kept = kept_of(source, w, set, 1u, 0, -1.0, m);
-  draw(source, w, set, kept, a.tokens + row, a.chance ? a.chance + row : nullptr, m);
+  answer(source, w, set, 1u, 0, -1.0, a.tokens + row, a.chance ? a.chance + row : nullptr, m);
 }
 
 // ---- a row over many blocks -----------------------------------------------------------------------------------------
@@ -539,9 +762,7 @@ __global__ __launch_bounds__(256) void hand_kernel(Sample a, Split sp) {
 #pragma unroll
   for (int i = 0; i < 4 * kBatch; i++) mine = fmaxf(mine, v[i]);  // (NaN: the other)
   const uint32_t key = key_of(mine);
-  uint32_t top = key;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor(top, o, 64));
+  const uint32_t top = wave_most(key);
   if (set.all()) {
     if (lane == 0) note->top = top;
   } else {
@@ -687,12 +908,7 @@ HQ_DEV void draw_of_all(const Sample &a, const Split &sp, int64_t row, const Wei
       x[c] = from + c < a.vocab ? w.of(key_of(v)) : 0.0;
       sum += x[c];
     }
-    double up_to = sum;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const double other = __shfl_up(up_to, o, 64);
-      if (lane >= o) up_to += other;
-    }
+    const double up_to = sum_up_to(sum);
     const uint64_t over = __ballot(sum > 0.0 && m.sums[0] + up_to > target), any = __ballot(sum > 0.0);
     if (!any) continue;
     const int l = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)any);
@@ -719,39 +935,42 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Sample a, Split sp, doub
   const Settings set = settings_of(a, row);
   const Note *notes = sp.notes + row * sp.chunks;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // the first of what the first chunks handed on, or whatever lies there, on its way before anything is known
+  constexpr int kEarly = 4;
+  const Pair *handed = sp.handed + row * sp.chunks * kHand;
+  Pair early[kEarly];
+#pragma unroll
+  for (int i = 0; i < kEarly; i++) early[i] = handed[min(wave + i * kWaves, sp.chunks - 1) * kHand + lane];
   if (threadIdx.x < 64) m.roots[threadIdx.x] = kRoots[threadIdx.x];
   // (steps in order of the row: step j of chunk c is the row's j chunks + c; up to 4096, where the histograms will be)
   const int32_t steps = kBatch * sp.chunks;
   uint32_t *const offset = m.offset;
-  uint64_t ends = 0;  // the largest key, and the highest line
+  uint32_t top = 0, line = 0;  // the largest key, and the highest line
+  double sum = 0.0;            // the row's sum of weights, by its chunks' largest
   for (int32_t c = threadIdx.x; c < sp.chunks; c += kThreads) {
-    ends = max(ends, (uint64_t)notes[c].top << 32);
+    top = max(top, notes[c].top);
     if (set.all()) continue;
-    const uint32_t line = notes[c].line;
+    line = max(line, notes[c].line);
     const uint4 q = *(const uint4 *)notes[c].counts;
     const uint32_t d[4] = {q.x, q.y, q.z, q.w};
-    ends = max(ends & ~(uint64_t)UINT32_MAX, (uint64_t)notes[c].top << 32) | max((uint32_t)ends, line);
 #pragma unroll
     for (int j = 0; j < kBatch; j++) offset[j * sp.chunks + c] = (d[j >> 1] >> (16 * (j & 1))) & 0xffffu;
   }
-  ends = block_all(ends, m.part, [](uint64_t x, uint64_t y) {
-    return max(x & ~(uint64_t)UINT32_MAX, y & ~(uint64_t)UINT32_MAX) | max((uint32_t)x, (uint32_t)y);
-  });
-  const uint32_t top = (uint32_t)(ends >> 32), line = (uint32_t)ends;
+  top = block_most(top, (uint32_t *)m.part);
+  line = block_most(line, (uint32_t *)m.part + kWaves);
   if (!top) return none(a, row);
   const Weights w{top, (double)value_of(top), slope_of(set.temperature), by, m.roots};
   if (set.all()) return draw_of_all<WIDE>(a, sp, row, w, set.u, m);
-  // the row's sum of weights
-  double sum = -1.0;
   if (set.whole_sum()) {
-    sum = 0.0;
     for (int32_t c = threadIdx.x; c < sp.chunks; c += kThreads) {
       double own = 0.0;
 #pragma unroll
       for (int j = 0; j < kBatch; j++) own += notes[c].sums[j];
       if (notes[c].top) sum += own * w.of(notes[c].top);
     }
-    sum = block_all(sum, (double *)m.part, Add());
+    sum = block_sum(sum, (double *)m.part);
+  } else {
+    sum = -1.0;
   }
   // each step's place in the list
   const int32_t each = (steps + kThreads - 1) / kThreads, first = min((int32_t)threadIdx.x * each, steps), last = min(first + each, steps);
@@ -763,39 +982,44 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Sample a, Split sp, doub
     offset[i] = before;
     before += n;
   }
+  if (threadIdx.x == 0) offset[steps] = total;
   __syncthreads();
   const int32_t n = (int32_t)total;
   if (n <= kList && line <= top) {
-    uint64_t keys = 0;
-    for (int32_t c = wave; c < sp.chunks; c += kWaves) {
-      const Pair *from = sp.handed + (row * sp.chunks + c) * kHand;
-      const uint4 q = *(const uint4 *)notes[c].counts;
-      const uint32_t d[4] = {q.x, q.y, q.z, q.w};
-      uint32_t start[kBatch + 1];
-      start[0] = 0;
+    uint32_t keys = 0;
+    const auto place = [&](int32_t c, uint32_t e, const Pair &pair) {
+      uint32_t before = 0, to = UINT32_MAX;  // (the chunk's before this step)
 #pragma unroll
-      for (int j = 0; j < kBatch; j++) start[j + 1] = start[j] + ((d[j >> 1] >> (16 * (j & 1))) & 0xffffu);
-      for (uint32_t e = lane; e < start[kBatch]; e += 64) {
-        const Pair pair = from[e];
-        uint32_t to = 0;
-#pragma unroll
-        for (int j = 0; j < kBatch; j++)
-          if (e >= start[j] && e < start[j + 1]) to = offset[j * sp.chunks + c] + (e - start[j]);
-        s.keys[to] = pair.key >= line ? pair.key : 0u;
-        s.at[to] = pair.at;
-        keys += pair.key >= line;
+      for (int j = 0; j < kBatch; j++) {
+        const uint32_t at = offset[j * sp.chunks + c], count = offset[j * sp.chunks + c + 1] - at;
+        if (e >= before && e < before + count) to = at + (e - before);
+        before += count;
       }
+      if (to == UINT32_MAX) return before;
+      s.keys[to] = pair.key >= line ? pair.key : 0u;
+      s.at[to] = pair.at;
+      keys += pair.key >= line;
+      return before;
+    };
+#pragma unroll
+    for (int i = 0; i < kEarly; i++) {
+      const int32_t c = wave + i * kWaves;
+      if (c >= sp.chunks) break;
+      if (place(c, lane, early[i]) > 64) place(c, lane + 64, handed[c * kHand + lane + 64]);
+    }
+    for (int32_t c = wave + kEarly * kWaves; c < sp.chunks; c += kWaves) {
+      const Pair first = handed[c * kHand + lane], second = handed[c * kHand + lane + 64];
+      place(c, lane, first);
+      place(c, lane + 64, second);
     }
     if ((int32_t)threadIdx.x < kStep) s.keys[n + threadIdx.x] = 0;
-    keys = block_all(keys, m.part, Add());
+    keys = block_sum(keys, (uint32_t *)m.part);
     const List<false> source(s.keys, s.at, n);
-    const Kept kept = kept_of(source, w, set, max(line, 1u), (int64_t)keys, sum, m);
-    if (kept.known) return draw(source, w, set, kept, a.tokens + row, a.chance ? a.chance + row : nullptr, m);
+    if (answer(source, w, set, max(line, 1u), keys, sum, a.tokens + row, a.chance ? a.chance + row : nullptr, m)) return;
   }
   __syncthreads();
   const Row<WIDE> source((const float *)(a.logits + row * a.stride), a.vocab);
-  const Kept kept = kept_of(source, w, set, 1u, 0, sum, m);
-  draw(source, w, set, kept, a.tokens + row, a.chance ? a.chance + row : nullptr, m);
+  answer(source, w, set, 1u, 0, sum, a.tokens + row, a.chance ? a.chance + row : nullptr, m);
 }
 
 int32_t chunks_of(int32_t vocab) { return (int32_t)(((int64_t)vocab + kBatch * kStep - 1) / (kBatch * kStep)); }
