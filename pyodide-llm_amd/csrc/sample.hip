@@ -9,7 +9,7 @@
 // Rows of up to 32768 logits: a block a row, whose keys stay in LDS.  Longer rows: every wave of a first launch takes
 // 2048 logits of a row and hands on those above a line of its own, some 90 at most (with what they sum to, where the settings
 // ask for the row's whole sum); a block a row of a second launch finds t among what was handed on, and goes to the row itself
-// only where t lies below one of these lines.  A wave's logits are 8 stripes of 256 over the whole row: words that stand out
+// only where t lies below one of these lines.  A wave's logits are 32 grains of 64 over the whole row: words that stand out
 // often have neighbouring numbers.
 #include <algorithm>
 #include <cmath>
@@ -25,7 +25,9 @@ constexpr int kThreads = 1024, kWaves = kThreads / 64, kBins = kThreads;
 constexpr int kStep = 256;               // logits a wave takes at a time, 4 a lane
 constexpr int kBatch = 8;                // steps whose loads are on their way together
 constexpr int kHeld = 32768, kSmall = 8192;  // the longest rows that a block holds in LDS (alone on its compute unit, beside others)
-constexpr int kHand = 128;               // logits that a wave of the first launch can hand on
+constexpr int kGrain = 64;               // neighbouring logits that the first launch gives to one wave
+constexpr int kGrains = kBatch * kStep / kGrain;
+constexpr int kHand = 192;               // logits that a wave of the first launch can hand on
 constexpr int kList = 7680;              // and what the second launch takes of a row (two blocks a compute unit)
 constexpr int kFew = 64;                 // keys that one wave finishes with
 constexpr uint32_t kLowest = 0x00800000u;  // the key of the lowest finite number
@@ -34,7 +36,7 @@ HQ_DEV uint32_t key_of(float v) {
   const uint32_t bits = __float_as_uint(fadd(v, 0.0f));  // (-0 orders as 0)
   return v > -__builtin_huge_valf() ? bits ^ ((uint32_t)((int32_t)bits >> 31) | 0x80000000u) : 0u;
 }
-HQ_DEV float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
+HQ_DEV float value_of(uint32_t key) { return __uint_as_float(key ^ ((uint32_t)((int32_t)~key >> 31) | 0x80000000u)); }
 
 // 2^(i / 64)
 __device__ const double kRoots[64] = {
@@ -57,29 +59,32 @@ __device__ const double kRoots[64] = {
 };
 
 // e^x for x = d c ln 2 / 64, d c <= 0: 2^(n / 64) from the table, times the series of what is left (|rest| < 0.0055: its sixth power
-// over 720 is below 2^-54), scaled by whole powers of two.  A third of the library's instructions; within 2^-50 of it.
+// over 720 is below 2^-54), scaled by whole powers of two; within 2^-50 of it.  Whole numbers come and go as the low bits of a sum
+// with 1.5 2^52: conversions and scalings of 64-bit numbers take several times an addition.
 HQ_DEV double power(double d, double c, const double *roots) {
-  const double y = fmax(d * c, -70000.0), whole = rint(y), f = y - whole;
-  const int n = (int)whole;
+  const double y = fmax(d * c, -70000.0), sum = y + 6755399441055744.0, f = y - (sum - 6755399441055744.0);
+  const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, sum);
   double s = fma(f, 0x1.5d87fe78a6731p-40, 0x1.3b2ab6fba4e77p-31);
   s = fma(f, s, 0x1.c6b08d704a0c0p-23);
   s = fma(f, s, 0x1.ebfbdff82c58fp-15);
   s = fma(f, s, 0x1.62e42fefa39efp-7);
-  const double root = roots[n & 63];
-  return ldexp(fma(root, f * s, root), n >> 6);
+  const double root = roots[n & 63], x = fma(root, f * s, root);
+  if (n < -65344) return ldexp(x, n >> 6);  // (below 2^-1021)
+  return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, x) + ((uint64_t)(uint32_t)((n >> 6) * (1 << 20)) << 32));
 }
 HQ_DEV double slope_of(double temperature) { return 92.332482616893656877 / temperature; }  // 64 / ln 2 of it
 
 // a row's largest key and temperature: its weights
 struct Weights {
   uint32_t top;
-  double most, slope, by;  // the largest logit; by: 1 / step
+  double most, slope, by;  // the largest logit; by: 1 / step, a power of two up to 2^51
   const double *roots;
   HQ_DEV double of(uint32_t key) const {
     const double x = power((double)value_of(key) - most, slope, roots);
     return key == top ? 1.0 : key ? x : 0.0;
   }
-  HQ_DEV uint64_t steps(uint32_t key) const { return (uint64_t)(of(key) * by + 0.5); }
+  HQ_DEV uint64_t steps_of(double x) const { return __builtin_bit_cast(uint64_t, x * by + 0x1p52) - 0x4330000000000000u; }
+  HQ_DEV uint64_t steps(uint32_t key) const { return steps_of(of(key)); }
 };
 
 struct Settings {
@@ -200,13 +205,8 @@ HQ_DEV T sum_before(T v, T *part, T &total) {
 
 struct Scratch {
   double roots[64];
-  union {
-    struct {
-      uint64_t weight[kBins];
-      uint32_t count[kBins], some[kBins];  // (a key of the bin)
-    };
-    uint32_t offset[4 * kBins + 1];  // (the second launch: a step's place in the list)
-  };
+  uint64_t weight[kBins];
+  uint32_t count[kBins], some[kBins];  // (a key of the bin)
   uint64_t part[kWaves];
   uint32_t part2[kWaves];
   uint64_t found[4];
@@ -222,14 +222,13 @@ struct Scratch {
 // A wave takes a part of the row, `part` logits (whole steps) from wave * part on, a step's 4 a lane at a time, in order:
 // sweep(f) calls f(keys, the first's place) until it returns false.
 
-// 8 steps of logits, `stride` apart from `from` on; -infinity from `to` on
+// 4 logits of each of 8 steps, `stride` apart from the lane's own `from` on; -infinity from `to` on.  whole: all lie before `to`
 template <bool WIDE>
-HQ_DEV void load(const float *p, int32_t n, int32_t from, int32_t stride, int32_t to, float v[4 * kBatch]) {
-  const int lane = threadIdx.x & 63;
-  if (from + (kBatch - 1) * stride + kStep <= to) {
+HQ_DEV void load(const float *p, int32_t n, int32_t from, int32_t stride, int32_t to, bool whole, float v[4 * kBatch]) {
+  if (whole) {
 #pragma unroll
     for (int j = 0; j < kBatch; j++) {
-      const float *q = p + from + j * stride + 4 * lane;
+      const float *q = p + from + j * stride;
       if (WIDE) {  // (rows that begin on 16 bytes)
         const float4 f = *(const float4 *)q;
         v[4 * j] = f.x, v[4 * j + 1] = f.y, v[4 * j + 2] = f.z, v[4 * j + 3] = f.w;
@@ -242,7 +241,7 @@ HQ_DEV void load(const float *p, int32_t n, int32_t from, int32_t stride, int32_
   }
 #pragma unroll
   for (int j = 0; j < kBatch; j++) {
-    const int32_t i = from + j * stride + 4 * lane;
+    const int32_t i = from + j * stride;
 #pragma unroll
     for (int c = 0; c < 4; c++) v[4 * j + c] = p[min(i + c, n - 1)];
 #pragma unroll
@@ -263,7 +262,7 @@ struct Row {  // a row in memory
     const int32_t from = (int32_t)(threadIdx.x >> 6) * part, to = min(from + part, n);
     for (int32_t i0 = from; i0 < to; i0 += kBatch * kStep) {
       float v[4 * kBatch];
-      load<WIDE>(p, n, i0, kStep, to, v);
+      load<WIDE>(p, n, i0 + 4 * (int32_t)(threadIdx.x & 63), kStep, to, i0 + kBatch * kStep <= to, v);
 #pragma unroll
       for (int j = 0; j < kBatch; j++) {
         uint32_t keys[4];
@@ -583,7 +582,7 @@ HQ_DEV void draw_few(const Weights &w, const Settings &set, uint32_t n, double t
   const uint32_t key = there ? m.few_keys[lane] : 0u, rank = there ? m.rank[lane] : 0u;
   const uint64_t ahead = there ? m.ahead[lane] : 0;
   const double x = there ? w.of(key) : 0.0;
-  const uint64_t mine = (uint64_t)(x * w.by + 0.5);
+  const uint64_t mine = w.steps_of(x);
   bool kept = there && (!set.top_k || rank < (uint32_t)set.top_k);
   if (set.top_p < 1.0) {
     const uint64_t all = wave_sum(kept ? mine : 0);
@@ -725,16 +724,17 @@ __global__ __launch_bounds__(kThreads) void row_kernel(Sample a, double by) {
 
 // ---- a row over many blocks -----------------------------------------------------------------------------------------
 // What a wave of the first launch leaves: its largest key, its line (it handed on all from there on; 1: all that there are), how
-// many of each of its steps it handed on, and the sums of each step's weights relative to its largest
+// many it handed on, and of each of its grains (grain 4 j + s at counts[s][j]), its weights' sum relative to its largest, and each grain's,
+// where nothing is cut off
 struct alignas(16) Note {
-  uint16_t counts[kBatch];
-  double sums[kBatch];
-  uint32_t top, line;
+  uint8_t counts[4][kBatch];
+  uint32_t top, line, handed;
+  double sum, sums[kGrains];
 };
 struct Pair {
-  uint32_t key;
-  int32_t at;
+  uint32_t key, at;  // (the index, and from bit 20 on how many of its grain come before it)
 };
+static_assert(kMostVocab <= 1 << 20 && kGrain <= 1 << 12, "a pair's index");
 struct Split {
   Note *notes;   // [rows][chunks]
   Pair *handed;  // [rows][chunks][kHand]
@@ -754,9 +754,11 @@ __global__ __launch_bounds__(256) void hand_kernel(Sample a, Split sp) {
   const int64_t row = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
   if (chunk >= sp.chunks || row >= a.rows) return;
   const Settings set = settings_of(a, row);
-  const int32_t stripe = sp.chunks * kStep;
+  // the lane's logits: 4 of grain (4 j + s) chunks + chunk of the row, s its 16 lanes
+  const int32_t stride = 4 * sp.chunks * kGrain, from = (lane >> 4) * (stride / 4) + chunk * kGrain + 4 * (lane & 15);
   float v[4 * kBatch];
-  load<WIDE>((const float *)(a.logits + row * a.stride), a.vocab, chunk * kStep, stripe, a.vocab, v);
+  load<WIDE>((const float *)(a.logits + row * a.stride), a.vocab, from, stride, a.vocab,
+             ((kGrains - 1) * sp.chunks + chunk + 1) * kGrain <= a.vocab, v);
   Note *note = sp.notes + row * sp.chunks + chunk;
   float mine = -__builtin_huge_valf();
 #pragma unroll
@@ -774,107 +776,98 @@ __global__ __launch_bounds__(256) void hand_kernel(Sample a, Split sp) {
       if (above >= lanes) line |= bit;
       if (above == lanes) break;
     }
-    uint16_t counts[kBatch];
     int total = 0;
-    const auto count = [&](float from) {
+    const auto count = [&](float least) {
       total = 0;
 #pragma unroll
-      for (int j = 0; j < kBatch; j++) {
-        int n = 0;
-#pragma unroll
-        for (int c = 0; c < 4; c++) n += __popcll(__ballot(v[4 * j + c] >= from));
-        counts[j] = (uint16_t)n, total += n;
+      for (int i = 0; i < 4 * kBatch; i++) {
+        total += __popcll(__ballot(v[i] >= least));
         __builtin_amdgcn_sched_barrier(0);
       }
     };
     line = line < kLowest ? 1u : line;
-    float from = value_of(max(line, kLowest));
-    count(from);
+    float least = value_of(max(line, kLowest));
+    count(least);
     if (total > kHand) {  // (equal ones by the dozen: those above them, if these are fewer)
       line = max(line, kLowest) + 1;
-      from = value_of(line);
-      if (line <= top) count(from);
-      if (line > top || total > kHand) {
-        line = UINT32_MAX, total = 0;
+      least = value_of(line);
+      if (line <= top) count(least);
+      if (line > top || total > kHand) line = UINT32_MAX, total = 0, least = __builtin_nanf("");
+    }
+    Pair *to = sp.handed + (row * sp.chunks + chunk) * kHand;
+    uint32_t counts[2] = {0, 0};  // of the lane's s, a byte a step
 #pragma unroll
-        for (int j = 0; j < kBatch; j++) counts[j] = 0;
+    for (int j = 0; j < kBatch; j++) {
+      anew(v + 4 * j);
+      uint64_t in[4], any = 0;
+#pragma unroll
+      for (int c = 0; c < 4; c++) in[c] = __ballot(v[4 * j + c] >= least), any |= in[c];
+      if (!any) continue;
+      // before it in the step, and in its grain
+      uint32_t before = 0, grain = 0, all = 0;
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        const uint32_t mine = (uint32_t)(in[c] >> (lane & 48)) & 0xffffu;
+        before += __popcll(in[c] & (((uint64_t)1 << lane) - 1));
+        grain += __popc(mine & ((1u << (lane & 15)) - 1));
+        all += __popc(mine);
       }
+      counts[j >> 2] |= all << (8 * (j & 3));
+#pragma unroll
+      for (int c = 0; c < 4; c++)
+        if (v[4 * j + c] >= least) to[before++] = Pair{key_of(v[4 * j + c]), (uint32_t)(from + j * stride + c) | (grain++ << 20)};
+#pragma unroll
+      for (int c = 0; c < 4; c++) to += __popcll(in[c]);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if (total) {
-      Pair *to = sp.handed + (row * sp.chunks + chunk) * kHand;
-#pragma unroll
-      for (int j = 0; j < kBatch; j++) {
-        if (!counts[j]) continue;
-        anew(v + 4 * j);
-        int before = 0, own = 0;
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-          const uint64_t in = __ballot(v[4 * j + c] >= from);
-          before += __popcll(in & (((uint64_t)1 << lane) - 1));
-        }
-#pragma unroll
-        for (int c = 0; c < 4; c++)
-          if (v[4 * j + c] >= from) to[before + own++] = Pair{key_of(v[4 * j + c]), chunk * kStep + j * stripe + 4 * lane + c};
-        to += counts[j];
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-    if (lane == 0) {
-      note->top = top, note->line = line;
-#pragma unroll
-      for (int j = 0; j < kBatch; j++) note->counts[j] = counts[j];
-    }
+    if ((lane & 15) == 0) *(uint2 *)note->counts[lane >> 4] = make_uint2(counts[0], counts[1]);
+    if (lane == 0) note->top = top, note->line = line, note->handed = (uint32_t)total;
   }
   if (!set.whole_sum()) return;
   const double slope = slope_of(set.temperature), most = (double)value_of(top);
-  double s[kBatch];
+  double sum = 0.0;
 #pragma unroll
   for (int j = 0; j < kBatch; j++) {
     anew(v + 4 * j);
-    s[j] = 0.0;
+    double s = 0.0;
 #pragma unroll
     for (int c = 0; c < 4; c++) {
       const float x = v[4 * j + c];
       const double e = power((double)x - most, slope, roots);
-      s[j] += x == value_of(top) ? 1.0 : x > -__builtin_huge_valf() ? e : 0.0;
+      s += x == value_of(top) ? 1.0 : x > -__builtin_huge_valf() ? e : 0.0;
     }
+    if (set.all()) {  // (the 16 lanes' last has their sum)
+      const double grain = sum_row(s);
+      if ((lane & 15) == 15) note->sums[4 * j + (lane >> 4)] = top ? grain : 0.0;
+    }
+    sum += s;
     __builtin_amdgcn_sched_barrier(0);
   }
-  // the eight sums over the lanes: halves of them change sides until a lane holds an eighth of one
-#pragma unroll
-  for (int half = kBatch / 2, mask = 32; half; half >>= 1, mask >>= 1) {
-    const bool upper = lane & mask;
-#pragma unroll
-    for (int j = 0; j < half; j++) {
-      const double give = upper ? s[j] : s[j + half], keep = upper ? s[j + half] : s[j];
-      s[j] = keep + __shfl_xor(give, mask, 64);
-    }
-  }
-#pragma unroll
-  for (int o = 4; o > 0; o >>= 1) s[0] += __shfl_xor(s[0], o, 64);
-  if ((lane & 7) == 0) note->sums[lane >> 3] = top ? s[0] : 0.0;
+  sum = wave_sum(sum);
+  if (lane == 0) note->sum = top ? sum : 0.0;
 }
 
 struct Joint {
   Scratch m;
+  uint16_t offset[kMostVocab / kGrain + kGrains];  // a grain's place in the list
   uint32_t keys[kList + kStep];
   int32_t at[kList + kStep];
 };
 
-// nothing is cut off: the step in which the sum is reached by what the first launch summed, then its 256 logits
+// nothing is cut off: the grain in which the sum is reached by what the first launch summed, then its 64 logits
 template <bool WIDE>
 HQ_DEV void draw_of_all(const Sample &a, const Split &sp, int64_t row, const Weights &w, double u, Scratch &m) {
   const Note *notes = sp.notes + row * sp.chunks;
-  const int32_t steps = kBatch * sp.chunks, each = (steps + kThreads - 1) / kThreads, first = threadIdx.x * each;
+  const int32_t grains = kGrains * sp.chunks, each = (grains + kThreads - 1) / kThreads, first = threadIdx.x * each;
   const auto sum_of = [&](int32_t i) {
-    if (i >= steps) return 0.0;
+    if (i >= grains) return 0.0;
     const Note &n = notes[i % sp.chunks];
     return n.top ? n.sums[i / sp.chunks] * w.of(n.top) : 0.0;
   };
   double mine = 0.0, total;
   for (int32_t i = first; i < first + each; i++) mine += sum_of(i);
   const double before = sum_before(mine, (double *)m.part, total), target = u * total;
-  // the thread in whose steps the target is passed, or the last that has any
+  // the thread in whose grains the target is passed, or the last that has any
   if (threadIdx.x == 0) m.found[0] = UINT64_MAX, m.found[1] = 0;
   __syncthreads();
   if (mine > 0.0) {
@@ -898,30 +891,16 @@ HQ_DEV void draw_of_all(const Sample &a, const Split &sp, int64_t row, const Wei
   if (threadIdx.x >= 64) return;
   const int lane = threadIdx.x;
   const float *p = (const float *)(a.logits + row * a.stride);
-  // (a step whose sum is some smallest number may have no weight that is one: then the next, or the one before)
-  for (int32_t i = (int32_t)m.found[2]; i >= 0 && i < steps; i += passed ? 1 : -1) {
-    const int32_t from = i * kStep + 4 * lane;
-    double x[4], sum = 0.0;
-#pragma unroll
-    for (int c = 0; c < 4; c++) {
-      const float v = p[min(from + c, a.vocab - 1)];
-      x[c] = from + c < a.vocab ? w.of(key_of(v)) : 0.0;
-      sum += x[c];
-    }
-    const double up_to = sum_up_to(sum);
-    const uint64_t over = __ballot(sum > 0.0 && m.sums[0] + up_to > target), any = __ballot(sum > 0.0);
+  // (a grain whose sum is some smallest number may have no weight that is one: then the next, or the one before)
+  for (int32_t g = (int32_t)m.found[2]; g >= 0 && g < grains; g += passed ? 1 : -1) {
+    const int32_t i = g * kGrain + lane;
+    const float v = p[min(i, a.vocab - 1)];
+    const double x = i < a.vocab ? w.of(key_of(v)) : 0.0, up_to = sum_up_to(x);
+    const uint64_t over = __ballot(x > 0.0 && m.sums[0] + up_to > target), any = __ballot(x > 0.0);
     if (!any) continue;
-    const int l = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)any);
-    double at = m.sums[0] + (up_to - sum), share = 0.0;
-    int32_t found = -1;
-#pragma unroll
-    for (int c = 0; c < 4; c++) {
-      if (x[c] > 0.0 && (found < 0 || !over || !(at > target))) found = from + c, share = x[c];
-      at += x[c];
-    }
-    if (lane == l) {
-      a.tokens[row] = found;
-      if (a.chance) a.chance[row] = (float)(share / total);
+    if (lane == (over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)any))) {
+      a.tokens[row] = i;
+      if (a.chance) a.chance[row] = (float)(x / total);
     }
     return;
   }
@@ -938,80 +917,71 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Sample a, Split sp, doub
   // the first of what the first chunks handed on, or whatever lies there, on its way before anything is known
   constexpr int kEarly = 4;
   const Pair *handed = sp.handed + row * sp.chunks * kHand;
+  const auto handed_by = [&](int32_t c) { return (int32_t)notes[c].handed; };
   Pair early[kEarly];
+  int32_t early_n[kEarly];
 #pragma unroll
-  for (int i = 0; i < kEarly; i++) early[i] = handed[min(wave + i * kWaves, sp.chunks - 1) * kHand + lane];
+  for (int i = 0; i < kEarly; i++) {
+    const int32_t c = min(wave + i * kWaves, sp.chunks - 1);
+    early[i] = handed[c * kHand + lane];
+    early_n[i] = handed_by(c);
+  }
   if (threadIdx.x < 64) m.roots[threadIdx.x] = kRoots[threadIdx.x];
-  // (steps in order of the row: step j of chunk c is the row's j chunks + c; up to 4096, where the histograms will be)
-  const int32_t steps = kBatch * sp.chunks;
-  uint32_t *const offset = m.offset;
+  // (grains in order of the row: number (4 j + s) chunks + c is chunk c's grain 4 j + s)
+  const int32_t grains = kGrains * sp.chunks;
   uint32_t top = 0, line = 0;  // the largest key, and the highest line
-  double sum = 0.0;            // the row's sum of weights, by its chunks' largest
   for (int32_t c = threadIdx.x; c < sp.chunks; c += kThreads) {
     top = max(top, notes[c].top);
     if (set.all()) continue;
     line = max(line, notes[c].line);
-    const uint4 q = *(const uint4 *)notes[c].counts;
-    const uint32_t d[4] = {q.x, q.y, q.z, q.w};
+    const uint4 q[2] = {*(const uint4 *)notes[c].counts[0], *(const uint4 *)notes[c].counts[2]};
+    const uint32_t d[8] = {q[0].x, q[0].y, q[0].z, q[0].w, q[1].x, q[1].y, q[1].z, q[1].w};
 #pragma unroll
-    for (int j = 0; j < kBatch; j++) offset[j * sp.chunks + c] = (d[j >> 1] >> (16 * (j & 1))) & 0xffffu;
+    for (int g = 0; g < kGrains; g++)  // (grain 4 j + s is byte j & 3 of dword 2 s + j / 4)
+      s.offset[g * sp.chunks + c] = (uint16_t)((d[2 * (g & 3) + (g >> 4)] >> (8 * ((g >> 2) & 3))) & 0xffu);
   }
   top = block_most(top, (uint32_t *)m.part);
   line = block_most(line, (uint32_t *)m.part + kWaves);
   if (!top) return none(a, row);
   const Weights w{top, (double)value_of(top), slope_of(set.temperature), by, m.roots};
   if (set.all()) return draw_of_all<WIDE>(a, sp, row, w, set.u, m);
+  double sum = -1.0;  // the row's sum of weights, by its chunks' largest
   if (set.whole_sum()) {
-    for (int32_t c = threadIdx.x; c < sp.chunks; c += kThreads) {
-      double own = 0.0;
-#pragma unroll
-      for (int j = 0; j < kBatch; j++) own += notes[c].sums[j];
-      if (notes[c].top) sum += own * w.of(notes[c].top);
-    }
+    sum = 0.0;
+    for (int32_t c = threadIdx.x; c < sp.chunks; c += kThreads)
+      if (notes[c].top) sum += notes[c].sum * w.of(notes[c].top);
     sum = block_sum(sum, (double *)m.part);
-  } else {
-    sum = -1.0;
   }
-  // each step's place in the list
-  const int32_t each = (steps + kThreads - 1) / kThreads, first = min((int32_t)threadIdx.x * each, steps), last = min(first + each, steps);
+  // each grain's place in the list
+  const int32_t each = (grains + kThreads - 1) / kThreads, first = min((int32_t)threadIdx.x * each, grains), last = min(first + each, grains);
   uint32_t mine = 0, total;
-  for (int32_t i = first; i < last; i++) mine += offset[i];
+  for (int32_t i = first; i < last; i++) mine += s.offset[i];
   uint32_t before = sum_before(mine, (uint32_t *)m.part, total);
   for (int32_t i = first; i < last; i++) {
-    const uint32_t n = offset[i];
-    offset[i] = before;
+    const uint32_t n = s.offset[i];
+    s.offset[i] = (uint16_t)before;  // (where it does not fit, neither does the list)
     before += n;
   }
-  if (threadIdx.x == 0) offset[steps] = total;
   __syncthreads();
   const int32_t n = (int32_t)total;
   if (n <= kList && line <= top) {
     uint32_t keys = 0;
-    const auto place = [&](int32_t c, uint32_t e, const Pair &pair) {
-      uint32_t before = 0, to = UINT32_MAX;  // (the chunk's before this step)
-#pragma unroll
-      for (int j = 0; j < kBatch; j++) {
-        const uint32_t at = offset[j * sp.chunks + c], count = offset[j * sp.chunks + c + 1] - at;
-        if (e >= before && e < before + count) to = at + (e - before);
-        before += count;
-      }
-      if (to == UINT32_MAX) return before;
+    const auto place = [&](const Pair &pair) {
+      const int32_t i = (int32_t)(pair.at & (kMostVocab - 1));
+      const uint32_t to = s.offset[i / kGrain] + (pair.at >> 20);
       s.keys[to] = pair.key >= line ? pair.key : 0u;
-      s.at[to] = pair.at;
+      s.at[to] = i;
       keys += pair.key >= line;
-      return before;
     };
 #pragma unroll
     for (int i = 0; i < kEarly; i++) {
       const int32_t c = wave + i * kWaves;
       if (c >= sp.chunks) break;
-      if (place(c, lane, early[i]) > 64) place(c, lane + 64, handed[c * kHand + lane + 64]);
+      if (lane < early_n[i]) place(early[i]);
+      for (int32_t e = lane + 64; e < early_n[i]; e += 64) place(handed[c * kHand + e]);
     }
-    for (int32_t c = wave + kEarly * kWaves; c < sp.chunks; c += kWaves) {
-      const Pair first = handed[c * kHand + lane], second = handed[c * kHand + lane + 64];
-      place(c, lane, first);
-      place(c, lane + 64, second);
-    }
+    for (int32_t c = wave + kEarly * kWaves; c < sp.chunks; c += kWaves)
+      for (int32_t e = lane, n = handed_by(c); e < n; e += 64) place(handed[c * kHand + e]);
     if ((int32_t)threadIdx.x < kStep) s.keys[n + threadIdx.x] = 0;
     keys = block_sum(keys, (uint32_t *)m.part);
     const List<false> source(s.keys, s.at, n);
@@ -1034,10 +1004,10 @@ int64_t sample_work_bytes(int32_t rows, int32_t vocab) {
 
 hipError_t launch_sample(const Sample &a, hipStream_t s) {
   if (a.rows <= 0 || a.vocab <= 0) return hipSuccess;
-  // (a row's steps stay below 2^62)
+  // (a weight's steps stay below 2^52, a row's below 2^62)
   int bits = 0;
   while (((int64_t)1 << bits) < a.vocab) bits++;
-  const double by = (double)((int64_t)1 << (62 - bits));
+  const double by = (double)((int64_t)1 << std::min(51, 62 - bits));
   const bool wide = a.vocab >= 4 && (uintptr_t)a.logits % 16 == 0 && (a.rows == 1 || a.stride % 16 == 0);
   if (a.vocab <= kHeld) {
     const auto kernel = a.vocab <= kSmall ? wide ? row_kernel<true, kSmall> : row_kernel<false, kSmall>
