@@ -6,7 +6,7 @@
 // histograms are whole numbers (steps of a power of two below the largest weight), so that no order of additions changes them.
 // The token is then found by a sum over the kept weights in index order, in 64 bits.
 //
-// Rows of up to 32768 logits: a block a row, whose keys stay in LDS.  Longer rows: every wave of a first launch takes
+// Rows of up to 8192 logits: a block a row, whose keys stay in LDS.  Longer rows: every wave of a first launch takes
 // 2048 logits of a row and hands on those above a line of its own, some 90 at most (with what they sum to, where the settings
 // ask for the row's whole sum); a block a row of a second launch finds t among what was handed on, and goes to the row itself
 // only where t lies below one of these lines.  A wave's logits are 32 grains of 64 over the whole row: words that stand out
@@ -24,7 +24,7 @@ namespace {
 constexpr int kThreads = 1024, kWaves = kThreads / 64, kBins = kThreads;
 constexpr int kStep = 256;               // logits a wave takes at a time, 4 a lane
 constexpr int kBatch = 8;                // steps whose loads are on their way together
-constexpr int kHeld = 32768, kSmall = 8192;  // the longest rows that a block holds in LDS (alone on its compute unit, beside others)
+constexpr int kHeld = 8192;              // the longest row that a block takes alone, in LDS
 constexpr int kGrain = 64;               // neighbouring logits that the first launch gives to one wave
 constexpr int kGrains = kBatch * kStep / kGrain;
 constexpr int kHand = 192;               // logits that a wave of the first launch can hand on
@@ -60,7 +60,7 @@ __device__ const double kRoots[64] = {
 
 // e^x for x = d c ln 2 / 64, d c <= 0: 2^(n / 64) from the table, times the series of what is left (|rest| < 0.0055: its sixth power
 // over 720 is below 2^-54), scaled by whole powers of two; within 2^-50 of it.  Whole numbers come and go as the low bits of a sum
-// with 1.5 2^52: conversions and scalings of 64-bit numbers take several times an addition.
+// with 1.5 2^52: conversions of 64-bit numbers take several times an addition.
 HQ_DEV double power(double d, double c, const double *roots) {
   const double y = fmax(d * c, -70000.0), sum = y + 6755399441055744.0, f = y - (sum - 6755399441055744.0);
   const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, sum);
@@ -68,9 +68,8 @@ HQ_DEV double power(double d, double c, const double *roots) {
   s = fma(f, s, 0x1.c6b08d704a0c0p-23);
   s = fma(f, s, 0x1.ebfbdff82c58fp-15);
   s = fma(f, s, 0x1.62e42fefa39efp-7);
-  const double root = roots[n & 63], x = fma(root, f * s, root);
-  if (n < -65344) return ldexp(x, n >> 6);  // (below 2^-1021)
-  return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, x) + ((uint64_t)(uint32_t)((n >> 6) * (1 << 20)) << 32));
+  const double root = roots[n & 63];
+  return ldexp(fma(root, f * s, root), n >> 6);
 }
 HQ_DEV double slope_of(double temperature) { return 92.332482616893656877 / temperature; }  // 64 / ln 2 of it
 
@@ -87,9 +86,11 @@ struct Weights {
   HQ_DEV uint64_t steps(uint32_t key) const { return steps_of(of(key)); }
 };
 
+HQ_DEV float range_of(const Weights &w) { return (float)fmin(40.0 * 92.332482616893656877 / w.slope, 3e38); }
+
 struct Settings {
   double temperature, top_p, min_p, u;
-  int32_t top_k;  // (0: all)
+  int32_t top_k, vocab;  // (0: all)
   HQ_DEV bool all() const { return !top_k && !(top_p < 1.0) && !(min_p > 0.0); }
   HQ_DEV bool whole_sum() const { return !top_k && (top_p < 1.0 || !(min_p > 0.0)); }  // the row's whole sum is needed
 };
@@ -99,6 +100,7 @@ HQ_DEV Settings settings_of(const Sample &a, int64_t row) {
   const float top_p = (a.top_p ? a.top_p : a.u)[row], min_p = (a.min_p ? a.min_p : a.u)[row];
   const int32_t top_k = (a.top_k ? a.top_k : (const int32_t *)a.u)[row];
   Settings o;
+  o.vocab = a.vocab;
   o.temperature = a.temperature ? temperature : 1.0f;
   o.top_k = a.top_k && top_k > 0 && top_k < a.vocab ? top_k : 0;
   o.top_p = a.top_p ? top_p : 1.0f;
@@ -222,12 +224,12 @@ struct Scratch {
 // A wave takes a part of the row, `part` logits (whole steps) from wave * part on, a step's 4 a lane at a time, in order:
 // sweep(f) calls f(keys, the first's place) until it returns false.
 
-// 4 logits of each of 8 steps, `stride` apart from the lane's own `from` on; -infinity from `to` on.  whole: all lie before `to`
-template <bool WIDE>
-HQ_DEV void load(const float *p, int32_t n, int32_t from, int32_t stride, int32_t to, bool whole, float v[4 * kBatch]) {
+// 4 logits of each of BATCH steps, `stride` apart from the lane's own `from` on; -infinity from `to` on.  whole: all lie before `to`
+template <bool WIDE, int BATCH>
+HQ_DEV void load(const float *p, int32_t n, int32_t from, int32_t stride, int32_t to, bool whole, float v[4 * BATCH]) {
   if (whole) {
 #pragma unroll
-    for (int j = 0; j < kBatch; j++) {
+    for (int j = 0; j < BATCH; j++) {
       const float *q = p + from + j * stride;
       if (WIDE) {  // (rows that begin on 16 bytes)
         const float4 f = *(const float4 *)q;
@@ -240,7 +242,7 @@ HQ_DEV void load(const float *p, int32_t n, int32_t from, int32_t stride, int32_
     return;
   }
 #pragma unroll
-  for (int j = 0; j < kBatch; j++) {
+  for (int j = 0; j < BATCH; j++) {
     const int32_t i = from + j * stride;
 #pragma unroll
     for (int c = 0; c < 4; c++) v[4 * j + c] = p[min(i + c, n - 1)];
@@ -251,20 +253,21 @@ HQ_DEV void load(const float *p, int32_t n, int32_t from, int32_t stride, int32_
   }
 }
 
-template <bool WIDE>
-struct Row {  // a row in memory
+template <bool WIDE, int BATCH = kBatch>
+struct Row {  // a row, or the part of one from `base` on, in memory
   const float *p;
-  int32_t n, part;
-  HQ_DEV Row(const float *p_, int32_t n_) : p(p_), n(n_), part((n_ + kWaves * kStep - 1) / (kWaves * kStep) * kStep) {}
-  HQ_DEV int32_t index(int32_t i) const { return i; }
+  int32_t n, part, base;
+  HQ_DEV Row(const float *row, int32_t n_, int32_t base_ = 0)
+      : p(row + base_), n(n_), part((n_ + kWaves * kStep - 1) / (kWaves * kStep) * kStep), base(base_) {}
+  HQ_DEV int32_t index(int32_t i) const { return base + i; }
   template <typename F>
   HQ_DEV void sweep(F f) const {
     const int32_t from = (int32_t)(threadIdx.x >> 6) * part, to = min(from + part, n);
-    for (int32_t i0 = from; i0 < to; i0 += kBatch * kStep) {
-      float v[4 * kBatch];
-      load<WIDE>(p, n, i0 + 4 * (int32_t)(threadIdx.x & 63), kStep, to, i0 + kBatch * kStep <= to, v);
+    for (int32_t i0 = from; i0 < to; i0 += BATCH * kStep) {
+      float v[4 * BATCH];
+      load<WIDE, BATCH>(p, n, i0 + 4 * (int32_t)(threadIdx.x & 63), kStep, to, i0 + BATCH * kStep <= to, v);
 #pragma unroll
-      for (int j = 0; j < kBatch; j++) {
+      for (int j = 0; j < BATCH; j++) {
         uint32_t keys[4];
 #pragma unroll
         for (int c = 0; c < 4; c++) keys[c] = key_of(v[4 * j + c]);
@@ -338,9 +341,9 @@ struct Search {
   HQ_DEV int bin_of(uint32_t key) const { return values ? value_bin(key) : (int)((hi - key) >> shift); }
   HQ_DEV bool inside(uint32_t key) const { return key >= lo && key <= hi; }
 
-  // false: there is no key
+  // the round's histogram in m
   template <bool WEIGHT, typename Source>
-  HQ_DEV bool round(const Source &source, double target, Scratch &m) {
+  HQ_DEV void tally(const Source &source, Scratch &m) {
     shift = max(22 - (int)__builtin_clz((hi - lo) | 1u), 0);  // hi - lo in 10 bits
     __syncthreads();
     m.count[threadIdx.x] = 0;
@@ -358,6 +361,10 @@ struct Search {
       return true;
     });
     __syncthreads();
+  }
+  // the line's bin by it; false: there is no key
+  template <bool WEIGHT>
+  HQ_DEV bool find(double target, Scratch &m) {
     const uint32_t count = m.count[threadIdx.x];
     const uint64_t mine = WEIGHT ? m.weight[threadIdx.x] : (uint64_t)count;
     // the sums over the bins before this thread's, of the line's measure and of keys
@@ -383,6 +390,11 @@ struct Search {
     return true;
   }
 
+  template <bool WEIGHT, typename Source>
+  HQ_DEV bool round(const Source &source, double target, Scratch &m) {
+    tally<WEIGHT>(source, m);
+    return find<WEIGHT>(target, m);
+  }
   // a key that none of the round's bin or before it lies below (the bins' edge, and a bin's width for what rounding does)
   HQ_DEV uint32_t edge() const {
     if (!values) return max(lo, hi - min(hi, ((uint32_t)bin << shift) | ((1u << shift) - 1)));
@@ -405,6 +417,17 @@ struct Search {
     return lo < hi;
   }
 };
+
+// How far below the largest value top-p's line can lie: the tokens from it on, n at most, have 1 - p of all weights (`sum`) or more, so
+// that it has w >= (1 - p) sum / n itself; and a little for roundings
+HQ_DEV float reach_of(const Weights &w, double top_p, double sum, double n) {
+  const double nats = log(n / ((1.0 - top_p) * sum)) + 0.01;
+  return (float)fmin(fmin(fmax(nats, 0.5), 40.0) * 92.332482616893656877 / w.slope, 3e38);
+}
+// and the lowest key that it can be
+HQ_DEV uint32_t floor_of(const Weights &w, float reach) {
+  return w.most < 3e38 ? max(key_of((float)w.most - reach), 9u) - 8u : 1u;
+}
 
 // the keys from `edge` on that `takes` says, up to kFew of them, in any order
 template <typename Source, typename F>
@@ -475,12 +498,20 @@ struct Kept {
 };
 constexpr uint32_t kAllTies = UINT32_MAX;
 
+// ties j = 0, 1, .. of a line with before + j each < target, of `equal`: at least one
+HQ_DEV uint32_t ties_of(const Line &p, uint32_t equal, double each, double target) {
+  const double room = (target - (double)p.before) / each;
+  uint32_t ties = room < (double)equal ? (uint32_t)ceil(room) : equal;
+  while (ties > 1 && !((double)p.before + (double)(ties - 1) * each < target)) ties--;
+  return max(ties, 1u);
+}
+
 // ---- the token ------------------------------------------------------------------------------------------------------
 // The first by index whose kept weights up to it are more than u times all.  Each wave sums its part, then the wave in whose part the
-// sum is reached goes through it again.
+// sum is reached goes through it again.  of_all: the source is a part of a row whose kept weights are that, `lead` of them before it.
 template <typename Source>
 HQ_DEV void draw(const Source &source, const Weights &w, const Settings &set, const Kept &kept, int32_t *token, float *chance,
-                 Scratch &m) {
+                 Scratch &m, double of_all = 0.0, double lead = 0.0) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const double edge = w.of(kept.t);  // the weight of one that is equal to t
   const uint32_t most = edge >= set.min_p || kept.t == w.top ? kept.ties : 0;
@@ -510,9 +541,10 @@ HQ_DEV void draw(const Source &source, const Weights &w, const Settings &set, co
     of_wave[i] = m.sums[i] + (double)min(m.ties[i], most - min(most, seen)) * edge;
     total += of_wave[i], seen += m.ties[i];
   }
+  if (of_all > 0.0) total = of_all;
   const double target = set.u * total;
   // the wave whose sum passes the target (none: the last that has any)
-  double before = 0.0, run = 0.0;
+  double before = lead, run = lead;
   uint32_t tied_before = 0;
   int which = -1;
   bool passed = false;
@@ -627,7 +659,7 @@ HQ_DEV bool answer(const Source &source, const Weights &w, const Settings &set, 
     return true;
   }
   Kept kept{lo, kAllTies};
-  const float range = (float)fmin(40.0 * 92.332482616893656877 / w.slope, 3e38);
+  const float range = range_of(w);
   bool cut = false;  // top-k or top-p leave something out
   if (set.top_k) {
     if (keys < (uint32_t)set.top_k && lo > 1) return false;
@@ -657,7 +689,8 @@ HQ_DEV bool answer(const Source &source, const Weights &w, const Settings &set, 
     }
     // (the first token is kept whatever its share)
     const double target = fmax(set.top_p * steps, 0.5);
-    Search f(w, max(kept.t, 1u), range);
+    const float reach = reach_of(w, set.top_p, steps / w.by, set.top_k ? set.top_k : set.vocab);
+    Search f(w, max(kept.t, floor_of(w, reach)), reach);
     f.template round<true>(source, target, m);
     // (the source ends before the line: all of it is kept)
     if (lo <= 1 || set.top_k || (double)(f.before + f.own) >= target) {
@@ -668,11 +701,7 @@ HQ_DEV bool answer(const Source &source, const Weights &w, const Settings &set, 
       }
       const Line p = line_of<true>(source, f, target, m);
       const uint32_t equal = p.key == kept.t ? min(p.equal, kept.ties) : p.equal;
-      // ties j = 0, 1, .. with before + j each < target
-      const double each = (double)w.steps(p.key), room = (target - (double)p.before) / each;
-      uint32_t ties = room < (double)equal ? (uint32_t)ceil(room) : equal;
-      while (ties > 1 && !((double)p.before + (double)(ties - 1) * each < target)) ties--;
-      kept = Kept{p.key, max(ties, 1u)};
+      kept = Kept{p.key, ties_of(p, equal, (double)w.steps(p.key), target)};
       cut = true;
     }
   }
@@ -701,14 +730,14 @@ HQ_DEV void none(const Sample &a, int64_t row) {
   }
 }
 
-template <bool WIDE, int MOST>
+template <bool WIDE>
 __global__ __launch_bounds__(kThreads) void row_kernel(Sample a, double by) {
   __shared__ Scratch m;
-  __shared__ uint32_t keys[MOST];
+  __shared__ uint32_t keys[kHeld];
   const int64_t row = blockIdx.x;
   const Settings set = settings_of(a, row);
   if (threadIdx.x < 64) m.roots[threadIdx.x] = kRoots[threadIdx.x];
-  const Row<WIDE> from((const float *)(a.logits + row * a.stride), a.vocab);
+  const Row<WIDE, 2> from((const float *)(a.logits + row * a.stride), a.vocab);
   uint32_t top = 0;
   from.sweep([&](const uint32_t k[4], int32_t i) {
     *(uint4 *)(keys + i) = make_uint4(k[0], k[1], k[2], k[3]);
@@ -724,10 +753,10 @@ __global__ __launch_bounds__(kThreads) void row_kernel(Sample a, double by) {
 
 // ---- a row over many blocks -----------------------------------------------------------------------------------------
 // What a wave of the first launch leaves: its largest key, its line (it handed on all from there on; 1: all that there are), how
-// many it handed on, and of each of its grains (grain 4 j + s at counts[s][j]), its weights' sum relative to its largest, and each grain's,
+// many it handed on, and of each of its grains (grain 4 j + s in counts[s][j & 1], byte 3 - j / 2), its weights' sum relative to its largest, and each grain's,
 // where nothing is cut off
 struct alignas(16) Note {
-  uint8_t counts[4][kBatch];
+  uint32_t counts[4][2];
   uint32_t top, line, handed;
   double sum, sums[kGrains];
 };
@@ -735,7 +764,19 @@ struct Pair {
   uint32_t key, at;  // (the index, and from bit 20 on how many of its grain come before it)
 };
 static_assert(kMostVocab <= 1 << 20 && kGrain <= 1 << 12, "a pair's index");
+// A row whose top-p reaches below what was handed on, spread over the whole vocabulary: the histogram over all of it, the keys of
+// the bin in which top-p's line lies (kBand at most), and the sums of the parts' weights before that bin
+constexpr int kParts = 16, kBand = 1024;
+struct alignas(16) Wide {
+  uint64_t weight[kBins];
+  uint32_t count[kBins], keys[kBand], at[kBand];
+  double sums[kParts], sum;
+  float reach;
+  uint32_t top, band;
+};
 struct Split {
+  Wide *wide;       // [rows]
+  uint32_t *rows;   // how many rows are wide, then which
   Note *notes;   // [rows][chunks]
   Pair *handed;  // [rows][chunks][kHand]
   int32_t chunks, lanes;  // waves a row; the lanes whose largest are to pass a wave's line
@@ -747,18 +788,23 @@ HQ_DEV void anew(float v[4]) { asm volatile("" : "+v"(v[0]), "+v"(v[1]), "+v"(v[
 template <bool WIDE>
 __global__ __launch_bounds__(256) void hand_kernel(Sample a, Split sp) {
   __shared__ double roots[64];
-  if (threadIdx.x < 64) roots[threadIdx.x] = kRoots[threadIdx.x];
-  __syncthreads();
   const int lane = threadIdx.x & 63;
   const int32_t chunk = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
   const int64_t row = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
-  if (chunk >= sp.chunks || row >= a.rows) return;
-  const Settings set = settings_of(a, row);
+  if (row >= a.rows) return;
   // the lane's logits: 4 of grain (4 j + s) chunks + chunk of the row, s its 16 lanes
   const int32_t stride = 4 * sp.chunks * kGrain, from = (lane >> 4) * (stride / 4) + chunk * kGrain + 4 * (lane & 15);
   float v[4 * kBatch];
-  load<WIDE>((const float *)(a.logits + row * a.stride), a.vocab, from, stride, a.vocab,
-             ((kGrains - 1) * sp.chunks + chunk + 1) * kGrain <= a.vocab, v);
+  if (chunk < sp.chunks)
+    load<WIDE, kBatch>((const float *)(a.logits + row * a.stride), a.vocab, from, stride, a.vocab,
+               ((kGrains - 1) * sp.chunks + chunk + 1) * kGrain <= a.vocab, v);
+  if (row == 0 && blockIdx.x == 0 && threadIdx.x == 0) sp.rows[0] = 0;
+  const Settings set = settings_of(a, row);
+  if (set.whole_sum()) {
+    if (threadIdx.x < 64) roots[threadIdx.x] = kRoots[threadIdx.x];
+    __syncthreads();
+  }
+  if (chunk >= sp.chunks) return;
   Note *note = sp.notes + row * sp.chunks + chunk;
   float mine = -__builtin_huge_valf();
 #pragma unroll
@@ -770,58 +816,48 @@ __global__ __launch_bounds__(256) void hand_kernel(Sample a, Split sp) {
   } else {
     // the line: so many lanes' largest are at or above it (the row's top_k, spread evenly, four times over)
     const int lanes = set.top_k == 1 ? 1 : set.top_k ? min(sp.lanes, 12 + 2 * (set.top_k / sp.chunks)) : sp.lanes;
-    uint32_t line = 0;
-    for (uint32_t bit = 1u << 31; bit; bit >>= 1) {
+    // (bits that all lanes' largest have in common are the line's)
+    const uint32_t apart = top ^ ~wave_most(~key);
+    uint32_t line = apart ? top & ~(UINT32_MAX >> __clz((int)apart)) : top;
+    for (uint32_t bit = apart ? 1u << 31 >> __clz((int)apart) : 0u; bit; bit >>= 1) {
       const int above = __popcll(__ballot(key >= (line | bit)));
       if (above >= lanes) line |= bit;
       if (above == lanes) break;
     }
-    int total = 0;
-    const auto count = [&](float least) {
-      total = 0;
-#pragma unroll
-      for (int i = 0; i < 4 * kBatch; i++) {
-        total += __popcll(__ballot(v[i] >= least));
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    };
     line = line < kLowest ? 1u : line;
-    float least = value_of(max(line, kLowest));
-    count(least);
+    // a bit for each of the lane's logits from the line on, the first the highest
+    const auto mask_of = [&](float least) {
+      uint32_t mask = 0;
+#pragma unroll
+      for (int i = 0; i < 4 * kBatch; i++) mask = 2 * mask + (v[i] >= least);
+      return mask;
+    };
+    uint32_t mask = mask_of(value_of(max(line, kLowest)));
+    uint32_t up_to = sum_up_to((uint32_t)__popc(mask)), total = from_lane(up_to, 63);
     if (total > kHand) {  // (equal ones by the dozen: those above them, if these are fewer)
       line = max(line, kLowest) + 1;
-      least = value_of(line);
-      if (line <= top) count(least);
-      if (line > top || total > kHand) line = UINT32_MAX, total = 0, least = __builtin_nanf("");
+      mask = line <= top ? mask_of(value_of(line)) : 0u;
+      up_to = sum_up_to((uint32_t)__popc(mask)), total = from_lane(up_to, 63);
+      if (line > top || total > kHand) line = UINT32_MAX, mask = 0, total = 0;
     }
-    Pair *to = sp.handed + (row * sp.chunks + chunk) * kHand;
-    uint32_t counts[2] = {0, 0};  // of the lane's s, a byte a step
-#pragma unroll
-    for (int j = 0; j < kBatch; j++) {
-      anew(v + 4 * j);
-      uint64_t in[4], any = 0;
-#pragma unroll
-      for (int c = 0; c < 4; c++) in[c] = __ballot(v[4 * j + c] >= least), any |= in[c];
-      if (!any) continue;
-      // before it in the step, and in its grain
-      uint32_t before = 0, grain = 0, all = 0;
-#pragma unroll
-      for (int c = 0; c < 4; c++) {
-        const uint32_t mine = (uint32_t)(in[c] >> (lane & 48)) & 0xffffu;
-        before += __popcll(in[c] & (((uint64_t)1 << lane) - 1));
-        grain += __popc(mine & ((1u << (lane & 15)) - 1));
-        all += __popc(mine);
-      }
-      counts[j >> 2] |= all << (8 * (j & 3));
-#pragma unroll
-      for (int c = 0; c < 4; c++)
-        if (v[4 * j + c] >= least) to[before++] = Pair{key_of(v[4 * j + c]), (uint32_t)(from + j * stride + c) | (grain++ << 20)};
-#pragma unroll
-      for (int c = 0; c < 4; c++) to += __popcll(in[c]);
-      __builtin_amdgcn_sched_barrier(0);
+    // how many of each step's 4, in bytes (steps 0, 2, 4, 6 and 1, 3, 5, 7 from the top), then of its grain's before the lane's
+    uint32_t pairs = mask - ((mask >> 1) & 0x55555555u);
+    pairs = (pairs & 0x33333333u) + ((pairs >> 2) & 0x33333333u);
+    const uint32_t even = (pairs >> 4) & 0x0f0f0f0fu, odd = pairs & 0x0f0f0f0fu;
+    const uint32_t even_to = sum_row(even), odd_to = sum_row(odd), even_from = even_to - even, odd_from = odd_to - odd;
+    const float *p = (const float *)(a.logits + row * a.stride);
+    const uint32_t mask_all = mask;
+    Pair *to = sp.handed + (row * sp.chunks + chunk) * kHand + (mask ? up_to - __popc(mask) : 0);
+    while (mask) {
+      const int bit = __clz((int)mask), j = bit >> 2;  // logit bit & 3 of step j
+      const int32_t i = from + j * stride + (bit & 3);
+      const uint32_t grain = ((j & 1 ? odd_from : even_from) >> (24 - 8 * (j >> 1))) & 0xffu;
+      const uint32_t step = mask_all >> (28 - 4 * j) & 15u;  // (the step's 4 bits)
+      *to++ = Pair{key_of(p[i]), (uint32_t)i | (grain + __popc(step >> (4 - (bit & 3)))) << 20};
+      mask &= ~(0x80000000u >> bit);
     }
-    if ((lane & 15) == 0) *(uint2 *)note->counts[lane >> 4] = make_uint2(counts[0], counts[1]);
-    if (lane == 0) note->top = top, note->line = line, note->handed = (uint32_t)total;
+    if ((lane & 15) == 15) *(uint2 *)note->counts[lane >> 4] = make_uint2(even_to, odd_to);
+    if (lane == 0) note->top = top, note->line = line, note->handed = total;
   }
   if (!set.whole_sum()) return;
   const double slope = slope_of(set.temperature), most = (double)value_of(top);
@@ -937,8 +973,8 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Sample a, Split sp, doub
     const uint4 q[2] = {*(const uint4 *)notes[c].counts[0], *(const uint4 *)notes[c].counts[2]};
     const uint32_t d[8] = {q[0].x, q[0].y, q[0].z, q[0].w, q[1].x, q[1].y, q[1].z, q[1].w};
 #pragma unroll
-    for (int g = 0; g < kGrains; g++)  // (grain 4 j + s is byte j & 3 of dword 2 s + j / 4)
-      s.offset[g * sp.chunks + c] = (uint16_t)((d[2 * (g & 3) + (g >> 4)] >> (8 * ((g >> 2) & 3))) & 0xffu);
+    for (int g = 0; g < kGrains; g++)
+      s.offset[g * sp.chunks + c] = (uint16_t)((d[2 * (g & 3) + ((g >> 2) & 1)] >> (24 - 8 * (g >> 3))) & 0xffu);
   }
   top = block_most(top, (uint32_t *)m.part);
   line = block_most(line, (uint32_t *)m.part + kWaves);
@@ -987,9 +1023,196 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Sample a, Split sp, doub
     const List<false> source(s.keys, s.at, n);
     if (answer(source, w, set, max(line, 1u), keys, sum, a.tokens + row, a.chance ? a.chance + row : nullptr, m)) return;
   }
+  if (!set.top_k && set.top_p < 1.0) {  // the wide kernels go on
+    Wide &wide = sp.wide[row];
+    wide.weight[threadIdx.x] = 0, wide.count[threadIdx.x] = 0;
+    if (threadIdx.x == 0) {
+      wide.sum = sum, wide.reach = reach_of(w, set.top_p, sum, a.vocab), wide.top = top, wide.band = 0;
+      sp.rows[1 + atomicAdd(&sp.rows[0], 1u)] = (uint32_t)row;
+    }
+    return;
+  }
   __syncthreads();
   const Row<WIDE> source((const float *)(a.logits + row * a.stride), a.vocab);
   answer(source, w, set, 1u, 0, sum, a.tokens + row, a.chance ? a.chance + row : nullptr, m);
+}
+
+// ---- wide rows: a part of one a block at a time ---------------------------------------------------------------------
+template <bool WIDE>
+using Part = Row<WIDE, 2>;
+// (parts begin on whole steps; the last may be short, or empty)
+HQ_DEV int32_t part_of(int32_t vocab) { return (vocab + kParts * kStep - 1) / (kParts * kStep) * kStep; }
+
+struct Item {  // a wide row's part
+  int64_t row;
+  int32_t part, from, n;
+};
+HQ_DEV Item item_of(const Sample &a, const Split &sp, uint32_t item) {
+  Item o;
+  o.row = sp.rows[1 + item / kParts], o.part = (int32_t)(item % kParts);
+  o.from = min(o.part * part_of(a.vocab), a.vocab);
+  o.n = min(part_of(a.vocab), a.vocab - o.from);
+  return o;
+}
+HQ_DEV Weights weights_of(const Wide &wide, const Settings &set, double by, const double *roots) {
+  return Weights{wide.top, (double)value_of(wide.top), slope_of(set.temperature), by, roots};
+}
+
+template <bool WIDE>
+__global__ __launch_bounds__(kThreads) void tally_kernel(Sample a, Split sp, double by) {
+  __shared__ Scratch m;
+  if (threadIdx.x < 64) m.roots[threadIdx.x] = kRoots[threadIdx.x];
+  const uint32_t items = sp.rows[0] * kParts;
+  for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const Item it = item_of(a, sp, item);
+    Wide &wide = sp.wide[it.row];
+    const Weights w = weights_of(wide, settings_of(a, it.row), by, m.roots);
+    Search f(w, floor_of(w, wide.reach), wide.reach);
+    f.template tally<true>(Part<WIDE>((const float *)(a.logits + it.row * a.stride), it.n, it.from), m);
+    if (m.count[threadIdx.x]) {
+      atomicAdd(&wide.count[threadIdx.x], m.count[threadIdx.x]);
+      atomicAdd((unsigned long long *)&wide.weight[threadIdx.x], (unsigned long long)m.weight[threadIdx.x]);
+    }
+  }
+}
+
+struct Band {
+  Scratch m;
+  uint32_t keys[kBand + kStep];
+  int32_t at[kBand + kStep];
+  uint32_t sorted[kBand];
+  int32_t sorted_at[kBand];
+  double starts[kParts + 1], sums[kParts];  // the band's kept weights before each part, the parts' before the band
+  uint32_t tied[kParts + 1];
+};
+
+// the search of a wide row, its first round done (the histogram is brought into m)
+HQ_DEV void find_in(const Wide &wide, Search &f, double target, Scratch &m) {
+  f.shift = max(22 - (int)__builtin_clz((f.hi - f.lo) | 1u), 0);
+  __syncthreads();
+  m.weight[threadIdx.x] = wide.weight[threadIdx.x], m.count[threadIdx.x] = wide.count[threadIdx.x];
+  __syncthreads();
+  f.template find<true>(target, m);
+}
+HQ_DEV double target_of(const Wide &wide, const Settings &set, double by) { return fmax(set.top_p * (wide.sum * by), 0.5); }
+
+// of a wide row the sum of each part's weights before the line's bin, and that bin's keys
+template <bool WIDE>
+__global__ __launch_bounds__(kThreads) void wide_kernel(Sample a, Split sp, double by) {
+  __shared__ Scratch m;
+  if (threadIdx.x < 64) m.roots[threadIdx.x] = kRoots[threadIdx.x];
+  const uint32_t items = sp.rows[0] * kParts;
+  for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const Item it = item_of(a, sp, item);
+    Wide &wide = sp.wide[it.row];
+    const Settings set = settings_of(a, it.row);
+    const Weights w = weights_of(wide, set, by, m.roots);
+    const float *p = (const float *)(a.logits + it.row * a.stride);
+    Search f(w, floor_of(w, wide.reach), wide.reach);
+    find_in(wide, f, target_of(wide, set, by), m);
+    const uint32_t edge = f.edge();
+    double sum = 0.0;
+    const Part<WIDE> source(p, it.n, it.from);
+    source.sweep([&](const uint32_t k[4], int32_t i) {
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        if (k[c] < edge || !f.inside(k[c])) continue;
+        const int bin = f.bin_of(k[c]);
+        if (bin < f.bin) {
+          const double x = w.of(k[c]);
+          sum += x >= set.min_p || k[c] == w.top ? x : 0.0;
+        } else if (bin == f.bin) {
+          const uint32_t to = atomicAdd(&wide.band, 1u);
+          if (to < kBand) wide.keys[to] = k[c], wide.at[to] = (uint32_t)source.index(i + c);
+        }
+      }
+      return true;
+    });
+    sum = block_sum(sum, (double *)m.part);
+    if (threadIdx.x == 0) wide.sums[it.part] = sum;
+  }
+}
+
+// of a wide row the line among its bin's keys, then the token
+template <bool WIDE>
+__global__ __launch_bounds__(kThreads) void end_kernel(Sample a, Split sp, double by) {
+  __shared__ Band b;
+  Scratch &m = b.m;
+  if (threadIdx.x < 64) m.roots[threadIdx.x] = kRoots[threadIdx.x];
+  if (blockIdx.x >= sp.rows[0]) return;
+  const int64_t row = sp.rows[1 + blockIdx.x];
+  const Wide &wide = sp.wide[row];
+  const Settings set = settings_of(a, row);
+  const Weights w = weights_of(wide, set, by, m.roots);
+  const float *p = (const float *)(a.logits + row * a.stride);
+  const double target = target_of(wide, set, by);
+  Search f(w, floor_of(w, wide.reach), wide.reach);
+  find_in(wide, f, target, m);
+  const int32_t n = (int32_t)wide.band;
+  for (int i = threadIdx.x; i < kBand + kStep; i += kThreads) {
+    b.keys[i] = i < n && i < kBand ? wide.keys[i] : 0u;
+    b.at[i] = i < n && i < kBand ? (int32_t)wide.at[i] : INT32_MAX;
+  }
+  if (threadIdx.x < kParts) b.sums[threadIdx.x] = wide.sums[threadIdx.x];
+  __syncthreads();
+  f.some = b.keys[0];  // (a bin of one key)
+  const bool fits = n <= kBand;  // (else equal ones by the thousand: the whole row again)
+  Line line;
+  if (fits) {
+    line = line_of<true>(List<false>(b.keys, b.at, n), f, target, m);
+  } else {
+    while (f.narrow() && f.template round<true>(Part<WIDE>(p, a.vocab), target, m)) {}
+    line = Line{f.some, f.before, f.equal};
+  }
+  Kept kept{line.key, ties_of(line, line.equal, (double)w.steps(line.key), target)};
+  int32_t from = 0, to = a.vocab;
+  double total = 0.0, lead = 0.0;
+  if (fits) {
+    // the bin's keys by index
+    if ((int)threadIdx.x < n) {
+      const int32_t at = b.at[threadIdx.x];
+      int rank = 0;
+#pragma unroll 2
+      for (int i = 0; i < n; i += 4) {
+        const int4 q = *(const int4 *)(b.at + i);
+        rank += (q.x < at) + (q.y < at) + (q.z < at) + (q.w < at);
+      }
+      b.sorted[rank] = b.keys[threadIdx.x], b.sorted_at[rank] = at;
+    }
+    __syncthreads();
+    const bool there = (int)threadIdx.x < n;
+    const uint32_t key = there ? b.sorted[threadIdx.x] : 0u;
+    uint32_t ties;
+    const uint32_t tied = sum_before((uint32_t)(there && key == kept.t), (uint32_t *)m.part, ties);
+    const double x = w.of(key);
+    const bool in = there && (key > kept.t || (key == kept.t && tied < kept.ties)) && (x >= set.min_p || key == w.top);
+    const double before = sum_before(in ? x : 0.0, m.sums, total);
+    // what comes before each part
+    const int32_t per = part_of(a.vocab);
+    const int part = there ? b.sorted_at[threadIdx.x] / per : kParts;
+    const int part_before = threadIdx.x && (int)threadIdx.x <= n ? b.sorted_at[threadIdx.x - 1] / per : -1;
+    if ((int)threadIdx.x <= n)
+      for (int q = part_before + 1; q <= part; q++) b.starts[q] = before, b.tied[q] = tied;
+    if (n == kBand && threadIdx.x == kThreads - 1)
+      for (int q = part + 1; q <= kParts; q++) b.starts[q] = total, b.tied[q] = ties;
+    __syncthreads();
+#pragma unroll 1
+    for (int q = 0; q < kParts; q++) total += b.sums[q];
+    // the part in which the sum is reached (none: the last that has any)
+    double run = 0.0;
+    int which = 0;
+    bool passed = false;
+#pragma unroll 1
+    for (int q = 0; q < kParts; q++) {
+      const double own = b.sums[q] + (b.starts[q + 1] - b.starts[q]);
+      if (!passed && own > 0.0) which = q, lead = run + b.starts[q], passed = run + b.sums[q] + b.starts[q + 1] > set.u * total;
+      run += b.sums[q];
+    }
+    from = min(which * per, a.vocab), to = min(from + per, a.vocab);
+    kept.ties -= min(b.tied[which], kept.ties);
+  }
+  __syncthreads();
+  draw(Part<WIDE>(p, to - from, from), w, set, kept, a.tokens + row, a.chance ? a.chance + row : nullptr, m, total, lead);
 }
 
 int32_t chunks_of(int32_t vocab) { return (int32_t)(((int64_t)vocab + kBatch * kStep - 1) / (kBatch * kStep)); }
@@ -999,7 +1222,7 @@ int64_t notes_bytes(int64_t rows, int32_t vocab) { return (rows * chunks_of(voca
 
 int64_t sample_work_bytes(int32_t rows, int32_t vocab) {
   if (vocab <= kHeld) return 0;
-  return notes_bytes(rows, vocab) + (int64_t)rows * chunks_of(vocab) * kHand * (int64_t)sizeof(Pair);
+  return notes_bytes(rows, vocab) + (int64_t)rows * (chunks_of(vocab) * kHand * (int64_t)sizeof(Pair) + (int64_t)sizeof(Wide) + 4) + 4;
 }
 
 hipError_t launch_sample(const Sample &a, hipStream_t s) {
@@ -1010,15 +1233,15 @@ hipError_t launch_sample(const Sample &a, hipStream_t s) {
   const double by = (double)((int64_t)1 << std::min(51, 62 - bits));
   const bool wide = a.vocab >= 4 && (uintptr_t)a.logits % 16 == 0 && (a.rows == 1 || a.stride % 16 == 0);
   if (a.vocab <= kHeld) {
-    const auto kernel = a.vocab <= kSmall ? wide ? row_kernel<true, kSmall> : row_kernel<false, kSmall>
-                                          : wide ? row_kernel<true, kHeld> : row_kernel<false, kHeld>;
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)a.rows), dim3(kThreads), 0, s, a, by);
+    hipLaunchKernelGGL(wide ? row_kernel<true> : row_kernel<false>, dim3((uint32_t)a.rows), dim3(kThreads), 0, s, a, by);
     return hipGetLastError();
   }
   Split sp{};
   sp.chunks = chunks_of(a.vocab);
   sp.notes = (Note *)a.work;
   sp.handed = (Pair *)(a.work + notes_bytes(a.rows, a.vocab));
+  sp.wide = (Wide *)(sp.handed + (int64_t)a.rows * sp.chunks * kHand);
+  sp.rows = (uint32_t *)(sp.wide + a.rows);
   // The lanes whose largest of 32 logits pass a wave's line, so that evenly spread logits hand on some 5500 of a row: of a share q of
   // the logits above the line, a lane has one with chance 1 - (1 - q)^32.  At most 48, which hand on 90 of a wave's 2048.
   const double share = std::min(1.0, 5500.0 / ((double)sp.chunks * kBatch * kStep));
@@ -1028,6 +1251,15 @@ hipError_t launch_sample(const Sample &a, hipStream_t s) {
   hipLaunchKernelGGL(wide ? hand_kernel<true> : hand_kernel<false>, grid, dim3(256), 0, s, a, sp);
   if (const hipError_t e = hipGetLastError()) return e;
   hipLaunchKernelGGL(wide ? join_kernel<true> : join_kernel<false>, dim3((uint32_t)a.rows), dim3(kThreads), 0, s, a, sp, by);
+  if (const hipError_t e = hipGetLastError()) return e;
+  if (!a.top_p) return hipSuccess;
+  // rows that top-p leaves wide: how many is known there; a block a compute unit, which ends at once where there are none
+  const dim3 blocks((uint32_t)std::min<int64_t>(cu_count(), (int64_t)a.rows * kParts));
+  hipLaunchKernelGGL(wide ? tally_kernel<true> : tally_kernel<false>, blocks, dim3(kThreads), 0, s, a, sp, by);
+  if (const hipError_t e = hipGetLastError()) return e;
+  hipLaunchKernelGGL(wide ? wide_kernel<true> : wide_kernel<false>, blocks, dim3(kThreads), 0, s, a, sp, by);
+  if (const hipError_t e = hipGetLastError()) return e;
+  hipLaunchKernelGGL(wide ? end_kernel<true> : end_kernel<false>, dim3((uint32_t)a.rows), dim3(kThreads), 0, s, a, sp, by);
   return hipGetLastError();
 }
 
