@@ -1004,7 +1004,8 @@ int32_t hq_adapters_ex(const hq_adapter *targets, int32_t count, const void *x, 
   if (count && !targets) return fail(HQ_ERR_NULL, "adapters: targets NULL");
   hq::Adapters a{};
   for (int32_t i = 0; i < count; i++)
-    if (targets[i].rows < 0) return fail(HQ_ERR_ARGUMENT, "adapters: target %d has %d rows", i, targets[i].rows);
+    if (targets[i].rows < 0 || targets[i].rows > (1 << 23))
+      return fail(HQ_ERR_ARGUMENT, "adapters: target %d has %d rows (at most 2^23)", i, targets[i].rows);
   if (count == 0 || batch->tokens == 0 || batch->sequences == 0) return HQ_OK;
   if (!batch->starts || !which || (adapters && !x)) return fail(HQ_ERR_NULL, "adapters: starts, which or x NULL");
   if (!aligned(batch->starts, 4) || !aligned(which, 4) || !aligned(scales, 4))

@@ -50,19 +50,20 @@ HQ_DEV int64_t vectors_of(const Cache &c, int32_t page, int32_t head) {
   return ((int64_t)page * c.heads + head) << c.shift;
 }
 
-// The sequence whose items a launch's `at`-th are, and which of them: sequence s has its tokens / 64 + 2 of the tokens / 64 +
-// 2 sequences items, from starts[s] / 64 + 2 s on (no sums over the sequences are needed), of which it may use fewer.  A lane a
-// sequence, 64 at a time; every lane of the wave calls it; s is -1 where no sequence has the item.
+// The sequence whose items (of 64 tokens, or 1 << SHIFT) a launch's `at`-th are, and which of them: sequence s has its tokens / 64 + 2
+// of the tokens / 64 + 2 sequences items, from starts[s] / 64 + 2 s on (no sums over the sequences are needed), of which it may
+// use fewer.  A lane a sequence, 64 at a time; every lane of the wave calls it; s is -1 where no sequence has the item.
 struct Place {
   int32_t s, rest;
   Sequence q;
 };
+template <int SHIFT = 6>
 HQ_DEV Place place_of(const Batch &b, int32_t at) {
   const int lane = threadIdx.x & 63;
   for (int32_t s0 = 0; s0 < b.sequences; s0 += 64) {
     const int32_t s = min(s0 + lane, b.sequences - 1);
     const Sequence q = sequence_of(b, s);
-    const int32_t first = (q.begin >> 6) + 2 * s, end = ((q.begin + q.count) >> 6) + 2 * s + 2;
+    const int32_t first = (q.begin >> SHIFT) + 2 * s, end = ((q.begin + q.count) >> SHIFT) + 2 * s + 2;
     const uint64_t in = __ballot(s0 + lane < b.sequences && at >= first && at < end);
     if (!in) continue;
     const int l = __ffsll((unsigned long long)in) - 1;

@@ -97,7 +97,7 @@ def adapters(pkg, L, less=0, **wrong):
 @pytest.mark.parametrize("wrong, code, words", [
     (dict(count=-1), 1, "count = -1"), (dict(count=9), 1, "count = 9"), (dict(rank=0), 1, "rank = 0"), (dict(rank=12), 1, "rank = 12"),
     (dict(rank=264), 1, "rank = 264"), (dict(n=0), 1, "n = 0"), (dict(n=48), 1, "n = 48"), (dict(adapters=-1), 1, "adapters = -1"),
-    (dict(form=0), 1, "form 0"), (dict(form=3), 1, "form 3"), (dict(rows=-1), 1, "-1 rows"), (dict(tokens=-1), 1, "tokens = -1"),
+    (dict(form=0), 1, "form 0"), (dict(form=3), 1, "form 3"), (dict(rows=-1), 1, "-1 rows"), (dict(rows=(1 << 23) + 1), 1, "rows"), (dict(tokens=-1), 1, "tokens = -1"),
     (dict(sequences=-1), 1, "sequences = -1"), (dict(tokens=(1 << 24) + 1), 1, "tokens = "), (dict(targets=None), 3, "targets"),
     (dict(batch=None), 3, "batch"), (dict(starts=None), 3, "starts"), (dict(which=None), 3, "which"), (dict(x=None), 3, "x NULL"),
     (dict(a=None), 3, "a, b or y"), (dict(b=None), 3, "a, b or y"), (dict(y=None), 3, "a, b or y"), (dict(x=4104), 2, "16-byte"),
