@@ -1040,7 +1040,8 @@ int32_t hq_adapters_ex(const hq_adapter *targets, int32_t count, const void *x, 
   a.x = (const char *)x, a.scales = (const float *)scales, a.which = (const int32_t *)which, a.work = (float *)work;
   a.x_stride = x_stride, a.n = n, a.rank = rank, a.adapters = adapters, a.bf16 = form == HQ_ADAPTER_BF16;
   const int32_t longest = batch->longest && batch->longest < batch->tokens ? batch->longest : batch->tokens;
-  const hq::Batch b{(const int32_t *)batch->starts, nullptr, nullptr, batch->sequences, batch->tokens, longest, 0};
+  // (its starts stand in for the lengths, which are not looked at)
+  const hq::Batch b{(const int32_t *)batch->starts, (const int32_t *)batch->starts, nullptr, batch->sequences, batch->tokens, longest, 0};
   return hip_status(hq::launch_adapters(a, b, stream_of(stream)), "adapters");
 }
 

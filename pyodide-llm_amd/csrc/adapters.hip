@@ -7,6 +7,7 @@
 // tokens and some rows a wave.  Factors widen to float32 exactly, so all that is rounded are float32's products and sums.
 // A token alone has a tile of its own: what such calls take is their factors' bytes.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.hpp"
 
@@ -17,7 +18,8 @@ namespace {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 16, kShift = 4;
-constexpr int kSplits = 8;   // blocks that share a tile's n values at most
+constexpr int kWaves = 8;      // of a block that makes low numbers: they share the n values,
+constexpr int kSplits = 4;     // as do so many blocks at most
 constexpr int kMostTiles = 4;  // tiles of 16 low numbers of a block
 
 // factors' numbers as float32
@@ -42,153 +44,215 @@ HQ_DEV Tokens tokens_of(const Adapters &a, const Batch &b, int32_t at) {
   return {p.q.begin + p.rest * kTile, min(max(rest, 0), kTile), (uint32_t)w < (uint32_t)a.adapters ? w : -1};
 }
 
-// Lane l of a tile: column (token) l & 15, and of every 32 values those from 8 (l / 16) on: instruction j of 8 takes value 8 (l / 16) + j
-// of both operands
+// A block takes its tokens' values 256 at a time, a token's kilobyte a wave's load (16 tokens' 128 bytes each reach 1.8 TB/s), into
+// LDS, from where wave w takes the w-th 32 of them.  Lane l has column (token) or row l & 15 and of the 32 those from 8 (l / 16)
+// on: instruction j of 8 takes value 8 (l / 16) + j of both operands.
+constexpr int kChunk = 32 * kWaves, kPitch = kChunk + 4;
+
 template <int BF16, int TILES>
-__global__ __launch_bounds__(256) void down_kernel(Adapters a, Batch b, int32_t splits) {
-  __shared__ f32x4 part[4][TILES][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, group = lane >> 4;
+__global__ __launch_bounds__(64 * kWaves) void down_kernel(Adapters a, Batch b, int32_t splits) {
+  __shared__ float held[2][kTile][kPitch];
+  __shared__ f32x4 part[kWaves][TILES][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, group = lane >> 4;
   const Tokens t = tokens_of(a, b, blockIdx.x);
   if (!t.count || t.adapter < 0) return;
   const int32_t numbers = a.count * a.rank, tile0 = blockIdx.z * TILES, split = blockIdx.y;
-  const int32_t steps = a.n >> 5, share = 4 * split + wave, shares = 4 * splits;
-  const int32_t from = (int32_t)((int64_t)steps * share / shares), to = (int32_t)((int64_t)steps * (share + 1) / shares);
-  const float *x = (const float *)(a.x + (t.first + min(col, t.count - 1)) * a.x_stride) + 8 * group;
+  const int32_t chunks = (a.n + kChunk - 1) / kChunk, from = chunks * split / splits, to = chunks * (split + 1) / splits;
   const char *f[TILES];
   f32x4 sum[TILES];
 #pragma unroll
   for (int i = 0; i < TILES; i++) {
     const int32_t q = min((tile0 + i) * kTile + col, numbers - 1), target = q / a.rank, r = q - target * a.rank;
-    f[i] = a.target[target].a + 2 * (((int64_t)t.adapter * a.rank + r) * a.n + 8 * group);
+    f[i] = a.target[target].a + 2 * (((int64_t)t.adapter * a.rank + r) * a.n + 8 * group + 32 * wave);
     sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-#pragma unroll 2
-  for (int32_t s = from; s < to; s++) {
-    const float4 x0 = *(const float4 *)(x + 32 * (int64_t)s), x1 = *(const float4 *)(x + 32 * (int64_t)s + 4);
-    uint4 h[TILES];
+  // the wave's two tokens (where there are fewer, the last), their values past the end the row's first
+  const float *x0 = (const float *)(a.x + (t.first + min(2 * wave, t.count - 1)) * a.x_stride);
+  const float *x1 = (const float *)(a.x + (t.first + min(2 * wave + 1, t.count - 1)) * a.x_stride);
+  float4 v0, v1;
+  uint4 h[TILES], next[TILES];
+  const auto begin = [&](int32_t c) {
+    const int32_t i = c * kChunk + 4 * lane, at = i < a.n ? i : 0;
+    v0 = *(const float4 *)(x0 + at), v1 = *(const float4 *)(x1 + at);
+    const int32_t mine = c * kChunk + 32 * wave < a.n ? c * kChunk : -32 * wave;
 #pragma unroll
-    for (int i = 0; i < TILES; i++) h[i] = *(const uint4 *)(f[i] + 64 * (int64_t)s);
-    const float e[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+    for (int k = 0; k < TILES; k++) next[k] = *(const uint4 *)(f[k] + 2 * (int64_t)mine);
+  };
+  if (from < to) begin(from);
+  for (int32_t c = from; c < to; c++) {
+    float (*x)[kPitch] = held[c & 1];
+    *(float4 *)&x[2 * wave][4 * lane] = v0, *(float4 *)&x[2 * wave + 1][4 * lane] = v1;
 #pragma unroll
-    for (int i = 0; i < TILES; i++) {
-      float m[8];
-      widen2<BF16>(h[i].x, m), widen2<BF16>(h[i].y, m + 2), widen2<BF16>(h[i].z, m + 4), widen2<BF16>(h[i].w, m + 6);
+    for (int k = 0; k < TILES; k++) h[k] = next[k];
+    if (c + 1 < to) begin(c + 1);
+    __syncthreads();  // (the other buffer is written when all have read this one: after the next of these)
+    if (c * kChunk + 32 * wave >= a.n) continue;
+    const float4 e0 = *(const float4 *)&x[col][32 * wave + 8 * group], e1 = *(const float4 *)&x[col][32 * wave + 8 * group + 4];
+    const float e[8] = {e0.x, e0.y, e0.z, e0.w, e1.x, e1.y, e1.z, e1.w};
+    float m[TILES][8];
 #pragma unroll
-      for (int j = 0; j < 8; j++) sum[i] = mfma(m[j], e[j], sum[i]);
-    }
+    for (int i = 0; i < TILES; i++)
+      widen2<BF16>(h[i].x, m[i]), widen2<BF16>(h[i].y, m[i] + 2), widen2<BF16>(h[i].z, m[i] + 4), widen2<BF16>(h[i].w, m[i] + 6);
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+#pragma unroll
+      for (int i = 0; i < TILES; i++) sum[i] = mfma(m[i][j], e[j], sum[i]);
   }
 #pragma unroll
   for (int i = 0; i < TILES; i++) part[wave][i][lane] = sum[i];
   __syncthreads();
   // low numbers 4 group .. + 3 of a tile, of token `col`
-  for (int i = wave; i < TILES; i += 4) {
+  for (int i = wave; i < TILES; i += kWaves) {
     const int32_t q = (tile0 + i) * kTile + 4 * group;
-    const f32x4 all = part[0][i][lane] + part[1][i][lane] + part[2][i][lane] + part[3][i][lane];
+    f32x4 all = part[0][i][lane];
+#pragma unroll
+    for (int k = 1; k < kWaves; k++) all += part[k][i][lane];
     if (q < numbers && col < t.count) *(f32x4 *)(a.work + ((int64_t)split * b.tokens + t.first + col) * numbers + q) = all;
   }
 }
 
-// ROWS: a wave's rows in tiles of 16
-template <int BF16, int RANK32, int ROWS>
+// the low numbers, or a row's factors, of a lane: of every 32 those from 8 group on, of 16 that are left from 4 group, of 8 from 2 group
+template <int WHOLE, typename T>
+struct Ranks {
+  T whole[WHOLE ? WHOLE : 1][8], half[4], quarter[2];
+};
+
+constexpr int kSpan = 64;  // rows at a time
+
+// WHOLE: 32s of the rank (8: up to so many); ROWS: a wave's rows in tiles of 16
+template <int BF16, int WHOLE, int ROWS>
 __global__ __launch_bounds__(256) void up_kernel(Adapters a, Batch b, int32_t splits) {
   const int lane = threadIdx.x & 63, col = lane & 15, group = lane >> 4;
   const Target &o = a.target[blockIdx.z];
   const int32_t row0 = __builtin_amdgcn_readfirstlane((blockIdx.y * 4 + (threadIdx.x >> 6)) * (kTile * ROWS));
-  if (blockIdx.y * (4 * kTile * ROWS) >= (uint32_t)o.rows) return;
+  if (row0 >= o.rows) return;
   const Tokens t = tokens_of(a, b, blockIdx.x);
-  if (!t.count || row0 >= o.rows) return;
-  const bool there = col < t.count;
+  if (!t.count) return;
+  __shared__ float turned[4][kTile][kSpan + 4];
+  float (*turn)[kSpan + 4] = turned[threadIdx.x >> 6];  // (the wave's own)
   const int64_t token = t.first + min(col, t.count - 1);
-  const float *from = o.from ? (const float *)(o.from + token * o.from_stride) : nullptr;
-  float *y = (float *)(o.y + token * o.y_stride);
-  // the token's low numbers times the adapter's scale: 8 group .. of every 32, 4 group .. of 16 and 2 group .. of 8 that are left
-  const bool adapted = t.adapter >= 0;
-  const int32_t numbers = a.count * a.rank, whole = a.rank >> 5;
-  float low[8 * RANK32], low16[4] = {0.f, 0.f, 0.f, 0.f}, low8[2] = {0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < 8 * RANK32; i++) low[i] = 0.f;
+  const bool adapted = t.adapter >= 0, halves = a.rank & 16, quarters = a.rank & 8;
+  const int32_t numbers = a.count * a.rank, whole = WHOLE < 8 ? WHOLE : a.rank >> 5;
+  Ranks<WHOLE, float> low = {};
   if (adapted) {
-    for (int32_t s = 0; s < splits; s++) {
+#pragma unroll
+    for (int s = 0; s < kSplits; s++) {
+      if (s >= splits) break;
       const float *w = a.work + ((int64_t)s * b.tokens + token) * numbers + blockIdx.z * a.rank;
 #pragma unroll
-      for (int i = 0; i < RANK32; i++) {
+      for (int i = 0; i < WHOLE; i++) {
         if (i >= whole) break;
         const float4 w0 = *(const float4 *)(w + 32 * i + 8 * group), w1 = *(const float4 *)(w + 32 * i + 8 * group + 4);
-        low[8 * i] += w0.x, low[8 * i + 1] += w0.y, low[8 * i + 2] += w0.z, low[8 * i + 3] += w0.w;
-        low[8 * i + 4] += w1.x, low[8 * i + 5] += w1.y, low[8 * i + 6] += w1.z, low[8 * i + 7] += w1.w;
+        const float e[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+        for (int j = 0; j < 8; j++) low.whole[i][j] += e[j];
       }
-      if (a.rank & 16) {
+      if (halves) {
         const float4 w0 = *(const float4 *)(w + 32 * whole + 4 * group);
-        low16[0] += w0.x, low16[1] += w0.y, low16[2] += w0.z, low16[3] += w0.w;
+        low.half[0] += w0.x, low.half[1] += w0.y, low.half[2] += w0.z, low.half[3] += w0.w;
       }
-      if (a.rank & 8) {
+      if (quarters) {
         const float2 w0 = *(const float2 *)(w + (a.rank & ~15) + 2 * group);
-        low8[0] += w0.x, low8[1] += w0.y;
+        low.quarter[0] += w0.x, low.quarter[1] += w0.y;
       }
     }
   }
   const float scale = adapted && a.scales ? a.scales[t.adapter] : 1.0f;
   const char *f = o.b + 2 * (int64_t)max(t.adapter, 0) * o.rows * a.rank;
-#pragma unroll 4
-  for (int r = 0; r < ROWS; r++) {
-    const int32_t tile = row0 + kTile * r, row = tile + 4 * group;
-    if (tile >= o.rows) break;
-    const bool full = tile + kTile <= o.rows;
-    float4 base = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (from) {
-      if (full) {
-        base = *(const float4 *)(from + row);
-      } else {
-        float *e = &base.x;
-#pragma unroll
-        for (int j = 0; j < 4; j++) e[j] = row + j < o.rows ? from[row + j] : 0.f;
-      }
-    }
+  // the product of 16 rows with these, the k-th 16 of a span
+  const auto multiply = [&](const uint4 *h, const uint2 &h16, uint32_t h8, int k) {
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < WHOLE; i++) {
+      if (WHOLE == 8 && i >= whole) break;
+      float e[8];
+      widen2<BF16>(h[i].x, e), widen2<BF16>(h[i].y, e + 2), widen2<BF16>(h[i].z, e + 4), widen2<BF16>(h[i].w, e + 6);
+#pragma unroll
+      for (int j = 0; j < 8; j++) sum = mfma(e[j], low.whole[i][j], sum);
+    }
+    if (halves) {
+      float e[4];
+      widen2<BF16>(h16.x, e), widen2<BF16>(h16.y, e + 2);
+#pragma unroll
+      for (int j = 0; j < 4; j++) sum = mfma(e[j], low.half[j], sum);
+    }
+    if (quarters) {
+      float e[2];
+      widen2<BF16>(h8, e);
+      sum = mfma(e[0], low.quarter[0], sum);
+      sum = mfma(e[1], low.quarter[1], sum);
+    }
+    *(f32x4 *)&turn[col][kTile * k + 4 * group] = sum;
+  };
+  const int32_t rows = min(o.rows - row0, kTile * ROWS);  // the wave's
+  // The products of 16 tokens and kSpan rows turn in LDS, so that a token's numbers are read and written 16 lanes (256 bytes) together
+  const int32_t first = lane >> 4, at4 = 4 * col;  // (tokens first, first + 4, ..)
+  for (int32_t r0 = 0; r0 < rows; r0 += kSpan) {
+    const int32_t row = row0 + r0 + at4;
+    const bool full = r0 + kSpan <= rows;
+    f32x4 base[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      base[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (!o.from) continue;
+      const float *from = (const float *)(o.from + (t.first + min(first + 4 * i, t.count - 1)) * o.from_stride);
+      if (full) {
+        base[i] = *(const f32x4 *)(from + row);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) base[i][j] = from[min(row + j, o.rows - 1)];
+      }
+    }
     if (adapted) {
-      const char *m = f + 2 * (int64_t)min(tile + col, o.rows - 1) * a.rank;
+      // (rows past the end are the last)
+      uint4 h[kSpan / kTile][WHOLE ? WHOLE : 1];
+      uint2 h16[kSpan / kTile];
+      uint32_t h8[kSpan / kTile];
 #pragma unroll
-      for (int i = 0; i < RANK32; i++) {
-        if (i >= whole) break;
-        const uint4 h = *(const uint4 *)(m + 64 * i + 16 * group);
-        float e[8];
-        widen2<BF16>(h.x, e), widen2<BF16>(h.y, e + 2), widen2<BF16>(h.z, e + 4), widen2<BF16>(h.w, e + 6);
+      for (int k = 0; k < kSpan / kTile; k++) {
+        const char *m = f + 2 * (int64_t)min(row0 + r0 + kTile * k + col, o.rows - 1) * a.rank;
+        h16[k] = make_uint2(0, 0), h8[k] = 0;
 #pragma unroll
-        for (int j = 0; j < 8; j++) sum = mfma(e[j], low[8 * i + j], sum);
+        for (int i = 0; i < WHOLE; i++)
+          if (WHOLE < 8 || i < whole) h[k][i] = *(const uint4 *)(m + 64 * i + 16 * group);
+        if (halves) h16[k] = *(const uint2 *)(m + 64 * whole + 8 * group);
+        if (quarters) h8[k] = *(const uint32_t *)(m + 2 * (a.rank & ~15) + 4 * group);
+        if (WHOLE == 8) multiply(h[k], h16[k], h8[k], k);
       }
-      if (a.rank & 16) {
-        const uint2 h = *(const uint2 *)(m + 64 * whole + 8 * group);
-        float e[4];
-        widen2<BF16>(h.x, e), widen2<BF16>(h.y, e + 2);
+      if (WHOLE < 8) {
 #pragma unroll
-        for (int j = 0; j < 4; j++) sum = mfma(e[j], low16[j], sum);
-      }
-      if (a.rank & 8) {
-        float e[2];
-        widen2<BF16>(*(const uint32_t *)(m + 2 * (a.rank & ~15) + 4 * group), e);
-        sum = mfma(e[0], low8[0], sum);
-        sum = mfma(e[1], low8[1], sum);
+        for (int k = 0; k < kSpan / kTile; k++) multiply(h[k], h16[k], h8[k], k);
       }
     }
-    const float4 out = make_float4(fmaf(scale, sum[0], base.x), fmaf(scale, sum[1], base.y), fmaf(scale, sum[2], base.z),
-                                   fmaf(scale, sum[3], base.w));
-    if (!there) continue;
-    if (full) {
-      *(float4 *)(y + row) = out;
-    } else {
-      const float e[4] = {out.x, out.y, out.z, out.w};
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int j = 0; j < 4; j++)
-        if (row + j < o.rows) y[row + j] = e[j];
+    for (int i = 0; i < 4; i++) {
+      const int32_t mine = first + 4 * i;
+      f32x4 sum = base[i];
+      if (adapted) {
+        const f32x4 add = *(const f32x4 *)&turn[mine][at4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) sum[j] = fmaf(scale, add[j], sum[j]);
+      }
+      if (mine >= t.count) continue;
+      float *y = (float *)(o.y + (int64_t)(t.first + mine) * o.y_stride);
+      if (full) {
+        *(f32x4 *)(y + row) = sum;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (row + j < o.rows) y[row + j] = sum[j];
+      }
     }
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
 int32_t tiles_of(int32_t count, int32_t rank) { return (count * rank + kTile - 1) / kTile; }
-// blocks that share a tile's n values: about two blocks a compute unit where there are few tokens
+// blocks that share a tile's n values: about one a compute unit where there are few tokens
 int32_t splits_of(int32_t count, int32_t rank, int32_t tokens) {
   const int64_t blocks = (int64_t)((tokens + kTile - 1) / kTile) * ((tiles_of(count, rank) + kMostTiles - 1) / kMostTiles);
-  return (int32_t)std::max<int64_t>(1, std::min<int64_t>(kSplits, 512 / std::max<int64_t>(blocks, 1)));
+  return (int32_t)std::max<int64_t>(1, std::min<int64_t>(kSplits, 256 / std::max<int64_t>(blocks, 1)));
 }
 
 }  // namespace
@@ -208,19 +272,28 @@ hipError_t launch_adapters(const Adapters &a, const Batch &b, hipStream_t s) {
     const dim3 grid(items, (uint32_t)splits, (uint32_t)((tiles + each - 1) / each));
     const auto kernel = a.bf16 ? each == 1 ? down_kernel<1, 1> : each == 2 ? down_kernel<1, 2> : each == 3 ? down_kernel<1, 3> : down_kernel<1, 4>
                                : each == 1 ? down_kernel<0, 1> : each == 2 ? down_kernel<0, 2> : each == 3 ? down_kernel<0, 3> : down_kernel<0, 4>;
-    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a, b, splits);
+    hipLaunchKernelGGL(kernel, grid, dim3(64 * kWaves), 0, s, a, b, splits);
     if (const hipError_t e = hipGetLastError()) return e;
   }
   if (rows == 0) return hipSuccess;
   const bool many = b.tokens >= 512;  // (a wave's rows: 256 where there are tokens enough, else 64)
   const int32_t block = 4 * kTile * (many ? 16 : 4);
   const dim3 grid(items, (uint32_t)((rows + block - 1) / block), (uint32_t)a.count);
-  const auto pick = [&](auto r2, auto r8) {
-    constexpr int R2 = decltype(r2)::value, R8 = decltype(r8)::value;
-    if (a.rank < 96) return a.bf16 ? many ? up_kernel<1, R2, 16> : up_kernel<1, R2, 4> : many ? up_kernel<0, R2, 16> : up_kernel<0, R2, 4>;
-    return a.bf16 ? many ? up_kernel<1, R8, 16> : up_kernel<1, R8, 4> : many ? up_kernel<0, R8, 16> : up_kernel<0, R8, 4>;
+  const int32_t whole = a.rank >> 5;
+  const auto launch = [&](auto bf16, auto most) {
+    constexpr int B = decltype(bf16)::value, W = decltype(most)::value;
+    const auto kernel = many ? up_kernel<B, W, 16> : up_kernel<B, W, 4>;
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a, b, splits);
   };
-  hipLaunchKernelGGL(pick(std::integral_constant<int, 2>(), std::integral_constant<int, 8>()), grid, dim3(256), 0, s, a, b, splits);
+  const auto pick = [&](auto bf16) {
+    using std::integral_constant;
+    if (whole == 0) launch(bf16, integral_constant<int, 0>());
+    else if (whole == 1) launch(bf16, integral_constant<int, 1>());
+    else if (whole == 2) launch(bf16, integral_constant<int, 2>());
+    else launch(bf16, integral_constant<int, 8>());
+  };
+  if (a.bf16) pick(std::integral_constant<int, 1>());
+  else pick(std::integral_constant<int, 0>());
   return hipGetLastError();
 }
 
