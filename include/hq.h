@@ -406,8 +406,8 @@ typedef struct hq_adapter {
 /* `count` projections (up to 8) of one input x (tokens x n float32, x_stride bytes apart) with the adapters of the batch's
  * sequences, after the products themselves: which (int32, device) is a sequence's adapter, none where it is outside 0 .. adapters
  * - 1; scales (float32, device; NULL: 1) an adapter's scale, the same for all projections; form HQ_ADAPTER_*.  Of the batch only
- * starts, sequences and tokens are read.  Rows that no sequence has are left alone.  Products and sums in float32, in an
- * order that depends on the sizes alone (tokens, projections, rank, n).  rank a multiple of 8 up to 256, n a multiple of 32, at most 2^23
+ * starts, sequences, tokens and longest are read.  Rows that no sequence has are left alone.  Products and sums in float32, in an
+ * order that depends on the sizes alone (tokens, longest, projections, rank, n).  rank a multiple of 8 up to 256, n a multiple of 32, at most 2^23
  * rows; a, b, x, from, y and their strides 16-byte aligned.  work: hq_adapters_work_bytes bytes (-1: bad
  * arguments), 256-byte aligned, of any content; calls that share it on one stream follow each other, on two they race. */
 enum { HQ_ADAPTER_F16 = 1, HQ_ADAPTER_BF16 = 2 };

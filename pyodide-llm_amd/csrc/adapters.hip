@@ -5,7 +5,7 @@
 // Two launches on the float32 matrix instructions (16 x 16 x 4): the low numbers of all projections, 16 tokens of a sequence a block whose
 // waves (and, for few tokens, blocks) share the n values and add what they have in a fixed order; then each projection's rows, 16
 // tokens and some rows a wave.  Factors widen to float32 exactly, so all that is rounded are float32's products and sums.
-// A token alone has a tile of its own: what such calls take is their factors' bytes.
+// Where the batch says that each sequence has one token, a tile would be empty but for one: tokens then have kernels of their own.
 #include <algorithm>
 #include <type_traits>
 
@@ -16,6 +16,7 @@ namespace hq {
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 16, kShift = 4;
 constexpr int kWaves = 8;      // of a block that makes low numbers: they share the n values,
@@ -49,6 +50,12 @@ HQ_DEV Tokens tokens_of(const Adapters &a, const Batch &b, int32_t at) {
 // on: instruction j of 8 takes value 8 (l / 16) + j of both operands.
 constexpr int kChunk = 32 * kWaves, kPitch = kChunk + 4;
 
+template <int TILES>
+struct Loads {  // of a chunk: the wave's two tokens' values, and its factors
+  f32x4 v0, v1;
+  u32x4 h[TILES];
+};
+
 template <int BF16, int TILES>
 __global__ __launch_bounds__(64 * kWaves) void down_kernel(Adapters a, Batch b, int32_t splits) {
   __shared__ float held[2][kTile][kPitch];
@@ -69,34 +76,42 @@ __global__ __launch_bounds__(64 * kWaves) void down_kernel(Adapters a, Batch b, 
   // the wave's two tokens (where there are fewer, the last), their values past the end the row's first
   const float *x0 = (const float *)(a.x + (t.first + min(2 * wave, t.count - 1)) * a.x_stride);
   const float *x1 = (const float *)(a.x + (t.first + min(2 * wave + 1, t.count - 1)) * a.x_stride);
-  float4 v0, v1;
-  uint4 h[TILES], next[TILES];
-  const auto begin = [&](int32_t c) {
-    const int32_t i = c * kChunk + 4 * lane, at = i < a.n ? i : 0;
-    v0 = *(const float4 *)(x0 + at), v1 = *(const float4 *)(x1 + at);
-    const int32_t mine = c * kChunk + 32 * wave < a.n ? c * kChunk : -32 * wave;
+  Loads<TILES> l0, l1, l2;  // three chunks on their way
+  const int32_t n = a.n;    // (a lambda that takes `a` keeps all of it in memory)
+  const auto begin = [&](Loads<TILES> &l, int32_t c) __attribute__((always_inline)) {
+    const int32_t i = c * kChunk + 4 * lane, at = i < n ? i : 0;
+    l.v0 = *(const f32x4 *)(x0 + at), l.v1 = *(const f32x4 *)(x1 + at);
+    const int32_t mine = c * kChunk + 32 * wave < n ? c * kChunk : -32 * wave;
 #pragma unroll
-    for (int k = 0; k < TILES; k++) next[k] = *(const uint4 *)(f[k] + 2 * (int64_t)mine);
+    for (int k = 0; k < TILES; k++) l.h[k] = *(const u32x4 *)(f[k] + 2 * (int64_t)mine);
   };
-  if (from < to) begin(from);
-  for (int32_t c = from; c < to; c++) {
+  const auto step = [&](Loads<TILES> &l, int32_t c) __attribute__((always_inline)) {
     float (*x)[kPitch] = held[c & 1];
-    *(float4 *)&x[2 * wave][4 * lane] = v0, *(float4 *)&x[2 * wave + 1][4 * lane] = v1;
-#pragma unroll
-    for (int k = 0; k < TILES; k++) h[k] = next[k];
-    if (c + 1 < to) begin(c + 1);
-    __syncthreads();  // (the other buffer is written when all have read this one: after the next of these)
-    if (c * kChunk + 32 * wave >= a.n) continue;
-    const float4 e0 = *(const float4 *)&x[col][32 * wave + 8 * group], e1 = *(const float4 *)&x[col][32 * wave + 8 * group + 4];
-    const float e[8] = {e0.x, e0.y, e0.z, e0.w, e1.x, e1.y, e1.z, e1.w};
+    *(f32x4 *)&x[2 * wave][4 * lane] = l.v0, *(f32x4 *)&x[2 * wave + 1][4 * lane] = l.v1;
     float m[TILES][8];
 #pragma unroll
     for (int i = 0; i < TILES; i++)
-      widen2<BF16>(h[i].x, m[i]), widen2<BF16>(h[i].y, m[i] + 2), widen2<BF16>(h[i].z, m[i] + 4), widen2<BF16>(h[i].w, m[i] + 6);
 #pragma unroll
-    for (int j = 0; j < 8; j++)
+      for (int j = 0; j < 4; j++) widen2<BF16>(l.h[i][j], m[i] + 2 * j);
+    if (c + 3 < to) begin(l, c + 3);
+    __syncthreads();  // (the other buffer is written when all have read this one: after the next of these)
+    const f32x4 e0 = *(const f32x4 *)&x[col][32 * wave + 8 * group], e1 = *(const f32x4 *)&x[col][32 * wave + 8 * group + 4];
+    if (c * kChunk + 32 * wave < n) {
 #pragma unroll
-      for (int i = 0; i < TILES; i++) sum[i] = mfma(m[i][j], e[j], sum[i]);
+      for (int j = 0; j < 8; j++)
+#pragma unroll
+        for (int i = 0; i < TILES; i++) sum[i] = mfma(m[i][j], j < 4 ? e0[j & 3] : e1[j & 3], sum[i]);
+    }
+  };
+  if (from < to) {
+    begin(l0, from);
+    if (from + 1 < to) begin(l1, from + 1);
+    if (from + 2 < to) begin(l2, from + 2);
+    for (int32_t c = from; c < to; c += 3) {
+      step(l0, c);
+      if (c + 1 < to) step(l1, c + 1);
+      if (c + 2 < to) step(l2, c + 2);
+    }
   }
 #pragma unroll
   for (int i = 0; i < TILES; i++) part[wave][i][lane] = sum[i];
@@ -248,6 +263,87 @@ __global__ __launch_bounds__(256) void up_kernel(Adapters a, Batch b, int32_t sp
   }
 }
 
+// ---- single tokens ----------------------------------------------------------------------------------------------------
+// A token's low numbers, four a wave; then its rows, one a thread: no tile waits for 15 tokens that are not there, and more waves
+// have loads on their way
+
+// the sequence that has row t (-1: none): the last whose first row is not behind t
+HQ_DEV int32_t sequence_at(const Batch &b, int32_t t) {
+  int32_t lo = 0, hi = b.sequences;
+  while (hi - lo > 1) {
+    const int32_t mid = (lo + hi) >> 1;
+    if (b.starts[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  return b.starts[lo] <= t && t < b.starts[lo + 1] ? lo : -1;
+}
+template <int BF16>
+HQ_DEV void widen8(const uint4 &v, float f[8]) {
+  widen2<BF16>(v.x, f), widen2<BF16>(v.y, f + 2), widen2<BF16>(v.z, f + 4), widen2<BF16>(v.w, f + 6);
+}
+
+constexpr int kEach = 4;  // low numbers of a wave
+
+template <int BF16>
+__global__ __launch_bounds__(256) void token_down_kernel(Adapters a, Batch b) {
+  const int32_t t = blockIdx.x, lane = threadIdx.x & 63;
+  const int32_t low = __builtin_amdgcn_readfirstlane((blockIdx.y * 4 + (threadIdx.x >> 6)) * kEach);
+  const int32_t s = sequence_at(b, t);
+  if (s < 0 || low >= a.count * a.rank) return;
+  const int32_t w = a.which[s];
+  if ((uint32_t)w >= (uint32_t)a.adapters) return;
+  const int32_t target = low / a.rank, r = low % a.rank;  // (rank is whole fours)
+  const float *x = (const float *)(a.x + t * a.x_stride);
+  const char *f = a.target[target].a + 2 * ((int64_t)w * a.rank + r) * a.n;
+  float sum[kEach] = {0.f, 0.f, 0.f, 0.f};
+  for (int32_t i = lane * 8; i < a.n; i += 512) {
+    const float4 x0 = *(const float4 *)(x + i), x1 = *(const float4 *)(x + i + 4);
+    const float e[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+#pragma unroll
+    for (int k = 0; k < kEach; k++) {
+      float m[8];
+      widen8<BF16>(*(const uint4 *)(f + 2 * ((int64_t)k * a.n + i)), m);
+#pragma unroll
+      for (int j = 0; j < 8; j++) sum[k] = fmaf(m[j], e[j], sum[k]);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kEach; k++) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum[k] += __shfl_xor(sum[k], o, 64);
+    if (lane == 0) a.work[(int64_t)t * a.count * a.rank + low + k] = sum[k];
+  }
+}
+
+template <int BF16>
+__global__ __launch_bounds__(256) void token_up_kernel(Adapters a, Batch b) {
+  __shared__ float low[256];
+  const int32_t t = blockIdx.x, row = blockIdx.y * 256 + threadIdx.x;
+  const Target &o = a.target[blockIdx.z];
+  if ((int32_t)blockIdx.y * 256 >= o.rows) return;
+  const int32_t s = sequence_at(b, t);
+  if (s < 0) return;
+  const int32_t w = a.which[s];
+  const bool adapted = (uint32_t)w < (uint32_t)a.adapters;
+  if (adapted && (int32_t)threadIdx.x < a.rank)
+    low[threadIdx.x] = a.work[((int64_t)t * a.count + blockIdx.z) * a.rank + threadIdx.x];
+  __syncthreads();
+  if (row >= o.rows) return;
+  float y = o.from ? ((const float *)(o.from + t * o.from_stride))[row] : 0.0f;
+  if (adapted) {
+    float sum = 0.0f;
+    const char *f = o.b + 2 * ((int64_t)w * o.rows + row) * a.rank;
+    for (int32_t i = 0; i < a.rank; i += 8) {
+      float m[8];
+      widen8<BF16>(*(const uint4 *)(f + 2 * i), m);
+#pragma unroll
+      for (int j = 0; j < 8; j++) sum = fmaf(m[j], low[i + j], sum);
+    }
+    y = fmaf(a.scales ? a.scales[w] : 1.0f, sum, y);
+  }
+  ((float *)(o.y + t * o.y_stride))[row] = y;
+}
+
 int32_t tiles_of(int32_t count, int32_t rank) { return (count * rank + kTile - 1) / kTile; }
 // blocks that share a tile's n values: about one a compute unit where there are few tokens
 int32_t splits_of(int32_t count, int32_t rank, int32_t tokens) {
@@ -265,6 +361,15 @@ hipError_t launch_adapters(const Adapters &a, const Batch &b, hipStream_t s) {
   if (b.tokens <= 0 || b.sequences <= 0 || a.count <= 0) return hipSuccess;
   int32_t rows = 0;
   for (int i = 0; i < a.count; i++) rows = std::max(rows, a.target[i].rows);
+  if (b.longest == 1) {  // 32 tokens of 3 projections, n 4096: 9.0 us of kernels, as tiles of one token 17.9
+    const dim3 down((uint32_t)b.tokens, (uint32_t)((a.count * a.rank + 4 * kEach - 1) / (4 * kEach)));
+    const auto lows = a.bf16 ? token_down_kernel<1> : token_down_kernel<0>;
+    if (a.adapters > 0) hipLaunchKernelGGL(lows, down, dim3(256), 0, s, a, b);
+    if (const hipError_t e = hipGetLastError()) return e;
+    const auto ups = a.bf16 ? token_up_kernel<1> : token_up_kernel<0>;
+    if (rows) hipLaunchKernelGGL(ups, dim3((uint32_t)b.tokens, (uint32_t)((rows + 255) / 256), (uint32_t)a.count), dim3(256), 0, s, a, b);
+    return hipGetLastError();
+  }
   const uint32_t items = (uint32_t)(b.tokens / kTile + 2 * b.sequences);
   const int32_t tiles = tiles_of(a.count, a.rank), splits = splits_of(a.count, a.rank, b.tokens);
   if (a.adapters > 0) {
@@ -276,13 +381,12 @@ hipError_t launch_adapters(const Adapters &a, const Batch &b, hipStream_t s) {
     if (const hipError_t e = hipGetLastError()) return e;
   }
   if (rows == 0) return hipSuccess;
-  const bool many = b.tokens >= 512;  // (a wave's rows: 256 where there are tokens enough, else 64)
-  const int32_t block = 4 * kTile * (many ? 16 : 4);
+  constexpr int32_t kRows = 4, block = 4 * kTile * kRows;  // a wave's rows are 64 (256 take a tenth longer: 30.0 us for 27.5 at 2048 tokens)
   const dim3 grid(items, (uint32_t)((rows + block - 1) / block), (uint32_t)a.count);
   const int32_t whole = a.rank >> 5;
   const auto launch = [&](auto bf16, auto most) {
     constexpr int B = decltype(bf16)::value, W = decltype(most)::value;
-    const auto kernel = many ? up_kernel<B, W, 16> : up_kernel<B, W, 4>;
+    const auto kernel = up_kernel<B, W, kRows>;
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a, b, splits);
   };
   const auto pick = [&](auto bf16) {
