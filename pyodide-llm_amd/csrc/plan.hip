@@ -2,7 +2,9 @@
 // from a stack, and for each token its sequence, position and slot; and pages given back to the stack.
 //
 // Two sums in a row: of the new tokens (a sequence's start), then of the pages that the tokens which fit need (where in the stack
-// its pages are).  One block takes the sequences 1024 at a time; a second launch finds each row's sequence in the starts.
+// its pages are).  One block takes the sequences 1024 at a time, and its threads the pages one each: a page's sequence is found in
+// the sums in LDS (a thread a sequence waits for a long prompt's pages one after another).  Rows find their sequence in the starts
+// alike, by the same block where all sequences are in LDS and the rows are a few a thread, else by a launch of its own.
 #include "paged.hpp"
 
 namespace hq {
@@ -10,6 +12,7 @@ namespace hq {
 namespace {
 
 constexpr int kThreads = 1024;
+constexpr int kFew = 4 * kThreads;  // rows that the planning block maps itself
 
 // the sum of v over the threads before this one, and over all in `total` (every thread calls it; `part`: 16 words of LDS)
 HQ_DEV int64_t sum_before(int64_t v, int64_t *part, int64_t &total) {
@@ -35,12 +38,33 @@ HQ_DEV int64_t sum_before(int64_t v, int64_t *part, int64_t &total) {
   return before + sum - v;
 }
 
+// what is written for row t: its sequence's number and its place there (s < 0: no sequence has it)
+HQ_DEV void map_row(const Plan &a, const Pool &p, int32_t t, int32_t s, int32_t position) {
+  if (a.sequence) a.sequence[t] = s;
+  if (a.position) a.position[t] = s < 0 ? -1 : position;
+  if (!a.slot) return;
+  const int32_t entry = position >> p.shift;
+  const int32_t page = s >= 0 && entry < a.width ? a.table[(int64_t)s * a.width + entry] : -1;
+  a.slot[t] = (uint32_t)page < (uint32_t)p.pages ? ((int64_t)page << p.shift) + (position & ((1 << p.shift) - 1)) : -1;
+}
+
+// the last of 1024 rising numbers that is not more than t (the first is not)
+HQ_DEV int32_t last_up_to(const int32_t *numbers, int32_t t) {
+  int32_t at = 0;
+#pragma unroll
+  for (int32_t step = kThreads / 2; step > 0; step >>= 1)
+    if (numbers[at + step] <= t) at += step;
+  return at;
+}
+
+template <bool MAP>
 __global__ __launch_bounds__(kThreads) void plan_kernel(Plan a, Pool p) {
   __shared__ int64_t part[kThreads / 64];
+  __shared__ int32_t begins[kThreads], firsts[kThreads], row_begins[MAP ? kThreads : 1], helds[MAP ? kThreads : 1];
   const int32_t count = min(max(*p.count, 0), p.pages), mask = (1 << p.shift) - 1;
   int64_t rows = 0, pages = 0;  // of the sequences before these
-  for (int32_t s0 = 0; s0 < a.sequences; s0 += kThreads) {
-    const int32_t s = s0 + threadIdx.x;
+  for (int64_t s0 = 0; s0 < a.sequences; s0 += kThreads) {
+    const int64_t s = s0 + threadIdx.x;
     const bool live = s < a.sequences;
     const int32_t held = live ? min(max(a.held[s], 0), kMostPositions) : 0;
     const int32_t asked = live ? min(max(a.fresh[s], 0), a.tokens) : 0;
@@ -48,47 +72,57 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(Plan a, Pool p) {
     const int64_t before = rows + sum_before(asked, part, total);
     rows += total;
     const int32_t begin = (int32_t)min(before, (int64_t)a.tokens), fresh = min(asked, a.tokens - begin);
-    // the pages that begin among the new positions, as far as the table goes
+    // the pages that begin among the new positions, as far as the table goes (all sequences' together: fewer than their tokens
+    // and one each)
     const int32_t length = held + fresh, first = min((held + mask) >> p.shift, a.width);
     const int32_t wanted = min((length + mask) >> p.shift, a.width) - first;
-    const int64_t at = pages + sum_before(wanted, part, total);
+    begins[threadIdx.x] = (int32_t)sum_before(wanted, part, total);
+    firsts[threadIdx.x] = first;
+    if (MAP) row_begins[threadIdx.x] = live ? begin : INT32_MAX, helds[threadIdx.x] = held;
+    if (live) {
+      a.starts[s] = begin;
+      a.lengths[s] = length;
+    }
+    __syncthreads();
+    for (int32_t i = threadIdx.x; i < (int32_t)total; i += kThreads) {
+      const int32_t w = last_up_to(begins, i);
+      const int64_t at = pages + i;
+      a.table[(s0 + w) * a.width + firsts[w] + (i - begins[w])] = at < count ? p.free[count - 1 - at] : -1;
+    }
     pages += total;
-    if (!live) continue;
-    a.starts[s] = begin;
-    a.lengths[s] = length;
-#pragma clang loop unroll(disable) vectorize(disable)
-    for (int32_t i = 0; i < wanted; i++)
-      a.table[(int64_t)s * a.width + first + i] = at + i < count ? p.free[count - 1 - (at + i)] : -1;
   }
+  const int32_t end = (int32_t)min(rows, (int64_t)a.tokens);
   if (threadIdx.x == 0) {
-    a.starts[a.sequences] = (int32_t)min(rows, (int64_t)a.tokens);
+    a.starts[a.sequences] = end;
     *p.left = (int32_t)max(count - pages, (int64_t)0);
     if (p.missing) *p.missing = (int32_t)max(pages - count, (int64_t)0);
   }
+  if (!MAP) return;
+  __syncthreads();  // (the table's entries are written)
+  for (int32_t t = threadIdx.x; t < a.tokens; t += kThreads) {
+    const int32_t s = t < end ? last_up_to(row_begins, t) : -1;
+    map_row(a, p, t, s, s < 0 ? 0 : helds[s] + (t - row_begins[s]));
+  }
 }
 
-__global__ __launch_bounds__(256) void map_kernel(Plan a, Pool p) {
-  const int32_t t = blockIdx.x * 256 + threadIdx.x;
+// A block has 1024 of the starts in LDS, evenly; what lies between two of them is searched in memory.
+__global__ __launch_bounds__(kThreads) void map_kernel(Plan a, Pool p) {
+  __shared__ int32_t begins[kThreads];
+  const int32_t each = (a.sequences - 1) / kThreads + 1, mine = threadIdx.x * each;
+  const int32_t end = a.starts[a.sequences];
+  begins[threadIdx.x] = (int32_t)threadIdx.x < (a.sequences - 1) / each + (a.sequences > 0) ? a.starts[mine] : INT32_MAX;
+  __syncthreads();
+  const int32_t t = blockIdx.x * kThreads + threadIdx.x;
   if (t >= a.tokens) return;
-  // the last sequence whose first token is not behind t
-  int32_t lo = 0, hi = a.sequences;  // starts[lo] <= t < starts[hi], where any sequence has t
+  if (t >= end) return map_row(a, p, t, -1, 0);
+  // starts[lo] <= t < starts[hi]
+  int32_t lo = last_up_to(begins, t) * each, hi = lo + min(each, a.sequences - lo);
   while (hi - lo > 1) {
     const int32_t mid = (lo + hi) >> 1;
     if (a.starts[mid] <= t) lo = mid;
     else hi = mid;
   }
-  if (t >= a.starts[a.sequences]) {  // (no sequence has it)
-    if (a.sequence) a.sequence[t] = -1;
-    if (a.position) a.position[t] = -1;
-    if (a.slot) a.slot[t] = -1;
-    return;
-  }
-  const int32_t position = a.lengths[lo] - (a.starts[lo + 1] - t), entry = position >> p.shift;
-  if (a.sequence) a.sequence[t] = lo;
-  if (a.position) a.position[t] = position;
-  if (!a.slot) return;
-  const int32_t page = entry < a.width ? a.table[(int64_t)lo * a.width + entry] : -1;
-  a.slot[t] = (uint32_t)page < (uint32_t)p.pages ? ((int64_t)page << p.shift) + (position & ((1 << p.shift) - 1)) : -1;
+  map_row(a, p, t, lo, a.lengths[lo] - (a.starts[lo + 1] - t));
 }
 
 __global__ __launch_bounds__(kThreads) void give_kernel(Pool p, int32_t *table, int32_t sequences, int32_t width, const int32_t *from,
@@ -117,10 +151,15 @@ __global__ __launch_bounds__(kThreads) void give_kernel(Pool p, int32_t *table, 
 }  // namespace
 
 hipError_t launch_plan(const Plan &a, const Pool &p, hipStream_t s) {
-  hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kThreads), 0, s, a, p);
+  const bool map = a.tokens > 0 && (a.sequence || a.position || a.slot);
+  if (map && a.sequences <= kThreads && a.tokens <= kFew) {
+    hipLaunchKernelGGL(plan_kernel<true>, dim3(1), dim3(kThreads), 0, s, a, p);
+    return hipGetLastError();
+  }
+  hipLaunchKernelGGL(plan_kernel<false>, dim3(1), dim3(kThreads), 0, s, a, p);
   if (const hipError_t e = hipGetLastError()) return e;
-  if (a.tokens <= 0 || (!a.sequence && !a.position && !a.slot)) return hipSuccess;
-  hipLaunchKernelGGL(map_kernel, dim3((uint32_t)((a.tokens + 255) / 256)), dim3(256), 0, s, a, p);
+  if (!map) return hipSuccess;
+  hipLaunchKernelGGL(map_kernel, dim3((uint32_t)(((int64_t)a.tokens + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, a, p);
   return hipGetLastError();
 }
 
