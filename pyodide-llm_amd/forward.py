@@ -56,6 +56,7 @@ class Forward:
         self.caches = [Cache(*(t.data_ptr() for t in held), FORMS[form], pages, page, s.kv_heads, s.head_size)
                        for held in self.held]
         self.work = torch.empty(0, dtype=torch.uint8, device=device)
+        self.older = []  # (workspaces that were too small: a captured step may still use them)
         self.normed = None  # (a norm's values beside the readied ones: where adapters read them)
         half = torch.arange(0, s.head_size, 2, device=device, dtype=torch.float64) / s.head_size
         angles = torch.arange(width * page, device=device, dtype=torch.float64)[:, None] * theta ** -half
@@ -177,6 +178,11 @@ class Forward:
             check(needed)
         needed = max(needed, extra)
         if self.work.numel() < needed:
+            if torch.cuda.is_current_stream_capturing():
+                raise ValueError("refused: a step is captured after one of its sizes has run, which makes its workspace")
+            if self.work.numel():
+                self.older.append(self.work)
+                needed = max(needed, 2 * self.work.numel())
             self.work = torch.empty(needed, dtype=torch.uint8, device=x.device)
         if at is None:
             # a token's position: its place before its sequence's end
@@ -187,6 +193,8 @@ class Forward:
         normed, both = None, {}
         if adapters is not None:
             if self.normed is None:
+                if torch.cuda.is_current_stream_capturing():
+                    raise ValueError("refused: a step with adapters is captured after one has run, which makes its buffer")
                 self.normed = torch.empty_like(self.y)
             normed = self.normed[:count]
             both = dict(y=normed, both=True)

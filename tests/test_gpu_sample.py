@@ -123,7 +123,7 @@ def test_settings(pkg, vocab):
 @pytest.mark.parametrize("setting", SETTINGS, ids=str)
 @pytest.mark.parametrize("shape", ["flat", "steep", "rising", "falling", "whole", "same", "two", "hidden", "huge", "around 0", "far apart", "one bin"])
 def test_shapes(pkg, setting, shape):
-    """logits of every kind of crowd: evenly spread, in order, with ties by the thousand, mostly hidden, of extreme sizes"""
+    """logits of every kind of crowd: evenly spread, in order, with ties by the thousand, mostly hidden, of extreme sizes (to infinity)"""
     rng = np.random.default_rng(len(shape))
     for vocab in (3000, 40001):
         x = rng.standard_normal((2, vocab))
@@ -276,4 +276,51 @@ def test_replayed(pkg):
         token, chance = rows.got()
         for r in range(6):
             want, share = model(l[r], u=u[r], **{k: v[r] for k, v in each.items()})
+            assert token[r] == want and near(chance[r], share)
+
+
+@pytest.mark.parametrize("vocab", [8192, 8193, 10239, 10241, 40000])
+@pytest.mark.parametrize("pad", [0, 3])
+def test_many_flat_rows(pkg, vocab, pad):
+    """rows whose top-p takes in most words, or words of one weight by the thousand, among ordinary ones"""
+    rng = np.random.default_rng(vocab)
+    kinds = [lambda: 0.05 * rng.standard_normal(vocab), lambda: language(rng, 1, vocab)[0], lambda: np.zeros(vocab),
+             lambda: np.where(rng.random(vocab) < 0.5, -np.inf, 1.0), lambda: np.round(rng.standard_normal(vocab)),
+             lambda: np.linspace(3, -3, vocab), lambda: np.full(vocab, -np.inf)]
+    n = 5 * len(kinds)
+    rows = Rows(pkg, np.stack([kinds[r % len(kinds)]() for r in range(n)]), pad)
+    each = dict(temperature=rng.choice([0.9, 1.0, 3.0, 40.0], n), top_k=rng.choice([0, 0, 0, vocab // 2, vocab + 5], n),
+                top_p=rng.choice([0.3, 0.9, 0.999, 1 - 2.0 ** -24], n), min_p=rng.choice([0.0, 0.0, 0.5], n))
+    for u in (rng.random(n).astype(F), np.zeros(n, F), np.full(n, 1 - 2.0 ** -24, F)):
+        rows.check(u, **each)
+
+
+def test_flat_rows_replayed(pkg):
+    """a captured call whose rows are flat in one replay and not in the next, two graphs on one workspace in turn"""
+    import torch
+    rng = np.random.default_rng(17)
+    rows = Rows(pkg, 0.1 * rng.standard_normal((4, 20000)))
+    stream, graphs = torch.cuda.Stream(), []
+    rows.check(rng.random(4).astype(F), stream=stream.cuda_stream, top_p=0.95)
+    held = rows.held
+    lib = pkg.library()
+    at = [None if t is None else t.data_ptr() for t in held]
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            assert lib.hq_sample_ex(rows.tokens.data_ptr(), rows.chance.data_ptr(), rows.logits, *at, 4, rows.vocab, rows.stride,
+                                    rows.work.data_ptr(), rows.need, stream.cuda_stream) == 0
+        graphs.append(g)
+    for i in range(6):
+        l = (0.1 * rng.standard_normal((4, 20000))).astype(F) if i % 3 else language(rng, 4, 20000)
+        u = rng.random(4).astype(F)
+        rows.memory[:4 * 20000].copy_(torch.from_numpy(l).view(-1))
+        held[0].copy_(torch.from_numpy(u))
+        rows.work[:rows.need].fill_(0xff)
+        rows.tokens[:4].fill_(-5)
+        torch.cuda.synchronize()
+        graphs[i % 2].replay()
+        token, chance = rows.got()
+        for r in range(4):
+            want, share = model(l[r], u=u[r], top_p=0.95)
             assert token[r] == want and near(chance[r], share)

@@ -187,6 +187,41 @@ def test_steps_replayed(pkg, kind):
         assert torch.equal(eager.lengths, other.lengths) and torch.equal(eager.table, other.table)
 
 
+def test_a_captured_step_keeps_its_workspace(pkg):
+    """a longer step of many more tokens, which needs a larger workspace, runs between a captured step's replays; a step whose
+    workspace is not there is not captured"""
+    import torch
+    from pyodide_llm_amd import checkpoint, forward, serve
+    rng = np.random.default_rng(6)
+    ck = checkpoint.Checkpoint(checkpoints.write((256, 768, 1, 4, 2, 300, 64), "int8", rng)[0])
+    n = 2
+    serves = [serve.Serving(forward.Forward(ck, tokens=1500, sequences=n, pages=64, width=30, page=64)) for _ in range(2)]
+    ids = torch.from_numpy(rng.integers(0, 300, 1400).astype(np.int32)).cuda()
+    ones, u = torch.ones(n, dtype=torch.int32, device="cuda"), torch.rand(n, device="cuda")
+    stream, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    eager, other = serves
+    for serving in serves:
+        serving.step(ids[:2], ones, u, 1)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=stream):
+        other.step(ids[:2], ones, u, 1)
+    was = other.forward.work.numel()
+    for many in (900, 1, 200):
+        eager.step(ids[:2], ones, u, 1)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(eager.scores, other.scores) and torch.equal(eager.tokens, other.tokens)
+        fresh = torch.tensor([many, 100], dtype=torch.int32, device="cuda")
+        for serving in serves:
+            serving.step(ids[:many + 100], fresh, u, max(many, 100))
+        if many == 900:
+            held = [torch.full((was,), 255, dtype=torch.uint8, device="cuda") for _ in range(4)]  # (what a freed one would become)
+        assert torch.equal(eager.scores, other.scores)
+        serves[0].finish(torch.ones(n, dtype=torch.bool, device="cuda"))
+        serves[1].finish(torch.ones(n, dtype=torch.bool, device="cuda"))
+    assert other.forward.work.numel() > was and all((t == 255).all() for t in held)
+
+
 def test_refused(pkg):
     import torch
     from pyodide_llm_amd import adapters, checkpoint, forward, serve
