@@ -1018,12 +1018,12 @@ int32_t hq_adapters_ex(const hq_adapter *targets, int32_t count, const void *x, 
     const hq_adapter &t = targets[i];
     if (t.rows == 0) continue;
     if (!t.y || (adapters && (!t.a || !t.b))) return fail(HQ_ERR_NULL, "adapters: target %d's a, b or y NULL", i);
-    if (!aligned(t.a, 16) || !aligned(t.b, 16) || !aligned(t.from, 16) || !aligned(t.y, 16))
-      return fail(HQ_ERR_ALIGNMENT, "adapters: target %d's a, b, from or y not 16-byte aligned", i);
+    if (!aligned(t.a, 16) || !aligned(t.b, 16) || !aligned(t.from, 4) || !aligned(t.y, 4))
+      return fail(HQ_ERR_ALIGNMENT, "adapters: target %d's a or b not 16-byte, or from or y not 4-byte aligned", i);
     if (batch->tokens > 1) {
       const int64_t row = 4 * (int64_t)t.rows;
-      if (t.y_stride < 0 || t.y_stride % 16 || (t.from && (t.from_stride < 0 || t.from_stride % 16)))
-        return fail(HQ_ERR_ALIGNMENT, "adapters: target %d's stride is not a multiple of 16", i);
+      if (t.y_stride < 0 || t.y_stride % 4 || (t.from && (t.from_stride < 0 || t.from_stride % 4)))
+        return fail(HQ_ERR_ALIGNMENT, "adapters: target %d's stride is not a multiple of 4", i);
       if (t.y_stride < row || (t.from && t.from_stride < row))
         return fail(HQ_ERR_ARGUMENT, "adapters: target %d's strides %d and %d, a token's row takes %lld", i, t.from_stride,
                     t.y_stride, (long long)row);

@@ -203,11 +203,12 @@ __global__ __launch_bounds__(256) void up_kernel(Adapters a, Batch b, int32_t sp
     *(f32x4 *)&turn[col][kTile * k + 4 * group] = sum;
   };
   const int32_t rows = min(o.rows - row0, kTile * ROWS);  // the wave's
+  const bool aligned = !(((uintptr_t)o.from | (uintptr_t)o.y | (uint32_t)o.from_stride | (uint32_t)o.y_stride) & 15);  // (else a float at a time)
   // The products of 16 tokens and kSpan rows turn in LDS, so that a token's numbers are read and written 16 lanes (256 bytes) together
   const int32_t first = lane >> 4, at4 = 4 * col;  // (tokens first, first + 4, ..)
   for (int32_t r0 = 0; r0 < rows; r0 += kSpan) {
     const int32_t row = row0 + r0 + at4;
-    const bool full = r0 + kSpan <= rows;
+    const bool full = r0 + kSpan <= rows && aligned;
     f32x4 base[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {

@@ -37,7 +37,7 @@ def wanted(x, a, b, base, scales, which, starts):
 
 class Call:
     def __init__(self, pkg, rng, form, n, rows, rank, adapters, fresh, which, with_scales=True, with_from=True, in_place=False, pad=0,
-                 spread=1.0, x_size=1.0, behind=2, longest=None):
+                 spread=1.0, x_size=1.0, behind=2, longest=None, packed=False):
         import torch
         self.pkg, self.form, self.n, self.rank, self.adapters = pkg, form, n, rank, adapters
         self.starts = np.concatenate([[0], np.cumsum(fresh)]).astype(np.int32)
@@ -54,7 +54,7 @@ class Call:
         self.da, self.db = [t.cuda() for t, _ in self.a], [t.cuda() for t, _ in self.b]
         self.dfrom, self.dy = [], []
         for base, r in zip(self.base, rows):
-            room = -r % 4 + pad
+            room = 0 if packed else -r % 4 + pad
             y = np.full((self.tokens, r + room), -9, F)
             if with_from:
                 given = y.copy()
@@ -246,3 +246,14 @@ def test_a_batch_that_contradicts_itself(pkg):
             call.run()
             torch.cuda.synchronize()
             assert (call.dy[0][:, 40:] == -9).all() and (call.work[call.need:] == 0xff).all()
+
+
+@pytest.mark.parametrize("fresh", [[1] * 7, [40, 1, 0, 17]], ids=str)
+@pytest.mark.parametrize("more", [dict(), dict(in_place=True), dict(with_from=False)], ids=str)
+def test_rows_that_are_not_whole_fours(pkg, fresh, more):
+    """rows back to back, so that tokens begin on any float; in a batch of single tokens and in tiles"""
+    rng = np.random.default_rng(len(fresh))
+    for rows in ((97,), (1, 2, 3), (64, 130), (515,)):
+        call = Call(pkg, rng, "bf16", 96, rows, 16, 3, fresh, (np.arange(len(fresh)) % 4).tolist(), packed=True, **more)
+        call.run()
+        call.check()

@@ -101,9 +101,9 @@ def adapters(pkg, L, less=0, **wrong):
     (dict(sequences=-1), 1, "sequences = -1"), (dict(tokens=(1 << 24) + 1), 1, "tokens = "), (dict(targets=None), 3, "targets"),
     (dict(batch=None), 3, "batch"), (dict(starts=None), 3, "starts"), (dict(which=None), 3, "which"), (dict(x=None), 3, "x NULL"),
     (dict(a=None), 3, "a, b or y"), (dict(b=None), 3, "a, b or y"), (dict(y=None), 3, "a, b or y"), (dict(x=4104), 2, "16-byte"),
-    (dict(a=4104), 2, "16-byte"), (dict(b=4098), 2, "16-byte"), (dict(from_=4100), 2, "16-byte"), (dict(y=4100), 2, "16-byte"),
+    (dict(a=4104), 2, "16-byte"), (dict(b=4098), 2, "16-byte"), (dict(from_=4098), 2, "4-byte"), (dict(y=4098), 2, "4-byte"),
     (dict(starts=4098), 2, "4-byte"), (dict(which=4098), 2, "4-byte"), (dict(scales=4097), 2, "4-byte"), (dict(x_stride=520), 2, "x_stride"),
-    (dict(x_stride=-512), 2, "x_stride"), (dict(x_stride=496), 1, "x_stride"), (dict(y_stride=260), 2, "stride"),
+    (dict(x_stride=-512), 2, "x_stride"), (dict(x_stride=496), 1, "x_stride"), (dict(y_stride=258), 2, "stride"),
     (dict(from_stride=-256), 2, "stride"), (dict(y_stride=240), 1, "strides"), (dict(from_stride=240), 1, "strides"),
     (dict(less=1), 1, "workspace"), (dict(work=None), 3, "work"), (dict(work=4224), 2, "256-byte"),
 ])
