@@ -409,7 +409,8 @@ typedef struct hq_adapter {
  * starts, sequences, tokens and longest are read.  Rows that no sequence has are left alone.  Products and sums in float32, in an
  * order that depends on the sizes alone (tokens, longest, projections, rank, n).  rank a multiple of 8 up to 256, n a multiple of 32, at most 2^23
  * rows; a, b, x and its stride 16-byte aligned, from, y and their strides 4 (16 is faster).  work: hq_adapters_work_bytes bytes (-1: bad
- * arguments), 256-byte aligned, of any content; calls that share it on one stream follow each other, on two they race. */
+ * arguments; never less for more projections, a larger rank or more tokens, so that one made for the most covers every smaller call),
+ * 256-byte aligned, of any content; calls that share it on one stream follow each other, on two they race. */
 enum { HQ_ADAPTER_F16 = 1, HQ_ADAPTER_BF16 = 2 };
 int64_t hq_adapters_work_bytes(int32_t count, int32_t rank, int32_t tokens);
 int32_t hq_adapters_ex(const hq_adapter *targets, int32_t count, const void *x, int32_t x_stride, int32_t n, int32_t rank,

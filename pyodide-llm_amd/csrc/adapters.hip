@@ -357,8 +357,13 @@ int32_t splits_of(int32_t count, int32_t rank, int32_t tokens) {
 
 }  // namespace
 
+// What is written is `splits` times tokens x count x rank numbers, which may be more for fewer projections or tokens, as these are
+// split more often.  A call may run fewer projections than it states (those without rows are left out), and a workspace is kept for
+// steps of many sizes: this grows with each of the three and covers them all.  A launch that splits has 256 blocks at most, and a
+// block writes at most 16 tokens' 16 kMostTiles numbers.
 int64_t adapters_work_bytes(int32_t count, int32_t rank, int32_t tokens) {
-  return 4 * (int64_t)splits_of(count, rank, tokens) * tokens * count * rank;
+  const int64_t numbers = (int64_t)tokens * count * rank, split = 256 * kTile * kTile * kMostTiles;
+  return 4 * std::max(numbers, std::min(kSplits * numbers, split));
 }
 
 hipError_t launch_adapters(const Adapters &a, const Batch &b, hipStream_t s) {

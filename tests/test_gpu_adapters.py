@@ -257,3 +257,12 @@ def test_rows_that_are_not_whole_fours(pkg, fresh, more):
         call = Call(pkg, rng, "bf16", 96, rows, 16, 3, fresh, (np.arange(len(fresh)) % 4).tolist(), packed=True, **more)
         call.run()
         call.check()
+
+
+@pytest.mark.parametrize("rows, rank, fresh", [((0, 64), 64, [1040]), ((0, 70, 0), 64, [1000]), ((33, 0, 0), 256, [100, 28]),
+                                               ((0, 50), 16, [1, 1, 1]), ((0, 0), 8, [20])], ids=str)
+def test_projections_without_rows(pkg, rows, rank, fresh):
+    """they are left out, and the rest, whose values more blocks may share, stays within the call's workspace"""
+    call = Call(pkg, np.random.default_rng(rank), "bf16", 1056, rows, rank, 2, fresh, [1, 0, 1][:len(fresh)])
+    call.run()
+    call.check()

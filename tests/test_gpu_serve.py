@@ -222,6 +222,24 @@ def test_a_captured_step_keeps_its_workspace(pkg):
     assert other.forward.work.numel() > was and all((t == 255).all() for t in held)
 
 
+def test_adapters_of_one_and_two_projections(pkg):
+    """a model whose attention needs less workspace than the adapters, of which one or two projections may need more than three"""
+    import torch
+    from pyodide_llm_amd import adapters, checkpoint, forward
+    rng = np.random.default_rng(7)
+    ck = checkpoint.Checkpoint(checkpoints.write((512, 768, 1, 8, 8, 100, 64), "int8", rng)[0])
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    x = torch.from_numpy(rng.standard_normal((128, 512)).astype(F)).cuda()
+    for names in (("wo", "w2"), ("w1", "w3"), ("wq", "wk", "wv", "w1")):
+        model = watched(forward)(ck, tokens=128, sequences=4, pages=8, width=2, page=16)
+        model.starts = np.arange(0, 129, 32)
+        held = adapters.Adapters(factors(torch, ck, rng, 1, 256, names, torch.float16))
+        batch = pkg.cache.Batch(4096, 4096, 4096, 4, 128, 32, 2)
+        assert pkg.library().hq_attention_work_bytes(model.caches[0], batch, 8) < pkg.library().hq_adapters_work_bytes(2, 256, 128)
+        model.step(x.clone(), ints(*model.starts), ints(32, 32, 32, 32), ints(*range(8)).view(4, 2), 32, None, held, ints(0, 0, 0, 0))
+        assert model.seen == 4 * len(names)
+
+
 def test_refused(pkg):
     import torch
     from pyodide_llm_amd import adapters, checkpoint, forward, serve

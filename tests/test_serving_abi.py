@@ -121,6 +121,24 @@ def test_adapters_work_bytes(L):
         assert L.hq_adapters_work_bytes(*wrong) == -1 and L.hq_last_error() == 1
 
 
+def test_adapters_work_covers_what_is_written(L):
+    """a launch writes splits x tokens x projections x rank numbers (up to 4 splits where its blocks, of 16 tokens and 64 numbers, are
+    so many times within 256), of the projections that have rows: fewer than the call states, which may be split more often; so the
+    bytes grow with projections, ranks and tokens"""
+    def written(count, rank, tokens):
+        blocks = max(1, -(-tokens // 16) * -(-(-(-count * rank // 16)) // 4))
+        return 4 * max(1, min(4, 256 // blocks)) * tokens * count * rank
+    tokens = [0, 1, 7, 16, 17, 100, 250, 256, 335, 336, 337, 447, 448, 449, 671, 672, 673, 1000, 1024, 1040, 1365, 2048, 4095, 4097, 1 << 24]
+    for rank in (8, 16, 24, 64, 72, 128, 136, 256):
+        for count in range(1, 9):
+            need = [L.hq_adapters_work_bytes(count, rank, t) for t in tokens]
+            assert need == sorted(need)
+            for t, n in zip(tokens, need):
+                assert n >= max(written(c, rank, t) for c in range(1, count + 1)), (count, rank, t)
+                assert n >= L.hq_adapters_work_bytes(count, rank - 8, t) or rank == 8
+                assert n >= L.hq_adapters_work_bytes(count - 1, rank, t)
+
+
 def sample(L, tokens=4096, chance=4096, logits=4096, u=4096, temperature=4096, top_k=4096, top_p=4096, min_p=4096, rows=2, vocab=100,
            stride=400, less=0, **more):
     need = L.hq_sample_work_bytes(2, 100)
