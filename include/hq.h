@@ -408,7 +408,7 @@ typedef struct hq_adapter {
  * - 1; scales (float32, device; NULL: 1) an adapter's scale, the same for all projections; form HQ_ADAPTER_*.  Of the batch only
  * starts, sequences, tokens and longest are read.  Rows that no sequence has are left alone.  Products and sums in float32, in an
  * order that depends on the sizes alone (tokens, longest, projections, rank, n).  rank a multiple of 8 up to 256, n a multiple of 32, at most 2^23
- * rows; a, b, x and its stride 16-byte aligned, from, y and their strides 4 (16 is faster).  work: hq_adapters_work_bytes bytes (-1: bad
+ * rows, and 2^21 sequences where longest is not 1; a, b, x and its stride 16-byte aligned, from, y and their strides 4 (16 is faster).  work: hq_adapters_work_bytes bytes (-1: bad
  * arguments; never less for more projections, a larger rank or more tokens, so that one made for the most covers every smaller call),
  * 256-byte aligned, of any content; calls that share it on one stream follow each other, on two they race. */
 enum { HQ_ADAPTER_F16 = 1, HQ_ADAPTER_BF16 = 2 };

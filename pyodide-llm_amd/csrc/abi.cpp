@@ -423,7 +423,7 @@ int32_t batch_sizes_of(const char *who, const hq_batch *batch, int32_t shift, bo
   if (table && ((int64_t)batch->width << shift) > 1 << 30)
     return fail(HQ_ERR_ARGUMENT, "%s: a table of %d pages of %d positions", who, batch->width, 1 << shift);
   if (batch->tokens > (1 << 24)) return fail(HQ_ERR_ARGUMENT, "%s: tokens = %d", who, batch->tokens);
-  // (a launch of two blocks a sequence stays below 2^32 threads)
+  // (a launch of two blocks of 256 a sequence stays below 2^32 threads)
   if (batch->sequences > (1 << 22)) return fail(HQ_ERR_ARGUMENT, "%s: sequences = %d", who, batch->sequences);
   return HQ_OK;
 }
@@ -1007,6 +1007,10 @@ int32_t hq_adapters_ex(const hq_adapter *targets, int32_t count, const void *x, 
     if (targets[i].rows < 0 || targets[i].rows > (1 << 23))
       return fail(HQ_ERR_ARGUMENT, "adapters: target %d has %d rows (at most 2^23)", i, targets[i].rows);
   if (count == 0 || batch->tokens == 0 || batch->sequences == 0) return HQ_OK;
+  const int32_t longest = batch->longest && batch->longest < batch->tokens ? batch->longest : batch->tokens;
+  // (tiles have two blocks of 512 a sequence)
+  if (longest != 1 && batch->sequences > (1 << 21))
+    return fail(HQ_ERR_ARGUMENT, "adapters: sequences = %d (at most 2^21 of more than a token each)", batch->sequences);
   if (!batch->starts || !which || (adapters && !x)) return fail(HQ_ERR_NULL, "adapters: starts, which or x NULL");
   if (!aligned(batch->starts, 4) || !aligned(which, 4) || !aligned(scales, 4))
     return fail(HQ_ERR_ALIGNMENT, "adapters: starts, which or scales not 4-byte aligned");
@@ -1039,7 +1043,6 @@ int32_t hq_adapters_ex(const hq_adapter *targets, int32_t count, const void *x, 
   if (int32_t st = ensure_device()) return st;
   a.x = (const char *)x, a.scales = (const float *)scales, a.which = (const int32_t *)which, a.work = (float *)work;
   a.x_stride = x_stride, a.n = n, a.rank = rank, a.adapters = adapters, a.bf16 = form == HQ_ADAPTER_BF16;
-  const int32_t longest = batch->longest && batch->longest < batch->tokens ? batch->longest : batch->tokens;
   // (its starts stand in for the lengths, which are not looked at)
   const hq::Batch b{(const int32_t *)batch->starts, (const int32_t *)batch->starts, nullptr, batch->sequences, batch->tokens, longest, 0};
   return hip_status(hq::launch_adapters(a, b, stream_of(stream)), "adapters");

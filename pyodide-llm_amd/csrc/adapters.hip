@@ -289,8 +289,8 @@ HQ_DEV void widen8(const uint4 &v, float f[8]) {
 constexpr int kEach = 4;  // low numbers of a wave
 
 template <int BF16>
-__global__ __launch_bounds__(256) void token_down_kernel(Adapters a, Batch b) {
-  const int32_t t = blockIdx.x, lane = threadIdx.x & 63;
+__global__ __launch_bounds__(256) void token_down_kernel(Adapters a, Batch b, int32_t first) {
+  const int32_t t = first + blockIdx.x, lane = threadIdx.x & 63;
   const int32_t low = __builtin_amdgcn_readfirstlane((blockIdx.y * 4 + (threadIdx.x >> 6)) * kEach);
   const int32_t s = sequence_at(b, t);
   if (s < 0 || low >= a.count * a.rank) return;
@@ -320,9 +320,9 @@ __global__ __launch_bounds__(256) void token_down_kernel(Adapters a, Batch b) {
 }
 
 template <int BF16>
-__global__ __launch_bounds__(256) void token_up_kernel(Adapters a, Batch b) {
+__global__ __launch_bounds__(256) void token_up_kernel(Adapters a, Batch b, int32_t first) {
   __shared__ float low[256];
-  const int32_t t = blockIdx.x, row = blockIdx.y * 256 + threadIdx.x;
+  const int32_t t = first + blockIdx.x, row = blockIdx.y * 256 + threadIdx.x;
   const Target &o = a.target[blockIdx.z];
   if ((int32_t)blockIdx.y * 256 >= o.rows) return;
   const int32_t s = sequence_at(b, t);
@@ -371,13 +371,19 @@ hipError_t launch_adapters(const Adapters &a, const Batch &b, hipStream_t s) {
   int32_t rows = 0;
   for (int i = 0; i < a.count; i++) rows = std::max(rows, a.target[i].rows);
   if (b.longest == 1) {  // 32 tokens of 3 projections, n 4096: 9.0 us of kernels, as tiles of one token 17.9
-    const dim3 down((uint32_t)b.tokens, (uint32_t)((a.count * a.rank + 4 * kEach - 1) / (4 * kEach)));
     const auto lows = a.bf16 ? token_down_kernel<1> : token_down_kernel<0>;
-    if (a.adapters > 0) hipLaunchKernelGGL(lows, down, dim3(256), 0, s, a, b);
-    if (const hipError_t e = hipGetLastError()) return e;
     const auto ups = a.bf16 ? token_up_kernel<1> : token_up_kernel<0>;
-    if (rows) hipLaunchKernelGGL(ups, dim3((uint32_t)b.tokens, (uint32_t)((rows + 255) / 256), (uint32_t)a.count), dim3(256), 0, s, a, b);
-    return hipGetLastError();
+    constexpr int32_t kTokens = 1 << 23;  // of a launch (a dimension has fewer than 2^32 threads)
+    for (int32_t first = 0; first < b.tokens; first += kTokens) {
+      const uint32_t tokens = (uint32_t)std::min(b.tokens - first, kTokens);
+      const dim3 down(tokens, (uint32_t)((a.count * a.rank + 4 * kEach - 1) / (4 * kEach)));
+      if (a.adapters > 0) hipLaunchKernelGGL(lows, down, dim3(256), 0, s, a, b, first);
+      if (const hipError_t e = hipGetLastError()) return e;
+      const dim3 up(tokens, (uint32_t)((rows + 255) / 256), (uint32_t)a.count);
+      if (rows) hipLaunchKernelGGL(ups, up, dim3(256), 0, s, a, b, first);
+      if (const hipError_t e = hipGetLastError()) return e;
+    }
+    return hipSuccess;
   }
   const uint32_t items = (uint32_t)(b.tokens / kTile + 2 * b.sequences);
   const int32_t tiles = tiles_of(a.count, a.rank), splits = splits_of(a.count, a.rank, b.tokens);

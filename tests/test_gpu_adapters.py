@@ -266,3 +266,28 @@ def test_projections_without_rows(pkg, rows, rank, fresh):
     call = Call(pkg, np.random.default_rng(rank), "bf16", 1056, rows, rank, 2, fresh, [1, 0, 1][:len(fresh)])
     call.run()
     call.check()
+
+
+def test_most_tokens(pkg):
+    """2^24 rows by the kernels of single tokens, whatever a sequence has of them"""
+    import torch
+    lib, n, rank, rows, tokens = pkg.library(), 32, 8, 4, 1 << 24
+    a, b = torch.randn(1, rank, n, device="cuda").half(), torch.randn(1, rows, rank, device="cuda").half()
+    x, y = torch.randn(tokens, n, device="cuda"), torch.full((tokens, rows), -9.0, device="cuda")
+    starts, which = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([0, tokens - 3], [0]))
+    need = lib.hq_adapters_work_bytes(1, rank, tokens)
+    work = torch.empty(need, dtype=torch.uint8, device="cuda")
+    target = pkg.adapters.Target(a.data_ptr(), b.data_ptr(), None, y.data_ptr(), rows, 4 * rows, 4 * rows)
+    batch = pkg.cache.Batch(starts.data_ptr(), None, None, 1, tokens, 1, 0)
+    torch.cuda.synchronize()
+    assert lib.hq_adapters_ex(target, 1, x.data_ptr(), 4 * n, n, rank, 1, 1, None, which.data_ptr(), batch, work.data_ptr(), need,
+                              torch.cuda.current_stream().cuda_stream) == 0, lib.hq_last_error_message()
+    assert (y[-3:] == -9).all()
+    a, b = a[0].double(), b[0].double()
+    for first in range(0, tokens - 3, 1 << 21):
+        rows_of = slice(first, min(first + (1 << 21), tokens - 3))
+        e = x[rows_of].double()
+        want = (e @ a.t()) @ b.t()
+        # (n and rank products and sums, a rounding each at most)
+        far = (e.abs() @ a.abs().t()) @ b.abs().t() * (n + rank + 3) * 2.0 ** -24
+        assert ((y[rows_of].double() - want).abs() <= far).all(), first

@@ -121,6 +121,14 @@ def test_adapters_work_bytes(L):
         assert L.hq_adapters_work_bytes(*wrong) == -1 and L.hq_last_error() == 1
 
 
+def test_adapters_of_many_sequences(pkg, L):
+    """more than 2^21 sequences of several tokens are refused before a launch that has no room for their blocks"""
+    for longest in (0, 2):
+        refused(L, adapters(pkg, L, sequences=(1 << 21) + 1, longest=longest), 1, "sequences = 2097153")
+    for more in (dict(sequences=1 << 21), dict(sequences=1 << 22, longest=1)):
+        refused(L, adapters(pkg, L, x=4104, **more), 2, "16-byte")  # (the sequences pass)
+
+
 def test_adapters_work_covers_what_is_written(L):
     """a launch writes splits x tokens x projections x rank numbers (up to 4 splits where its blocks, of 16 tokens and 64 numbers, are
     so many times within 256), of the projections that have rows: fewer than the call states, which may be split more often; so the
