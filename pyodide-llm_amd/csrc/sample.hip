@@ -113,7 +113,8 @@ HQ_DEV Settings settings_of(const Sample &a, int64_t row) {
   o.top_k = a.top_k && top_k > 0 && top_k < a.vocab ? top_k : 0;
   o.top_p = a.top_p ? top_p : 1.0f;
   o.min_p = a.min_p && min_p > 0.0f ? fminf(min_p, 1.0f) : 0.0f;
-  o.u = u >= 0.0f ? u : 0.0f;
+  // (1 or more: no sum passes it, so that the last that has any is drawn; times 1 a sum in another order might, by a rounding)
+  o.u = u >= 1.0f ? __builtin_huge_val() : u >= 0.0f ? u : 0.0f;
   if (!(o.temperature > 0.0)) o.temperature = 1.0, o.top_k = 1;
   return o;
 }

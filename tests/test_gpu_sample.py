@@ -324,3 +324,17 @@ def test_flat_rows_replayed(pkg):
         for r in range(4):
             want, share = model(l[r], u=u[r], top_p=0.95)
             assert token[r] == want and near(chance[r], share)
+
+
+@pytest.mark.parametrize("vocab", [50, 700, 8192, 8193, 32000, 128256])
+@pytest.mark.parametrize("settings", [dict(), dict(top_p=0.9999), dict(min_p=1e-30), dict(top_k=40), dict(top_k=600, top_p=0.99999)], ids=str)
+def test_the_last_kept_one_where_it_weighs_nothing(pkg, vocab, settings):
+    """numbers of 1 and more draw the last kept token, also where what lies behind the heavy ones is less than a sum's rounding"""
+    rng = np.random.default_rng(vocab + len(settings))
+    l = language(rng, 24, vocab) * 2
+    l[:, vocab // 3:] -= 60  # (10^-26 of the first third's)
+    rows = Rows(pkg, l)
+    for u in (1.0, 7.0, 3e38, np.inf):
+        rows.check(u, **settings)
+        rows.check(u, temperature=0.9, **settings)
+    rows.check(np.where(np.arange(24) % 2, F(1.0), F(0.3)), **settings)
