@@ -338,3 +338,24 @@ def test_the_last_kept_one_where_it_weighs_nothing(pkg, vocab, settings):
         rows.check(u, **settings)
         rows.check(u, temperature=0.9, **settings)
     rows.check(np.where(np.arange(24) % 2, F(1.0), F(0.3)), **settings)
+
+
+@pytest.mark.parametrize("u", [1.0, 7.0])
+def test_the_last_kept_one_where_parts_keep_none(pkg, u):
+    """flat rows whose top-p is spread over blocks, the last of which have words at the line that are not kept, and nothing else that is:
+    the last kept one lies before them"""
+    rng = np.random.default_rng(17)
+    vocab, part = 128256, 8192
+    for behind in (1, 3):
+        l = rng.random((16, vocab)).astype(F)
+        few = (16 - behind) * part
+        l[:, few:] = -9
+        for r in range(16):
+            w = np.sort(np.exp(l[r].astype(np.float64)))[::-1]
+            line = np.log(w[np.searchsorted(np.cumsum(w), 0.9 * w.sum())])
+            for q in range(16 - behind, 16):
+                l[r, q * part + rng.choice(5000, 3, replace=False)] = line - 2e-4 - 1e-4 * rng.random(3)
+        rows = Rows(pkg, l)
+        rows.check(u, top_p=0.9)
+        assert (rows.got()[0] < few).all()
+        rows.check(rng.random(16).astype(F), top_p=0.9)
