@@ -1092,7 +1092,7 @@ struct Band {
   uint32_t sorted[kBand];
   int32_t sorted_at[kBand];
   double starts[kParts + 1], sums[kParts];  // the band's kept weights before each part, the parts' before the band
-  uint32_t tied[kParts + 1], kept[kParts + 1];  // (and how many of its equals of the line, and how many it keeps)
+  uint32_t tied[kParts + 1], any[kParts];  // (and how many of its equals of the line; whether the part keeps one of its keys)
 };
 
 // the search of a wide row, its first round done (the histogram is brought into m)
@@ -1162,7 +1162,7 @@ __global__ __launch_bounds__(kThreads) void end_kernel(Sample a, Split sp, doubl
     b.keys[i] = i < n && i < kBand ? wide.keys[i] : 0u;
     b.at[i] = i < n && i < kBand ? (int32_t)wide.at[i] : INT32_MAX;
   }
-  if (threadIdx.x < kParts) b.sums[threadIdx.x] = wide.sums[threadIdx.x];
+  if (threadIdx.x < kParts) b.sums[threadIdx.x] = wide.sums[threadIdx.x], b.any[threadIdx.x] = 0;
   __syncthreads();
   f.some = b.keys[0];  // (a bin of one key)
   const bool fits = n <= kBand;  // (else equal ones by the thousand: the whole row again)
@@ -1196,16 +1196,15 @@ __global__ __launch_bounds__(kThreads) void end_kernel(Sample a, Split sp, doubl
     const double x = w.of(key);
     const bool in = there && (key > kept.t || (key == kept.t && tied < kept.ties)) && (x >= set.min_p || key == w.top);
     const double before = sum_before(in ? x : 0.0, m.sums, total);
-    uint32_t all;
-    const uint32_t kept_before = sum_before((uint32_t)(in && x > 0.0), m.part2, all);
     // what comes before each part
     const int32_t per = part_of(a.vocab);
     const int part = there ? b.sorted_at[threadIdx.x] / per : kParts;
     const int part_before = threadIdx.x && (int)threadIdx.x <= n ? b.sorted_at[threadIdx.x - 1] / per : -1;
+    if (in && x > 0.0) b.any[part] = 1;
     if ((int)threadIdx.x <= n)
-      for (int q = part_before + 1; q <= part; q++) b.starts[q] = before, b.tied[q] = tied, b.kept[q] = kept_before;
+      for (int q = part_before + 1; q <= part; q++) b.starts[q] = before, b.tied[q] = tied;
     if (n == kBand && threadIdx.x == kThreads - 1)
-      for (int q = part + 1; q <= kParts; q++) b.starts[q] = total, b.tied[q] = ties, b.kept[q] = all;
+      for (int q = part + 1; q <= kParts; q++) b.starts[q] = total, b.tied[q] = ties;
     __syncthreads();
 #pragma unroll 1
     for (int q = 0; q < kParts; q++) total += b.sums[q];
@@ -1215,9 +1214,8 @@ __global__ __launch_bounds__(kThreads) void end_kernel(Sample a, Split sp, doubl
     bool passed = false;
 #pragma unroll 1
     for (int q = 0; q < kParts; q++) {
-      // (by count: two sums over the same keys may differ by a rounding)
-      const bool any = b.sums[q] > 0.0 || b.kept[q + 1] != b.kept[q];
-      if (!passed && any) which = q, lead = run + b.starts[q], passed = run + b.sums[q] + b.starts[q + 1] > set.u * total;
+      // (not by starts' difference: two sums over the same keys may differ by a rounding)
+      if (!passed && (b.sums[q] > 0.0 || b.any[q])) which = q, lead = run + b.starts[q], passed = run + b.sums[q] + b.starts[q + 1] > set.u * total;
       run += b.sums[q];
     }
     from = min(which * per, a.vocab), to = min(from + per, a.vocab);
