@@ -177,9 +177,8 @@ class Forward:
         if needed < 0:
             check(needed)
         needed = max(needed, extra)
+        # (what is made while a step is captured is the graph's memory, and stays as long as this object)
         if self.work.numel() < needed:
-            if torch.cuda.is_current_stream_capturing():
-                raise ValueError("refused: a step is captured after one of its sizes has run, which makes its workspace")
             if self.work.numel():
                 self.older.append(self.work)
                 needed = max(needed, 2 * self.work.numel())
@@ -193,8 +192,6 @@ class Forward:
         normed, both = None, {}
         if adapters is not None:
             if self.normed is None:
-                if torch.cuda.is_current_stream_capturing():
-                    raise ValueError("refused: a step with adapters is captured after one has run, which makes its buffer")
                 self.normed = torch.empty_like(self.y)
             normed = self.normed[:count]
             both = dict(y=normed, both=True)

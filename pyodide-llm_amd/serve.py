@@ -1,8 +1,7 @@
 """Requests served step by step over a Forward's paged cache, with all that a step needs on the device: the new tokens' places and
 pages (hq_batch_plan_ex), their embeddings (hq_embed_ex), the layers with the requests' adapters, the classifier for each
-request's last token, and the tokens drawn from the logits (hq_sample_ex).  Nothing comes back to the host inside a step: a step of
-the same sizes can be captured into a graph once it has run, and replayed on new contents of its tensors (`longest` is the captured
-step's).  A Serving has its Forward to itself: the pages that it gives out are the Forward's.
+request's last token, and the tokens drawn from the logits (hq_sample_ex).  Nothing comes back to the host inside a step: a step
+can be captured into a graph and replayed on new contents of its tensors (`longest` is the captured step's).  A Serving has its Forward to itself: the pages that it gives out are the Forward's.
 """
 from . import check, library
 from .cache import Batch, Pool

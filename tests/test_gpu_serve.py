@@ -222,6 +222,45 @@ def test_a_captured_step_keeps_its_workspace(pkg):
     assert other.forward.work.numel() > was and all((t == 255).all() for t in held)
 
 
+@pytest.mark.parametrize("kind", [None, "bfloat16"])
+def test_a_first_step_is_captured(pkg, kind):
+    """a step whose workspace is not there yet makes it in its graph; larger steps between its replays"""
+    import torch
+    from pyodide_llm_amd import adapters, checkpoint, forward
+    rng = np.random.default_rng(8)
+    ck = checkpoint.Checkpoint(checkpoints.write((256, 768, 2, 4, 2, 300, 64), "int8", rng)[0])
+    beside = adapters.Adapters(factors(torch, ck, rng, 2, 64, ("wq", "w2"), getattr(torch, kind))) if kind else None
+    eager, other = (forward.Forward(ck, tokens=1500, sequences=2, pages=64, width=32, page=64) for _ in range(2))
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    table, which = torch.arange(64, dtype=torch.int32, device="cuda").view(2, 32), ints(1, 0)
+    starts, lengths, x = ints(0, 1, 2), ints(1, 1), torch.zeros(2, 256, device="cuda")
+    extra = (None, beside, which) if kind else ()
+    eager.step(torch.zeros_like(x), starts, lengths, table, 1, *extra)  # (the library has run; `other` has not)
+    torch.cuda.synchronize()
+    assert other.work.numel() == 0
+    stream, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        taken = other.step(x, starts, lengths, table, 1, *extra)
+    first = other.work
+    held = np.zeros(2, int)
+    for many in (0, 700, 3, 1100):
+        held += 1
+        new = torch.from_numpy(rng.standard_normal((2, 256)).astype(F)).cuda()
+        x.copy_(new)
+        lengths.copy_(ints(*held))
+        want = eager.step(new, starts, lengths, table, 1, *extra).clone()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(want, taken)
+        if many:
+            rows = torch.from_numpy(rng.standard_normal((many + 1, 256)).astype(F)).cuda()
+            held += [many, 1]
+            got = [m.step(rows.clone(), ints(0, many, many + 1), ints(*held), table, many, *extra) for m in (eager, other)]
+            assert torch.equal(*got)
+    assert other.work is not first and any(t is first for t in other.older)
+
+
 def test_adapters_of_one_and_two_projections(pkg):
     """a model whose attention needs less workspace than the adapters, of which one or two projections may need more than three"""
     import torch
