@@ -56,7 +56,8 @@ class Forward:
         self.caches = [Cache(*(t.data_ptr() for t in held), FORMS[form], pages, page, s.kv_heads, s.head_size)
                        for held in self.held]
         self.work = torch.empty(0, dtype=torch.uint8, device=device)
-        self.older = []  # (workspaces that were too small: a captured step may still use them)
+        self.captured = False  # (whether a captured step uses this workspace: it is kept then)
+        self.older = []  # (such workspaces that were too small for a later step)
         self.normed = None  # (a norm's values beside the readied ones: where adapters read them)
         half = torch.arange(0, s.head_size, 2, device=device, dtype=torch.float64) / s.head_size
         angles = torch.arange(width * page, device=device, dtype=torch.float64)[:, None] * theta ** -half
@@ -178,11 +179,14 @@ class Forward:
             check(needed)
         needed = max(needed, extra)
         # (what is made while a step is captured is the graph's memory, and stays as long as this object)
+        capturing = torch.cuda.is_current_stream_capturing()
         if self.work.numel() < needed:
-            if self.work.numel():
+            if self.captured or capturing:
                 self.older.append(self.work)
-                needed = max(needed, 2 * self.work.numel())
-            self.work = torch.empty(needed, dtype=torch.uint8, device=x.device)
+            else:
+                self.work.record_stream(stream)  # (it may be another stream's)
+            self.work, self.captured = torch.empty(needed, dtype=torch.uint8, device=x.device), False
+        self.captured = self.captured or capturing
         if at is None:
             # a token's position: its place before its sequence's end
             rows = torch.arange(count, device=x.device, dtype=torch.int32)

@@ -261,6 +261,22 @@ def test_a_first_step_is_captured(pkg, kind):
     assert other.work is not first and any(t is first for t in other.older)
 
 
+def test_workspaces_are_what_steps_need(pkg):
+    """a workspace that no captured step uses is not kept, and none is larger than a step needed"""
+    import torch
+    from pyodide_llm_amd import checkpoint, forward
+    rng = np.random.default_rng(9)
+    ck = checkpoint.Checkpoint(checkpoints.write((256, 768, 1, 4, 2, 300, 64), "int8", rng)[0])
+    model = forward.Forward(ck, tokens=1500, sequences=1, pages=32, width=32, page=64)
+    table, most = torch.arange(32, dtype=torch.int32, device="cuda")[None], 0
+    for many in (1, 500, 600, 1500, 20):
+        starts, lengths = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([0, many], [many]))
+        model.step(torch.zeros(many, 256, device="cuda"), starts, lengths, table, many)
+        batch = pkg.cache.Batch(starts.data_ptr(), lengths.data_ptr(), table.data_ptr(), 1, many, many, 32)
+        most = max(most, pkg.library().hq_attention_work_bytes(model.caches[0], batch, 4))
+        assert model.work.numel() == most and not model.older
+
+
 def test_adapters_of_one_and_two_projections(pkg):
     """a model whose attention needs less workspace than the adapters, of which one or two projections may need more than three"""
     import torch
