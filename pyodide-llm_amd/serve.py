@@ -17,6 +17,8 @@ class Serving:
         torch, n, device = forward.torch, forward.sequences, forward.y.device
         if n > forward.tokens:
             raise ValueError(f"refused: {n} places over steps of {forward.tokens} tokens")
+        if adapters is not None:  # (a step would refuse them with its places and pages taken)
+            forward.adapters_fit(adapters, forward.tokens)
         self.forward, self.torch, self.lib, self.adapters = forward, torch, library(), adapters
 
         def ints(count, value=0):
