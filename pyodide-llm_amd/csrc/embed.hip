@@ -45,7 +45,7 @@ constexpr int64_t row_bytes(int packing, int64_t dim) {
 template <int PACKING>
 __global__ __launch_bounds__(256) void embed_kernel(Embed e, int32_t group_shift) {
   const int32_t q = blockIdx.x * 256 + threadIdx.x;
-  if (4 * q >= e.dim) return;
+  if (q >= (e.dim >> 2)) return;
   for (int64_t t = blockIdx.y; t < e.count; t += gridDim.y) {
     float4 *to = (float4 *)(e.out + t * e.out_stride) + q;
     const int32_t id = e.ids[t];
@@ -64,8 +64,8 @@ __global__ __launch_bounds__(256) void embed_kernel(Embed e, int32_t group_shift
 
 // int8 rows that are no whole dwords (groups of 1 or 2): a thread a weight
 __global__ __launch_bounds__(256) void embed_odd_kernel(Embed e, int32_t group_shift) {
-  const int32_t i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= e.dim) return;
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x;  // (a row may end within 256 of 2^31)
+  if (i >= (uint32_t)e.dim) return;
   for (int64_t t = blockIdx.y; t < e.count; t += gridDim.y) {
     const int32_t id = e.ids[t];
     float x = 0.0f;
@@ -82,7 +82,7 @@ __global__ __launch_bounds__(256) void embed_odd_kernel(Embed e, int32_t group_s
 hipError_t launch_embed(int32_t packing, const Embed &e, int32_t group, hipStream_t s) {
   if (e.count <= 0 || e.dim <= 0) return hipSuccess;
   const int32_t shift = __builtin_ctz(group), lanes = e.dim % 4 ? e.dim : e.dim / 4;
-  const dim3 grid((uint32_t)((lanes + 255) / 256), (uint32_t)(e.count < 65535 ? e.count : 65535));
+  const dim3 grid((uint32_t)(((int64_t)lanes + 255) / 256), (uint32_t)(e.count < 65535 ? e.count : 65535));
   const auto kernel = e.dim % 4 ? embed_odd_kernel : packing == kPackInt8 ? embed_kernel<kPackInt8>
                     : packing == kPackInt6 ? embed_kernel<kPackInt6> : packing == kPackTernary ? embed_kernel<kPackTernary>
                     : embed_kernel<kPackBinary>;

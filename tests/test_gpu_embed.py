@@ -169,3 +169,24 @@ def test_replayed(pkg, arena):
         torch.cuda.synchronize()
         g.replay()
         assert same_bits(arena.get(out, F, 7 * 256).reshape(7, 256), wanted(rows, ids, 1.5))
+
+
+@pytest.mark.parametrize("dim", [2 ** 31 - 1, 2 ** 31 - 4])
+def test_rows_as_long_as_can_be(pkg, dim):
+    """a row that ends less than a block's values before 2^31, a weight and four a thread"""
+    import torch
+    group, guard = dim & -dim, 1024
+    values = torch.randint(-128, 128, (dim + -dim % 16,), dtype=torch.int8, device="cuda")
+    scales = torch.rand(dim // group, device="cuda")
+    memory = torch.full((dim + 2 * guard,), -7.0, device="cuda")
+    out, ids = memory[guard:], torch.zeros(1, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    lib = pkg.library()
+    assert lib.hq_embed_ex(out.data_ptr(), ids.data_ptr(), values.data_ptr(), scales.data_ptr(), 0, 1, dim, 0.5, 1, 0, None) == 0, \
+        lib.hq_last_error_message()
+    torch.cuda.synchronize()
+    assert (memory[:guard] == -7).all() and (memory[-guard:] == -7).all()
+    for at in range(0, dim, 1 << 28):
+        end = min(at + (1 << 28), dim)
+        want = values[at:end].float().view(-1, group) * scales[at // group:end // group, None] * 0.5
+        assert torch.equal(out[at:end], want.view(-1))
