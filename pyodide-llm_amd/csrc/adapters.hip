@@ -300,7 +300,7 @@ __global__ __launch_bounds__(256) void token_down_kernel(Adapters a, Batch b, in
   const float *x = (const float *)(a.x + t * a.x_stride);
   const char *f = a.target[target].a + 2 * ((int64_t)w * a.rank + r) * a.n;
   float sum[kEach] = {0.f, 0.f, 0.f, 0.f};
-  for (int32_t i = lane * 8; i < a.n; i += 512) {
+  for (uint32_t i = lane * 8; i < (uint32_t)a.n; i += 512) {  // (a single token's row may end within 512 of 2^31)
     const float4 x0 = *(const float4 *)(x + i), x1 = *(const float4 *)(x + i + 4);
     const float e[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
 #pragma unroll

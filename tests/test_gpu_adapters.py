@@ -291,3 +291,27 @@ def test_most_tokens(pkg):
         # (n and rank products and sums, a rounding each at most)
         far = (e.abs() @ a.abs().t()) @ b.abs().t() * (n + rank + 3) * 2.0 ** -24
         assert ((y[rows_of].double() - want).abs() <= far).all(), first
+
+
+def test_a_row_as_long_as_can_be(pkg):
+    """a token of 2^31 - 32 values (more tokens' stride would pass 2^31): factors of 32 GiB, 0 but for both ends"""
+    import torch
+    lib, n, rank, rows, ends = pkg.library(), 2 ** 31 - 32, 8, 5, 1024
+    a, x = torch.zeros(1, rank, n, dtype=torch.float16, device="cuda"), torch.zeros(1, n, device="cuda")
+    for part in (slice(0, ends), slice(n - ends, n)):
+        a[0, :, part] = torch.randn(rank, ends, device="cuda").half()
+        x[0, part] = torch.randn(ends, device="cuda")
+    b, y = torch.randn(1, rows, rank, device="cuda").half(), torch.full((rows + 8,), -9.0, device="cuda")
+    starts, which = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([0, 1], [0]))
+    need = lib.hq_adapters_work_bytes(1, rank, 1)
+    work = torch.empty(need, dtype=torch.uint8, device="cuda")
+    target = pkg.adapters.Target(a.data_ptr(), b.data_ptr(), None, y.data_ptr(), rows, 0, 0)
+    batch = pkg.cache.Batch(starts.data_ptr(), None, None, 1, 1, 0, 0)
+    torch.cuda.synchronize()
+    assert lib.hq_adapters_ex(target, 1, x.data_ptr(), 0, n, rank, 1, 1, None, which.data_ptr(), batch, work.data_ptr(), need,
+                              torch.cuda.current_stream().cuda_stream) == 0, lib.hq_last_error_message()
+    torch.cuda.synchronize()
+    both = lambda t: torch.cat([t[..., :ends], t[..., n - ends:]], -1).double()  # noqa: E731
+    low, size = both(x) @ both(a[0]).t(), both(x).abs() @ both(a[0]).abs().t()
+    want, far = low @ b[0].double().t(), size @ b[0].double().abs().t() * (2 * ends + rank + 3) * 2.0 ** -24
+    assert ((y[:rows].double() - want).abs() <= far).all() and (y[rows:] == -9).all()
