@@ -21,9 +21,22 @@ comes before and after the layers (serve.py runs them all).
 The forward pass of the reference (src/runtime/forward/engine.ts) takes one sequence and a cache as long as the model's
 sequence; its products are these, the operators between them are its own.
 """
+import functools
+
 from . import HQ_PACK, check, jobs, library
 from .adapters import Target
 from .cache import FORMS, READY, READY_BYTES, Batch, Cache, shapes
+
+
+def on_its_device(method):
+    """`method` with the device of its object's buffers as the current one, on which the library's calls run"""
+    @functools.wraps(method)
+    def run(self, *args, **kwargs):
+        if self.device.type != "cuda":  # (nothing runs on the host's memory)
+            return method(self, *args, **kwargs)
+        with self.torch.cuda.device(self.device):
+            return method(self, *args, **kwargs)
+    return run
 
 
 class Forward:
@@ -46,6 +59,7 @@ class Forward:
         self.q, self.att = floats(tokens, s.heads, s.head_size), floats(tokens, s.heads, s.head_size)
         self.k, self.v = floats(tokens, s.kv_heads, s.head_size), floats(tokens, s.kv_heads, s.head_size)
         self.given, self.y = floats(tokens, s.dim), floats(tokens, s.dim)
+        self.device = self.y.device
         self.gate, self.up = floats(tokens, s.hidden_dim), floats(tokens, s.hidden_dim)
         self.xq = torch.empty(tokens * max(self.frames.values()), dtype=torch.uint8, device=device)
         # a layer's cache is (k, v, ks, vs); no value is needed to start with
@@ -102,6 +116,7 @@ class Forward:
                 raise ValueError(f"refused: {name}'s factors of {tuple(a.shape)} and {tuple(b.shape)} on {a.device}")
         return self.lib.hq_adapters_work_bytes(3, adapters.rank, count)
 
+    @on_its_device
     def embed(self, ids, x, scale=1.0):
         """x (float32 rows) = the embeddings of ids (int32), both on the device; an id that is none gives zeros"""
         m, s = self.ck.matrices["token_embedding_table"], self.ck.shape
@@ -112,6 +127,7 @@ class Forward:
         check(self.lib.hq_embed_ex(x.data_ptr(), ids.data_ptr(), m.values, m.scales, HQ_PACK[m.kind], s.vocab, s.dim, scale,
                                    x.shape[0], 4 * s.dim, self.torch.cuda.current_stream().cuda_stream))
 
+    @on_its_device
     def logits(self, y, out):
         """out[i] = the classifier's logits of y[i], a final norm's row whose outlier channels are set to 0 on the way, as
         Checkpoint.classify's are: one product for all rows, the channels a row after another"""
@@ -142,6 +158,7 @@ class Forward:
         pairs = self.torch.view_as_complex(t.view(*t.shape[:-1], -1, 2))
         pairs.mul_(self.turn[at][:, None, :])
 
+    @on_its_device
     def step(self, x, starts, lengths, table, longest=0, at=None, adapters=None, which=None):
         """x: the new tokens' embeddings (float32, on the device), which become the residual stream; starts, lengths and
         table: hq_batch's, int32 on the device, lengths with the new tokens among them; longest: the most new tokens that a

@@ -5,6 +5,7 @@ can be captured into a graph and replayed on new contents of its tensors (`longe
 """
 from . import check, library
 from .cache import Batch, Pool
+from .forward import on_its_device
 
 
 class Serving:
@@ -19,7 +20,7 @@ class Serving:
             raise ValueError(f"refused: {n} places over steps of {forward.tokens} tokens")
         if adapters is not None:  # (a step would refuse them with its places and pages taken)
             forward.adapters_fit(adapters, forward.tokens)
-        self.forward, self.torch, self.lib, self.adapters = forward, torch, library(), adapters
+        self.forward, self.torch, self.lib, self.adapters, self.device = forward, torch, library(), adapters, device
 
         def ints(count, value=0):
             return torch.full((count,), value, dtype=torch.int32, device=device)
@@ -40,6 +41,7 @@ class Serving:
         self.tokens, self.chance = ints(n, -1), floats(n, 0.0)
         self.work = torch.empty(self.lib.hq_sample_work_bytes(n, forward.ck.shape.vocab), dtype=torch.uint8, device=device)
 
+    @on_its_device
     def step(self, ids, fresh, u, longest=0):
         """ids (int32): the step's new tokens, place after place; fresh (int32): how many each place has of them; u (float32): a
         number of [0, 1) a place; longest: the most that one has (0: not known).  Returns each place's next token (int32, a buffer
@@ -70,6 +72,7 @@ class Serving:
         self.tokens.masked_fill_(self.starts[1:] == self.starts[:-1], -1)
         return self.tokens
 
+    @on_its_device
     def finish(self, done):
         """done (bool, on the device, a place each): these requests end; their pages go back to the pool, their places are empty"""
         torch, f = self.torch, self.forward

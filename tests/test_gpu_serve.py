@@ -277,6 +277,43 @@ def test_workspaces_are_what_steps_need(pkg):
         assert model.work.numel() == most and not model.older
 
 
+def test_steps_run_on_their_device(pkg, monkeypatch):
+    """every call of the library is made with the buffers' device as the current one, whichever the caller's is"""
+    import torch
+    from pyodide_llm_amd import checkpoint, forward, serve
+    rng = np.random.default_rng(10)
+    ck = checkpoint.Checkpoint(checkpoints.write((256, 768, 1, 4, 2, 300, 64), "int8", rng)[0])
+    model = forward.Forward(ck, tokens=4, sequences=2, pages=4, width=2, page=16)
+    serving = serve.Serving(model)
+    inside, calls = [], []
+
+    class Entered(torch.cuda.device):
+        def __enter__(self):
+            inside.append(self.idx)
+            return super().__enter__()
+
+        def __exit__(self, *error):
+            inside.pop()
+            return super().__exit__(*error)
+
+    class Watched:
+        def __getattr__(self, name):
+            calls.append((name, list(inside)))
+            return getattr(pkg.library(), name)
+
+    monkeypatch.setattr(torch.cuda, "device", Entered)
+    model.lib = serving.lib = Watched()
+    ids, ones = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([1, 2], [1, 1]))
+    serving.step(ids, ones, torch.rand(2, device="cuda"), 1)
+    serving.finish(torch.ones(2, dtype=torch.bool, device="cuda"))
+    x = torch.empty(2, 256, device="cuda")
+    model.embed(ids, x)
+    model.logits(model.step(x, serving.starts, ones, serving.table, 1), torch.empty(2, 300, device="cuda"))
+    names = {name for name, _ in calls}
+    assert {"hq_batch_plan_ex", "hq_embed_ex", "hq_attention_ex", "hq_sample_ex", "hq_pages_give_ex"} <= names
+    assert all(at and at[-1] == model.y.device.index for _, at in calls)
+
+
 def test_adapters_of_one_and_two_projections(pkg):
     """a model whose attention needs less workspace than the adapters, of which one or two projections may need more than three"""
     import torch
