@@ -378,7 +378,8 @@ typedef struct hq_pool {
   int32_t pages, page;
 } hq_pool;
 /* What a step's new tokens make of a batch, on the device: sequence s has held[s] positions and gets fresh[s] new tokens
- * (negative numbers count as 0; what would pass the batch's `tokens` rows is left out, from the last sequences).  Written:
+ * (negative numbers count as 0, held of more than 2^30 + 2^25 as that; what would pass the batch's `tokens` rows is left out, from
+ * the last sequences).  Written:
  *   batch->starts    sums of the new tokens before each sequence, and after the last
  *   batch->lengths   held + new (may be held)
  *   batch->table     the pages of positions that begin on a new page, from the top of the stack, in order of sequences and
@@ -425,8 +426,8 @@ int32_t hq_adapters_ex(const hq_adapter *targets, int32_t count, const void *x, 
  *   the first i, by rising index, whose kept w up to and with it are more than u times the sum of all kept
  * into tokens (int32), and w_i over that sum into chance (float32, may be NULL).  -infinity and NaN logits are never drawn (a row
  * of nothing else: token -1, chance 0); +infinity ones have all the weight.  temperature, top_p, min_p and u (float32) and top_k
- * (int32) are a number a row in device memory; each but u may be NULL (temperature 1, the others off), and NaN is off as well.  u below 0 or NaN counts as
- * 0, and where u is 1 or more the last kept token is drawn.  Sums behind top_p are of w in steps of 2^-42 or finer, in any order; the last sum
+ * (int32) are a number a row in device memory; each but u may be NULL (temperature 1, the others off); a NaN of the others is off as well, a NaN temperature is
+ * one not above 0.  u below 0 or NaN counts as 0, and where u is 1 or more the last kept token is drawn.  Sums behind top_p are of w in steps of 2^-42 or finer, in any order; the last sum
  * is in 64 bits by rising index: the same numbers always draw the same token.  logits and stride 4-byte aligned; vocab at most
  * 2^20, rows too.  work: hq_sample_work_bytes bytes (-1: bad arguments), 256-byte aligned, of any content, as hq_attention_ex's. */
 int64_t hq_sample_work_bytes(int32_t rows, int32_t vocab);

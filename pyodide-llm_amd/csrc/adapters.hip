@@ -6,8 +6,10 @@
 // waves (and, for few tokens, blocks) share the n values and add what they have in a fixed order; then each projection's rows, 16
 // tokens and some rows a wave.  Factors widen to float32 exactly, so all that is rounded are float32's products and sums.
 // Measured: 2048 tokens of a sequence, rank 64, n and rows 4096: down 22.6 us, up 27.4 (x, from and y are 100 MB, 20 us at a large
-// copy's 5.1 TB/s); five prompts of rank 32, n 2048, two projections of 8192 rows: 15.9 and 41.0.  Loads whose addresses follow
-// from the batch's arrays, and LDS barriers, bound them; four times the blocks, or rows of 16 x 128 bytes straight from memory, gain nothing.
+// copy's 5.1 TB/s); five prompts of rank 32, n 2048, two projections of 8192 rows: 15.9 and 41.0.  Four tiles of low
+// numbers take 142 registers and 66 KB of LDS, one block a compute unit, whose barriers nobody covers: its waves wait to issue 54 % of
+// their time (after a barrier all begin their matrix instructions, which are busy 30 %) and for loads and barriers 33 %.  The rows'
+// waves wait for loads 59 to 73 %.  Four times the blocks, or rows of 16 x 128 bytes straight from memory, gain nothing.
 // Where the batch says that each sequence has one token, a tile would be empty but for one: tokens then have kernels of their own.
 #include <algorithm>
 #include <type_traits>

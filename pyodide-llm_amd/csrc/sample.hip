@@ -16,8 +16,8 @@
 // weights tallied and its line found by 16 blocks (tally, wide), and drawn by one (end); other rows leave them at once (1.6 to
 // 4 us a launch).  One block for such a row takes as long however few there are.
 //
-// Measured: 256 rows of 128256 with their own settings: hand 49.4 us (131 MB, 2.7 TB/s: a key's compares and the emission bound
-// it), join 29.9 (the list's rounds, a barrier or two each), tally 13.2, wide 16.2, end 26.9 (rows whose line is low); 32 rows: 12.2, 25.8, 4.6, 4.6,
+// Measured: 256 rows of 128256 with their own settings: hand 49.4 us (131 MB, 2.7 TB/s: its waves wait for loads
+// half of their time and to issue a third), join 29.9 (waits, for barriers and LDS, are 63 % of it), tally 13.2, wide 16.2, end 26.9 (rows whose line is low); 32 rows: 12.2, 25.8, 4.6, 4.6,
 // 3.9.  A block a row over everything: 505 us and 373.
 #include <algorithm>
 #include <cmath>
@@ -36,7 +36,7 @@ constexpr int kHeld = 8192;              // the longest row that a block takes a
 constexpr int kGrain = 64;               // neighbouring logits that the first launch gives to one wave
 constexpr int kGrains = kBatch * kStep / kGrain;
 constexpr int kHand = 192;               // logits that a wave of the first launch can hand on
-constexpr int kList = 7680;              // and what the second launch takes of a row (two blocks a compute unit)
+constexpr int kList = 7680;              // and what the second launch takes of a row (62 KB of its 115: one block a compute unit)
 constexpr int kFew = 64;                 // keys that one wave finishes with
 constexpr uint32_t kLowest = 0x00800000u;  // the key of the lowest finite number
 
